@@ -357,6 +357,104 @@ st_status st_knn_synth_store_2bit(uint64_t seed, int64_t row0, int64_t n, int64_
 st_status st_knn_synth_keys_f32(uint64_t seed, int64_t row0, int64_t n, int64_t d, float *keys,
                                 st_stream stream);
 
+/* ---- A decoding step in 4 bits -------------------------------------------
+ * No reference counterpart: what running the trained model token by token needs
+ * beside the training path, weights and cached keys and values held as the 2-bit
+ * store holds its keys (codes and f32 scales).
+ *
+ * The format: a group of values x has lo = min x, hi = max x and scale =
+ * f32((hi - lo) / 15); value i is held as code = round_half_even((x - lo) * 15 /
+ * (hi - lo)), decided in 64 bits (0 where hi = lo), and stands for scale * code +
+ * lo.  Code i is at byte i / 2, bits 4 (i % 2); a group's scale and lo are two
+ * floats side by side.  A group that holds a NaN or an infinity has scale = lo =
+ * NaN and codes 0: every value of it reads as NaN.
+ *
+ * Buffers of activations and weights have one of three element types (`dtype`);
+ * rows may be any number of elements apart and need the alignment of their
+ * elements only (16-byte aligned rows are read faster).  Sums, softmax statistics
+ * and scales are f32; outputs are rounded once, to nearest even.  None of these
+ * calls uses the scratch arena. */
+#define ST_F32 0
+#define ST_F16 1
+#define ST_BF16 2
+
+/* Weights x [n, k] (rows x_stride elements apart) in groups of `group` (32, 64
+ * or 128, a divisor of k) along a row: codes [n, k / 2], 4-byte aligned, and
+ * scales [n, k / group, 2], 8-byte aligned.  values (NULL: not wanted) [n, k] in
+ * x's type gets what the codes stand for, for a straight-through gradient.  It
+ * may not overlap x. */
+st_status st_quantize_4bit(const void *x, int32_t dtype, int64_t n, int64_t k, int64_t x_stride,
+                           int64_t group, uint8_t *codes, float *scales, void *values,
+                           st_stream stream);
+
+/* out[i, j] = sum over l of x[i, l] w[j, l] + bias[j] (f32, NULL: none), then
+ * ReLU where relu != 0, for m rows x [m, k] and weights w [n, k] as
+ * st_quantize_4bit writes them (codes 16-byte aligned): the Linear layer
+ * x @ w^T of a decoding step.  m, k <= 2^20, n <= 2^31; every 16 rows read the weights
+ * once, so large batches belong in st_matmul over dequantised weights.  out may
+ * not overlap x. */
+st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int64_t k, int64_t x_stride,
+                         const uint8_t *codes, const float *scales, int64_t group, int64_t n,
+                         const float *bias, int32_t relu, void *out, int64_t out_stride,
+                         st_stream stream);
+
+/* The paged cache of one layer: codes [pages, hkv, page, hd / 2] and scales
+ * [pages, hkv, page, 2] for the keys and for the values, 16-byte aligned; a
+ * token's head vector is one group of the 4-bit format.  hd is 32, 64, 96, 128,
+ * 192 or 256; page a power of two from 16 to 1024 tokens; hq a multiple of hkv.
+ * Token p of sequence s is in page table[s, p / page] (table [nseq, max_pages]),
+ * slot p % page; entries that no call needs are not read.
+ *
+ * Appends n tokens: token t belongs at position pos[t] of sequence seq[t].  Its
+ * queries q [n, hq, hd] (NULL: none) and keys k [n, hkv, hd] have their first
+ * `rot` components rotated by the angles pos[t] inv_freq[i], i < rot / 2, taken
+ * in 64 bits: the pairs are (i, i + rot / 2), or (2i, 2i + 1) where interleaved
+ * != 0; rot 0 (inv_freq may be NULL) rotates nothing.  q_out [n, hq, hd] gets the
+ * rotated queries; keys (rotated, in f32) and values v are quantised into the
+ * cache; k_out and v_out [n, hkv, hd] (NULL: not wanted) get what the cache now
+ * holds for them.  A token's heads are contiguous, tokens q_stride, k_stride and
+ * v_stride elements apart (views of a fused projection's output).  A token whose
+ * sequence is not in 0..nseq (padding), whose position is negative or past the
+ * table, or whose page is not in 0..pages writes nothing at all.  No two tokens
+ * of a call may name the same place, and the outputs may not overlap the inputs. */
+st_status st_kv_append_4bit(const void *q, const void *k, const void *v, int32_t dtype, int64_t n,
+                            int64_t hq, int64_t hkv, int64_t hd, int64_t q_stride,
+                            int64_t k_stride, int64_t v_stride, const int32_t *seq,
+                            const int32_t *pos, int64_t nseq, const int32_t *table,
+                            int64_t max_pages, int64_t pages, int64_t page, const float *inv_freq,
+                            int64_t rot, int32_t interleaved, uint8_t *k_codes, float *k_scales,
+                            uint8_t *v_codes, float *v_scales, void *q_out, void *k_out,
+                            void *v_out, st_stream stream);
+
+/* Bytes of device memory that st_kv_attention_4bit needs for these sizes (0:
+ * none): partial results where a sequence's keys are shared among workgroups. */
+int64_t st_kv_attention_4bit_bytes(int64_t n, int64_t nseq, int64_t hq, int64_t hkv, int64_t hd,
+                                   int64_t max_pages, int64_t page);
+
+/* Attention of rows q [n, hq, hd] (rotated, q_stride elements apart) over the
+ * cache: out[t, h] = softmax(scale q k^T) v with head h reading key head
+ * h / (hq / hkv).  Sequence s has rows q_start[s] .. q_start[s + 1] (q_start [nseq
+ * + 1], ascending) and kv_len[s] cached tokens, its own rows' among them: the
+ * rows are its last tokens.  causal: a row sees the tokens up to its own position
+ * (else all kv_len), and the last `window` of those where window > 0.  one:
+ * softmax1 (a phantom logit 0), as st_softmax.  out [n, hq, hd] in q's type; lse
+ * [n, hq] f32 (NULL: not wanted) the log-sum-exp of the scaled scores, the
+ * phantom's among them.  A row that sees no token gets 0 and -inf (softmax1: 0);
+ * masked tokens, and what lies behind a sequence's end, never reach a result,
+ * whatever they hold; a row that sees a token whose page is not in 0..pages, or one
+ * past the table, gets NaN.  Rows before q_start[0] and from q_start[nseq] on are left
+ * as they were.  The lengths are read on the device: a captured graph follows them.  work:
+ * st_kv_attention_4bit_bytes of device memory, 16-byte aligned, the call's own until its
+ * work on `stream` is done.  out may not overlap q. */
+st_status st_kv_attention_4bit(const void *q, int32_t dtype, int64_t n, int64_t hq, int64_t hkv,
+                               int64_t hd, int64_t q_stride, const int32_t *q_start,
+                               const int32_t *kv_len, int64_t nseq, const int32_t *table,
+                               int64_t max_pages, int64_t pages, int64_t page,
+                               const uint8_t *k_codes, const float *k_scales,
+                               const uint8_t *v_codes, const float *v_scales, float scale,
+                               int32_t causal, int64_t window, int32_t one, void *out, float *lse,
+                               void *work, int64_t work_bytes, st_stream stream);
+
 /* ---- Device ceilings (benchmark support, no reference counterpart) ------- */
 
 /* The current device's CU count, shader clock and memory clock (kHz) and

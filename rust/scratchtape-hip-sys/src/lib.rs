@@ -37,6 +37,11 @@ pub const ST_ERR_NO_DEVICE: st_status = -4;
 /// Size of the fixed device scratch of `st_matmul_grouped_noalloc`.
 pub const ST_NOALLOC_SCRATCH_BYTES: u32 = 64 << 20;
 
+/// Element types of the 4-bit calls' activations and weights.
+pub const ST_F32: i32 = 0;
+pub const ST_F16: i32 = 1;
+pub const ST_BF16: i32 = 2;
+
 /// `hipStream_t`; null is the default stream.
 pub type st_stream = *mut c_void;
 
@@ -403,6 +408,109 @@ extern "C" {
     ) -> st_status;
     pub fn st_knn_synth_keys_f32(seed: u64, row0: i64, n: i64, d: i64, keys: *mut f32, stream: st_stream)
         -> st_status;
+    // A decoding step in 4 bits (no reference counterpart): the format is described in the header.
+    /// Weights to 4-bit codes with a scale and a lowest value per group.
+    pub fn st_quantize_4bit(
+        x: *const c_void,
+        dtype: i32,
+        n: i64,
+        k: i64,
+        x_stride: i64,
+        group: i64,
+        codes: *mut u8,
+        scales: *mut f32,
+        values: *mut c_void,
+        stream: st_stream,
+    ) -> st_status;
+    /// A Linear layer of 4-bit weights on a few rows.
+    pub fn st_matvec_4bit(
+        x: *const c_void,
+        dtype: i32,
+        m: i64,
+        k: i64,
+        x_stride: i64,
+        codes: *const u8,
+        scales: *const f32,
+        group: i64,
+        n: i64,
+        bias: *const f32,
+        relu: i32,
+        out: *mut c_void,
+        out_stride: i64,
+        stream: st_stream,
+    ) -> st_status;
+    /// Appends rotated keys and values, quantised, to a paged 4-bit cache, and rotates the queries.
+    pub fn st_kv_append_4bit(
+        q: *const c_void,
+        k: *const c_void,
+        v: *const c_void,
+        dtype: i32,
+        n: i64,
+        hq: i64,
+        hkv: i64,
+        hd: i64,
+        q_stride: i64,
+        k_stride: i64,
+        v_stride: i64,
+        seq: *const i32,
+        pos: *const i32,
+        nseq: i64,
+        table: *const i32,
+        max_pages: i64,
+        pages: i64,
+        page: i64,
+        inv_freq: *const f32,
+        rot: i64,
+        interleaved: i32,
+        k_codes: *mut u8,
+        k_scales: *mut f32,
+        v_codes: *mut u8,
+        v_scales: *mut f32,
+        q_out: *mut c_void,
+        k_out: *mut c_void,
+        v_out: *mut c_void,
+        stream: st_stream,
+    ) -> st_status;
+    /// Bytes of `work` that `st_kv_attention_4bit` needs.
+    pub fn st_kv_attention_4bit_bytes(
+        n: i64,
+        nseq: i64,
+        hq: i64,
+        hkv: i64,
+        hd: i64,
+        max_pages: i64,
+        page: i64,
+    ) -> i64;
+    /// Attention of ragged rows over the paged 4-bit cache.
+    pub fn st_kv_attention_4bit(
+        q: *const c_void,
+        dtype: i32,
+        n: i64,
+        hq: i64,
+        hkv: i64,
+        hd: i64,
+        q_stride: i64,
+        q_start: *const i32,
+        kv_len: *const i32,
+        nseq: i64,
+        table: *const i32,
+        max_pages: i64,
+        pages: i64,
+        page: i64,
+        k_codes: *const u8,
+        k_scales: *const f32,
+        v_codes: *const u8,
+        v_scales: *const f32,
+        scale: f32,
+        causal: i32,
+        window: i64,
+        one: i32,
+        out: *mut c_void,
+        lse: *mut f32,
+        work: *mut c_void,
+        work_bytes: i64,
+        stream: st_stream,
+    ) -> st_status;
     // Device ceilings (benchmark support; no reference counterpart).
     pub fn st_device_info(cus: *mut i32, clock_khz: *mut i32, mem_clock_khz: *mut i32, mem_bus_bits: *mut i32)
         -> st_status;

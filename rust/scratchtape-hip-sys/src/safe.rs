@@ -731,6 +731,294 @@ pub fn knn_search_masked_2bit<H: DeviceBuffer + ?Sized>(
     });
 }
 
+/// Element type of the activations and weights of the 4-bit calls.
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+pub enum Dtype {
+    F32,
+    F16,
+    Bf16,
+}
+
+impl Dtype {
+    fn code(self) -> i32 {
+        match self {
+            Dtype::F32 => sys::ST_F32,
+            Dtype::F16 => sys::ST_F16,
+            Dtype::Bf16 => sys::ST_BF16,
+        }
+    }
+
+    /// Panics unless `h` holds `count` elements of this type.
+    fn need<H: DeviceBuffer + ?Sized>(self, h: &H, count: usize, what: &str) {
+        match self {
+            Dtype::F32 => need::<f32, H>(h, count, what),
+            _ => need::<u16, H>(h, count, what),
+        }
+    }
+}
+
+/// Elements that `rows` rows of `width` elements, `stride` apart, span.
+fn span(rows: usize, width: usize, stride: usize) -> usize {
+    if rows == 0 {
+        0
+    } else {
+        add(mul(rows - 1, stride), width)
+    }
+}
+
+/// Weights x [n, k] (rows `x_stride` elements apart) to 4-bit codes [n, k / 2] and (scale, lo) pairs
+/// [n, k / group, 2]; `values`, where given, gets what the codes stand for.
+pub fn quantize_4bit<H: DeviceBuffer + ?Sized>(
+    x: &H,
+    dtype: Dtype,
+    n: usize,
+    k: usize,
+    x_stride: usize,
+    group: usize,
+    codes: &H,
+    scales: &H,
+    values: Option<&H>,
+) {
+    dtype.need(x, span(n, k, x_stride), "quantize_4bit x");
+    need::<u8, H>(codes, mul(n, k) / 2, "quantize_4bit codes");
+    need::<f32, H>(scales, mul(mul(n, k / group.max(1)), 2), "quantize_4bit scales");
+    if let Some(v) = values {
+        dtype.need(v, mul(n, k), "quantize_4bit values");
+    }
+    check(unsafe {
+        sys::st_quantize_4bit(
+            ptr(x),
+            dtype.code(),
+            n as i64,
+            k as i64,
+            x_stride as i64,
+            group as i64,
+            dptr(codes),
+            dptr(scales),
+            values.map_or(std::ptr::null_mut(), |v| dptr(v)),
+            stream(),
+        )
+    });
+}
+
+/// out [m, n] = x [m, k] @ w^T (+ bias, then ReLU) with the 4-bit weights w [n, k].
+pub fn matvec_4bit<H: DeviceBuffer + ?Sized>(
+    x: &H,
+    dtype: Dtype,
+    m: usize,
+    k: usize,
+    x_stride: usize,
+    codes: &H,
+    scales: &H,
+    group: usize,
+    n: usize,
+    bias: Option<&H>,
+    relu: bool,
+    out: &H,
+    out_stride: usize,
+) {
+    dtype.need(x, span(m, k, x_stride), "matvec_4bit x");
+    need::<u8, H>(codes, mul(n, k) / 2, "matvec_4bit codes");
+    need::<f32, H>(scales, mul(mul(n, k / group.max(1)), 2), "matvec_4bit scales");
+    if let Some(b) = bias {
+        need::<f32, H>(b, n, "matvec_4bit bias");
+    }
+    dtype.need(out, span(m, n, out_stride), "matvec_4bit out");
+    check(unsafe {
+        sys::st_matvec_4bit(
+            ptr(x),
+            dtype.code(),
+            m as i64,
+            k as i64,
+            x_stride as i64,
+            ptr(codes),
+            ptr(scales),
+            group as i64,
+            n as i64,
+            bias.map_or(std::ptr::null(), |b| ptr(b)),
+            relu as i32,
+            dptr(out),
+            out_stride as i64,
+            stream(),
+        )
+    });
+}
+
+/// One layer's paged cache of keys and values in 4 bits: codes [pages, heads, page, hd / 2] and
+/// (scale, lo) pairs [pages, heads, page, 2] of each, and the page table [nseq, max_pages].
+pub struct KvCache4bit<'a, H: DeviceBuffer + ?Sized> {
+    pub k_codes: &'a H,
+    pub k_scales: &'a H,
+    pub v_codes: &'a H,
+    pub v_scales: &'a H,
+    pub table: &'a H,
+    pub pages: usize,
+    pub heads: usize,
+    pub page: usize,
+    pub hd: usize,
+    pub nseq: usize,
+    pub max_pages: usize,
+}
+
+impl<'a, H: DeviceBuffer + ?Sized> KvCache4bit<'a, H> {
+    fn check_extents(&self) {
+        let rows = mul(mul(self.pages, self.heads), self.page);
+        for codes in [self.k_codes, self.v_codes] {
+            need::<u8, H>(codes, mul(rows, self.hd) / 2, "KvCache4bit codes");
+        }
+        for scales in [self.k_scales, self.v_scales] {
+            need::<f32, H>(scales, mul(rows, 2), "KvCache4bit scales");
+        }
+        need::<i32, H>(self.table, mul(self.nseq, self.max_pages), "KvCache4bit table");
+    }
+
+    /// Appends n tokens (`seq`, `pos`: their places): q and k rotated by `inv_freq` (`rot` components), k and v
+    /// quantised into the cache. `q`: the queries, their stride and where they go, rotated.
+    pub fn append(
+        &self,
+        q: Option<(&H, usize, &H)>,
+        hq: usize,
+        k: &H,
+        k_stride: usize,
+        v: &H,
+        v_stride: usize,
+        dtype: Dtype,
+        n: usize,
+        seq: &H,
+        pos: &H,
+        inv_freq: Option<&H>,
+        rot: usize,
+        interleaved: bool,
+        k_out: Option<&H>,
+        v_out: Option<&H>,
+    ) {
+        self.check_extents();
+        let width = mul(self.heads, self.hd);
+        if let Some((src, stride, dst)) = q {
+            dtype.need(src, span(n, mul(hq, self.hd), stride), "append q");
+            dtype.need(dst, mul(n, mul(hq, self.hd)), "append q_out");
+        }
+        dtype.need(k, span(n, width, k_stride), "append k");
+        dtype.need(v, span(n, width, v_stride), "append v");
+        need::<i32, H>(seq, n, "append seq");
+        need::<i32, H>(pos, n, "append pos");
+        match inv_freq {
+            Some(f) => need::<f32, H>(f, rot / 2, "append inv_freq"),
+            None => assert!(rot == 0, "append: {} rotated components without inv_freq", rot),
+        }
+        for out in [k_out, v_out].into_iter().flatten() {
+            dtype.need(out, mul(n, width), "append k_out / v_out");
+        }
+        check(unsafe {
+            sys::st_kv_append_4bit(
+                q.map_or(std::ptr::null(), |(src, _, _)| ptr(src)),
+                ptr(k),
+                ptr(v),
+                dtype.code(),
+                n as i64,
+                hq as i64,
+                self.heads as i64,
+                self.hd as i64,
+                q.map_or(0, |(_, stride, _)| stride as i64),
+                k_stride as i64,
+                v_stride as i64,
+                ptr(seq),
+                ptr(pos),
+                self.nseq as i64,
+                ptr(self.table),
+                self.max_pages as i64,
+                self.pages as i64,
+                self.page as i64,
+                inv_freq.map_or(std::ptr::null(), |f| ptr(f)),
+                rot as i64,
+                interleaved as i32,
+                dptr(self.k_codes),
+                dptr(self.k_scales),
+                dptr(self.v_codes),
+                dptr(self.v_scales),
+                q.map_or(std::ptr::null_mut(), |(_, _, dst)| dptr(dst)),
+                k_out.map_or(std::ptr::null_mut(), |o| dptr(o)),
+                v_out.map_or(std::ptr::null_mut(), |o| dptr(o)),
+                stream(),
+            )
+        });
+    }
+
+    /// Bytes of device memory that [`KvCache4bit::attention`] needs for n rows of hq heads.
+    pub fn attention_bytes(&self, n: usize, hq: usize) -> usize {
+        unsafe {
+            sys::st_kv_attention_4bit_bytes(
+                n as i64,
+                self.nseq as i64,
+                hq as i64,
+                self.heads as i64,
+                self.hd as i64,
+                self.max_pages as i64,
+                self.page as i64,
+            ) as usize
+        }
+    }
+
+    /// Attention of rows q [n, hq, hd] over the cache into out [n, hq, hd] (and `lse` [n, hq]).
+    pub fn attention(
+        &self,
+        q: &H,
+        dtype: Dtype,
+        n: usize,
+        hq: usize,
+        q_stride: usize,
+        q_start: &H,
+        kv_len: &H,
+        scale: f32,
+        causal: bool,
+        window: usize,
+        one: bool,
+        out: &H,
+        lse: Option<&H>,
+        work: &H,
+    ) {
+        self.check_extents();
+        dtype.need(q, span(n, mul(hq, self.hd), q_stride), "attention q");
+        dtype.need(out, mul(n, mul(hq, self.hd)), "attention out");
+        need::<i32, H>(q_start, add(self.nseq, 1), "attention q_start");
+        need::<i32, H>(kv_len, self.nseq, "attention kv_len");
+        if let Some(l) = lse {
+            need::<f32, H>(l, mul(n, hq), "attention lse");
+        }
+        check(unsafe {
+            sys::st_kv_attention_4bit(
+                ptr(q),
+                dtype.code(),
+                n as i64,
+                hq as i64,
+                self.heads as i64,
+                self.hd as i64,
+                q_stride as i64,
+                ptr(q_start),
+                ptr(kv_len),
+                self.nseq as i64,
+                ptr(self.table),
+                self.max_pages as i64,
+                self.pages as i64,
+                self.page as i64,
+                ptr(self.k_codes),
+                ptr(self.k_scales),
+                ptr(self.v_codes),
+                ptr(self.v_scales),
+                scale,
+                causal as i32,
+                window as i64,
+                one as i32,
+                dptr(out),
+                lse.map_or(std::ptr::null_mut(), |l| dptr(l)),
+                dptr(work),
+                work.byte_len() as i64,
+                stream(),
+            )
+        });
+    }
+}
+
 /// Waits for the calling thread's stream, then panics if a bounded wait of the grouped f16 kernel (grouped
 /// calls and large single f16 products) gave up since the last check.
 pub fn sync() {

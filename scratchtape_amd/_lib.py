@@ -85,6 +85,13 @@ SIGNATURES = {
     "st_knn_centroid_digit_bytes": [_i64, _i64],
     "st_knn_centroids_prep": [_vp, _i64, _i64, _vp, _vp, _vp, _vp],
     "st_knn_probe": [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp],
+    "st_quantize_4bit": [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp],
+    "st_matvec_4bit": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _vp],
+    "st_kv_append_4bit": [_vp, _vp, _vp, _i32] + 7 * [_i64] + [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i32]
+    + 8 * [_vp],
+    "st_kv_attention_4bit_bytes": 7 * [_i64],
+    "st_kv_attention_4bit": [_vp, _i32] + 5 * [_i64] + [_vp, _vp, _i64, _vp, _i64, _i64, _i64] + 4 * [_vp]
+    + [_f32, _i32, _i64, _i32, _vp, _vp, _vp, _i64, _vp],
     "st_device_info": [_vp, _vp, _vp, _vp],
     "st_peak_mfma": [_i32, _i64, _i32, _vp, _vp],
     "st_peak_read": [_vp, _i64, _i32, _vp, _vp],
@@ -96,7 +103,7 @@ SIGNATURES = {
     "st_version": [],
 }
 _RESTYPES = {"st_last_error": ctypes.c_char_p, "st_version": ctypes.c_char_p, "st_f16_enabled": _i32,
-             "st_knn_centroid_digit_bytes": _i64, "st_knn_split_bytes": _i64}
+             "st_knn_centroid_digit_bytes": _i64, "st_knn_split_bytes": _i64, "st_kv_attention_4bit_bytes": _i64}
 
 _lib = None
 
