@@ -199,28 +199,35 @@ __device__ __forceinline__ h8 as_h8(uint32_t a, uint32_t b, uint32_t c, uint32_t
     return __builtin_bit_cast(h8, x);
 }
 
-// Four code pairs of a word, less 8: a nibble under f16's exponent of 2^10 reads as 1024 + n (or 1024 + 16 n), which one
-// packed f16 operation takes to n - 8 without rounding.
-__device__ __forceinline__ uint32_t lower_less8(uint32_t x) {
-    const h2 y = __builtin_bit_cast(h2, (x & 0x000F000Fu) | 0x64006400u) + h2{(_Float16)-1032.f, (_Float16)-1032.f};
-    return __builtin_bit_cast(uint32_t, y);
-}
-__device__ __forceinline__ uint32_t upper_less8(uint32_t x) {
-    const h2 y = __builtin_bit_cast(h2, (x & 0x00F000F0u) | 0x64006400u);
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(y, h2{(_Float16)0.0625f, (_Float16)0.0625f}, h2{(_Float16)-72.f, (_Float16)-72.f}));
-}
+// Code pairs of a word, less 8: a nibble under f16's exponent of 2^10 reads as 1024 + n (or 1024 + 16 n), which one packed
+// f16 operation takes to n - 8 without rounding.  The masks are held in a scalar register and the exponent in a vector
+// register that the compiler cannot see through, so that masking and setting the exponent is one v_and_or_b32.
+struct Taker {
+    uint32_t lower_mask, upper_mask, exponent;
 
-// 8 codes of a word less 8, in the order 0 4 1 5 2 6 3 7.
-__device__ __forceinline__ h8 codes8(uint32_t w) {
-    return as_h8(lower_less8(w), upper_less8(w), lower_less8(w >> 8), upper_less8(w >> 8));
-}
+    __device__ __forceinline__ Taker() {
+        asm("s_mov_b32 %0, 0x000F000F" : "=s"(lower_mask));
+        asm("s_mov_b32 %0, 0x00F000F0" : "=s"(upper_mask));
+        asm("v_mov_b32 %0, 0x64006400" : "=v"(exponent));
+    }
+    __device__ __forceinline__ uint32_t lower(uint32_t x) const {
+        const h2 y = __builtin_bit_cast(h2, (x & lower_mask) | exponent) + h2{(_Float16)-1032.f, (_Float16)-1032.f};
+        return __builtin_bit_cast(uint32_t, y);
+    }
+    __device__ __forceinline__ uint32_t upper(uint32_t x) const {
+        const h2 y = __builtin_bit_cast(h2, (x & upper_mask) | exponent);
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(y, h2{(_Float16)0.0625f, (_Float16)0.0625f}, h2{(_Float16)-72.f, (_Float16)-72.f}));
+    }
+    // 8 codes of a word in the order 0 4 1 5 2 6 3 7.
+    __device__ __forceinline__ h8 codes8(uint32_t w) const { return as_h8(lower(w), upper(w), lower(w >> 8), upper(w >> 8)); }
+};
 
 template <int HD, int PARTS, int RT>
 __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
     constexpr int NW = HD / 32, NB = blocks_of(HD), WAVE_ROWS = 16 * RT, TILE_ROWS = 4 * WAVE_ROWS, LDO = HD + 4;
     __shared__ float red[4][WAVE_ROWS][LDO];
     __shared__ float2 ml[4][WAVE_ROWS];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const Cache &c = a.c;
     const int share = a.hq / c.hkv, cap = (int)(c.max_pages << c.page_log2);
     const int chunk = chunk_keys(a, share, TILE_ROWS, cap, lane);
@@ -320,8 +327,9 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
             sel[b][i] = 0x0c000c00u | (uint32_t)(4 + byte) << 16 | (uint32_t)byte;
         }
 
+    const Taker take;
     // Pages of the next 32 tiles' halves, a half a lane: -1 one outside the cache, 0 (not looked at) behind the end.
-    int entries = 0;
+    int entries = 0, entries_to = 0;
     auto load_entries = [&](int it) {
         const int key = first_key + (it + (lane >> 1)) * step + 16 * (lane & 1);
         entries = 0;
@@ -331,22 +339,23 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
         }
     };
     auto load_tile = [&](int it, Tile<HD> &t, int &bad) {
-        if ((it & 31) == 0) load_entries(it);
+        if (it >= entries_to) load_entries(it), entries_to = it + 32;
         const int key = first_key + it * step;
-        const int p0 = st::lane_value(entries, 2 * (it & 31)), p1 = st::lane_value(entries, 2 * (it & 31) + 1);
+        const int at = 2 * (it + 32 - entries_to), p0 = st::lane_value(entries, at), p1 = st::lane_value(entries, at + 1);
         bad = (p0 < 0 ? 1 : 0) | (p1 < 0 ? 2 : 0);
         load_half<HD>(c, h, max(p0, 0), key & (c.page - 1), 0, lane, t);
         load_half<HD>(c, h, max(p1, 0), (key + 16) & (c.page - 1), 1, lane, t);
     };
 
-    auto scores = [&](const f4 (&s)[RT][2], const float (&ak)[2][4], const float (&bk)[2][4], bool masked, int key0, int rt,
+    auto scores = [&](auto masked_, const f4 (&s)[RT][2], const float (&ak)[2][4], const float (&bk)[2][4], int key0, int rt,
                       float shift, float (&z)[2][4]) {
+        constexpr bool masked = decltype(masked_)::value;
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 z[i][r] = __builtin_fmaf(ak[i][r], s[rt][i][r] * unscale[rt], __builtin_fmaf(bk[i][r], qsum[rt], shift));
-                if (masked) {
+                if constexpr (masked) {
                     const int key = key0 + 16 * i + r;
                     const bool seen = key <= pos[rt] && (a.window <= 0 || key > pos[rt] - a.window);
                     z[i][r] = seen ? z[i][r] : -INFINITY;
@@ -354,8 +363,9 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
             }
     };
 
-    auto process = [&](const Tile<HD> &t, int it, int bad) {
-        const int kt = first_key + it * step, key0 = kt + 4 * g;
+    auto work_on = [&](auto masked_, const Tile<HD> &t, int kt, int bad) {
+        constexpr bool masked = decltype(masked_)::value;
+        const int key0 = kt + 4 * g;
         f4 s[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = f4{0.f, 0.f, 0.f, 0.f};
@@ -363,7 +373,7 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
         for (int i = 0; i < 2; i++)
 #pragma unroll
             for (int w = 0; w < NW; w++) {
-                const h8 k8 = codes8(t.k[i][w]);
+                const h8 k8 = take.codes8(t.k[i][w]);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
                     s[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[rt][w], s[rt][i], 0, 0, 0);
@@ -386,8 +396,7 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
                 if (bad & 2) ak[1][r] = NAN, av[1][r] = 0.f, bv[1][r] = 0.f;
             }
         }
-        const bool masked = kt + 31 > pos_first || kt + 31 >= end || (a.window > 0 && kt <= pos_last - a.window);
-        if (masked) {  // what lies behind the end never counts, whatever it holds
+        if constexpr (masked) {  // what lies behind the end never counts, whatever it holds
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -402,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
         float p[RT][2][4], x[RT][2][4];
         float most_z = -INFINITY, most_x = 0.f;
         auto weigh = [&](int rt) {
-            scores(s, ak, bk, masked, key0, rt, -ref[rt], p[rt]);
+            scores(masked_, s, ak, bk, key0, rt, -ref[rt], p[rt]);
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -420,7 +429,7 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
                 float z[2][4];
-                scores(s, ak, bk, masked, key0, rt, 0.f, z);
+                scores(masked_, s, ak, bk, key0, rt, 0.f, z);
                 float m = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 2; i++)
@@ -465,8 +474,8 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
                 const uint32_t x1 = __builtin_amdgcn_perm(t.v[0][b][3], t.v[0][b][2], sel[b][i]);
                 const uint32_t x2 = __builtin_amdgcn_perm(t.v[1][b][1], t.v[1][b][0], sel[b][i]);
                 const uint32_t x3 = __builtin_amdgcn_perm(t.v[1][b][3], t.v[1][b][2], sel[b][i]);
-                const h8 even = as_h8(lower_less8(x0), lower_less8(x1), lower_less8(x2), lower_less8(x3));
-                const h8 odd = as_h8(upper_less8(x0), upper_less8(x1), upper_less8(x2), upper_less8(x3));
+                const h8 even = as_h8(take.lower(x0), take.lower(x1), take.lower(x2), take.lower(x3));
+                const h8 odd = as_h8(take.upper(x0), take.upper(x1), take.upper(x2), take.upper(x3));
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
                     f4 &e = o[rt][b * first + 2 * i], &d = o[rt][b * first + 2 * i + 1];
@@ -481,16 +490,25 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
         }
     };
 
-    if (count > 0) {  // the next tile's loads are in flight while one is worked on
+    auto process = [&](const Tile<HD> &t, int it, int bad) {
+        const int kt = first_key + it * step;
+        if (kt + 31 > pos_first || kt + 31 >= end || (a.window > 0 && kt <= pos_last - a.window))
+            work_on(std::true_type(), t, kt, bad);
+        else
+            work_on(std::false_type(), t, kt, bad);
+    };
+
+    if (count > 0) {
+        // The next tile's loads are in flight while one is worked on.  They are issued without a condition (the last tile again
+        // behind the end): the wait for a tile would else have to be one for everything.
         Tile<HD> t0, t1;
         int bad0, bad1;
         load_tile(0, t0, bad0);
         for (int it = 0; it < count; it += 2) {
-            if (it + 1 < count) load_tile(it + 1, t1, bad1);
+            load_tile(min(it + 1, count - 1), t1, bad1);
             process(t0, it, bad0);
-            if (it + 1 >= count) break;
-            if (it + 2 < count) load_tile(it + 2, t0, bad0);
-            process(t1, it + 1, bad1);
+            load_tile(min(it + 2, count - 1), t0, bad0);
+            if (it + 1 < count) process(t1, it + 1, bad1);
         }
     }
 
