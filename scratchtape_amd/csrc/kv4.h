@@ -55,6 +55,10 @@ inline bool cache_ok(const char *name, Cache &c, int64_t nseq, const int32_t *ta
         fail(ST_ERR_INVALID, "%s: %lld pages of %lld tokens a sequence pass 2^31", name, (long long)max_pages, (long long)page);
         return false;
     }
+    if (page * hkv * 256 > INT32_MAX) {
+        fail(ST_ERR_INVALID, "%s: %lld heads of %lld tokens a page are too many", name, (long long)hkv, (long long)page);
+        return false;
+    }
     if ((nseq * max_pages > 0 && !table) || (pages > 0 && (!k_codes || !k_scales || !v_codes || !v_scales))) {
         fail(ST_ERR_INVALID, "%s: NULL table or cache", name);
         return false;

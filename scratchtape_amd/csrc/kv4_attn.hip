@@ -20,14 +20,16 @@
 // V's operand wants 8 keys of one component in a lane: a lane reads a word (8 components) of 8 keys and v_perm pairs
 // their bytes.
 //
-// A workgroup of 4 waves has a tile of up to 64 RT rows of one sequence and key head, and a chunk of its keys; waves
-// without rows of their own share the tile's keys (a single token's rows: all four).  Chunks are cut so that about
-// `target` workgroups have equal shares of all sequences' keys together; the lengths are read on the device, and each
-// workgroup finds its place by a scan over the sequences.  Where a sequence has several chunks, k_merge4 joins them.
+// Work is cut on the device, where the lengths are.  A unit is a tile of up to 64 RT rows of one sequence and key head with
+// the keys that it sees; the units of all sequences stand one behind the other on a line of keys, which the launch's
+// workgroups (two to a CU) divide evenly.  A workgroup of 4 waves goes through its stretch of the line unit by unit; waves
+// without rows of their own share the unit's keys (a single token's rows: all four).  What a workgroup has of a unit
+// that others work on too goes to its slots in `work`, and k_merge4 joins the parts.
 #include <algorithm>
 #include <cmath>
 
 #include "common.h"
+#include "dma_tile.h"
 #include "kv4.h"
 #include "lanes.h"
 #include "quant4.h"
@@ -41,8 +43,9 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int MIN_CHUNK = 256;    // keys: below this a merge costs more than it shares out
-constexpr int MAX_CHUNKS = 8192;  // of one sequence (st_kv_attention_4bit keeps target below this)
+constexpr int MIN_STRETCH = 128;  // keys of a workgroup's stretch: less is not worth its start
+constexpr int WHOLE = 512;        // units of up to so many keys are not shared among workgroups: a merge would cost more
+constexpr int MAX_GROUPS = 1024;  // workgroups of a launch
 constexpr float BASE = 7.f, MOST_X = 32768.f;  // p aV is set to 2^7 at most, and may grow to 2^15
 constexpr float MIN_E = -86.f, MOST_P = 101.f;  // values below 2^-86 of scale count as that for the reference: p <= 2^93, 2^101
 
@@ -52,89 +55,170 @@ struct AttnArgs {
     void *out;
     float *lse;
     const int32_t *q_start, *kv_len;
-    float *part_o;    // [part_rows, hd] sums over a chunk's keys
-    float2 *part_ml;  // [part_rows] their bounds and totals
-    int64_t q_stride, part_rows;
+    float *part_o;    // [2 groups, part_rows, hd] sums of parts of units
+    float2 *part_ml;  // [2 groups, part_rows] their references and totals
+    int64_t q_stride;
     float scale2;  // scale log2 e
-    int32_t n, hq, dtype, causal, window, one, target;
+    int32_t n, hq, dtype, causal, window, one, groups, part_rows;
+    int32_t share, cap;      // query heads of a key head, tokens of a table's row
+    int32_t per, tile_rows;  // tokens (0: less than one) and rows of a tile
+    int32_t most, small;     // the most keys that a tile sees; whether the line's positions fit 32 bits
+    float inv_share, inv_groups;
     bool vec_q, vec_out;
 };
 
-// A sequence's rows and keys.
-struct Seq {
-    int first, rows, len, lo, span, tiles;
-};
+// A value that is the same in every lane, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int64_t s, int share, int tile_rows, int cap) {
-    Seq q;
-    const int b = min(max(a.q_start[s], 0), a.n), e = min(max(a.q_start[s + 1], 0), a.n);
-    q.first = b;
-    q.rows = max(e - b, 0);
-    q.len = max(a.kv_len[s], 0);
-    // The first key that the first row sees, down to a tile's start.
-    const int64_t lo = a.window > 0 ? max((int64_t)0, (int64_t)q.len - q.rows + 1 - a.window) : 0;
-    q.lo = (int)(lo & ~31);
-    q.span = max(min(q.len, cap) - q.lo, 0);
-    q.tiles = (q.rows * share + tile_rows - 1) / tile_rows;
+// x / y for quotients below 2^22: the f32 quotient is off by one at most.
+__device__ __forceinline__ int quotient(int64_t x, int64_t y) {
+    int q = (int)((float)x * __builtin_amdgcn_rcpf((float)y));
+    const int64_t r = x - (int64_t)q * y;
+    q += r >= y ? 1 : r < 0 ? -1 : 0;
     return q;
 }
 
-// Keys per chunk: a multiple of 128, the same in every workgroup (one order of additions).
-__device__ __forceinline__ int chunk_keys(const AttnArgs &a, int share, int tile_rows, int cap, int lane) {
-    float total = 0.f;
-    for (int64_t s0 = 0; s0 < a.c.nseq; s0 += 64) {
-        if (s0 + lane < a.c.nseq) {
-            const Seq q = seq_of(a, s0 + lane, share, tile_rows, cap);
-            total += (float)q.tiles * (float)q.span;
-        }
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += st::xor_lane(total, o, lane);
-    const float each = total * (float)a.c.hkv / (float)a.target;
-    const int keys = each < 2.0e9f ? (int)each : 2000000000;
-    return max((keys + 127) / 128 * 128, MIN_CHUNK);
-}
-
-struct Place {
-    Seq q;
-    int64_t s;
-    int64_t part;  // the first of the sequence's partial rows: row (i hq + head) chunks + chunk
-    int chunks, index;
+// A wave's copy, in LDS, of what the line's position needs of 64 sequences: registers are for tiles.
+struct Rows {
+    int64_t upto[64], head[64];  // keys on the line up to a sequence's end from the first of the 64 on, and those of one head
+    int first[64], rows[64], len[64], tiles[64];
 };
 
-// Finds the sequence that has workgroup `w` (by = items) or row `w` (by = rows); false: none has it.
-template <bool BY_ITEM>
-__device__ __forceinline__ bool place_of(const AttnArgs &a, int64_t w, int share, int tile_rows, int cap, int chunk, int lane,
-                                         Place &p) {
-    int64_t items = 0, parts = 0;
-    for (int64_t s0 = 0; s0 < a.c.nseq; s0 += 64) {
-        Seq q = {};
-        int mine = 0, chunks = 1;
-        if (s0 + lane < a.c.nseq) {
-            q = seq_of(a, s0 + lane, share, tile_rows, cap);
-            chunks = max((q.span + chunk - 1) / chunk, 1);
-            mine = q.tiles * a.c.hkv * chunks;
+// The line of keys: how units lie on it.
+struct Line {
+    const AttnArgs &a;
+    Rows &m;
+    int lane;
+    // `m` holds the 64 sequences from s0 on, `before` the line's keys before them, `inside` theirs.
+    int64_t s0 = 0, before = 0, inside = 0, length = 0, stretch = 0;
+
+    __device__ __forceinline__ Line(const AttnArgs &args, Rows &mem, int lane_) : a(args), m(mem), lane(lane_) {
+        for (;; s0 += 64) {
+            load();
+            length += inside;
+            if (s0 + 64 >= a.c.nseq) break;
         }
-        // Partial rows of up to 64 sequences in 32 bits: st_kv_attention_4bit bounds their number.
-        const int partial = chunks > 1 ? q.rows * a.hq * chunks : 0;
-        const int upto = st::wave_incl_scan(mine), parts_upto = st::wave_incl_scan(partial);
-        const bool here = BY_ITEM ? items + upto > w : q.first <= w && w < (int64_t)q.first + q.rows;
-        const uint64_t any = __ballot(here);
-        if (any) {
-            const int l = __ffsll((unsigned long long)any) - 1;
-            p.s = s0 + l;
-            p.q.first = st::lane_value(q.first, l), p.q.rows = st::lane_value(q.rows, l), p.q.len = st::lane_value(q.len, l);
-            p.q.lo = st::lane_value(q.lo, l), p.q.span = st::lane_value(q.span, l), p.q.tiles = st::lane_value(q.tiles, l);
-            p.chunks = st::lane_value(chunks, l);
-            p.part = parts + st::lane_value(parts_upto - partial, l);
-            p.index = (int)(w - items) - st::lane_value(upto - mine, l);
-            return true;
-        }
-        items += st::lane_value(upto, 63);
-        parts += st::lane_value(parts_upto, 63);
+        // length / groups, not less: the f32 product is within 2^-22 of it.
+        int64_t each = (int64_t)((float)length * a.inv_groups);
+        each += (each >> 20) + 1;
+        stretch = max((each + 127) & ~(int64_t)127, (int64_t)MIN_STRETCH);
+        if (s0 > 0) s0 = 0, load();
     }
-    return false;
-}
+
+    // Keys of a sequence's first j tiles of `tiles` (an upper bound where a window or rows without keys make it less; a tile has
+    // one at least, so that each is some workgroup's).
+    __device__ __forceinline__ int64_t keys_of(int j, int tiles, int rows, int len) const {
+        const int base = max(len - rows, 0), all = base + rows, most = a.most;
+        if (!a.causal || a.per == 0 || tiles == 1) return (int64_t)j * min(all, most);
+        // Tile i ends at token min((i + 1) per, rows) and sees base + that many keys, `most` of them.
+        int64_t sum = 0;
+        if (j == tiles) sum = min(all, most), j--;
+        const int64_t grow = min(j, most > base ? (most - base) / a.per : 0);
+        return sum + grow * base + a.per * (grow * (grow + 1) / 2) + (j - grow) * most;
+    }
+
+    __device__ __forceinline__ void load() {
+        int first = 0, rows = 0, len = 0, tiles = 0;
+        int64_t head = 0;
+        if (s0 + lane < a.c.nseq) {
+            const int64_t s = s0 + lane;
+            const int next = a.q_start[s + 1];
+            first = min(max(a.q_start[s], 0), a.n);
+            len = max(a.kv_len[s], 0);
+            rows = max(min(max(next, 0), a.n) - first, 0);
+        }
+        int64_t upto;
+        if (a.small && !__any(rows > a.per)) {  // a tile each at most, and 32 bits suffice: a decoding step
+            tiles = rows > 0 ? 1 : 0;
+            head = tiles ? min(max(len, rows), a.most) : 0;
+            upto = st::wave_incl_scan((int)head * a.c.hkv);
+        } else {
+            tiles = a.per ? (rows + a.per - 1) / a.per : (int)(((int64_t)rows * a.share + a.tile_rows - 1) / a.tile_rows);
+            if (tiles > 0) head = keys_of(tiles, tiles, rows, len);
+            // Prefix sums in two halves of 20 and more bits.
+            const int64_t here = head * a.c.hkv;
+            const int lo = st::wave_incl_scan((int)(here & 0xFFFFF)), hi = st::wave_incl_scan((int)(here >> 20));
+            upto = ((int64_t)hi << 20) + lo;
+        }
+        inside = st::lane_value64(upto, 63);
+        m.upto[lane] = upto, m.head[lane] = head;
+        m.first[lane] = first, m.rows[lane] = rows, m.len[lane] = len, m.tiles[lane] = tiles;
+    }
+
+    // A unit on the line.
+    struct Unit {
+        int64_t s, start;  // sequence, first position
+        int keys, first, rows, len, tiles, head, tile;
+    };
+
+    // Fills in `u` what goes by its sequence (the l-th of the 64): returns its first position, and the keys of a head.
+    __device__ __forceinline__ int64_t take(int l, Unit &u, int64_t &head) const {
+        u.s = s0 + l;
+        u.first = uniform(m.first[l]), u.rows = uniform(m.rows[l]), u.len = uniform(m.len[l]), u.tiles = uniform(m.tiles[l]);
+        head = st::lane_value64(m.head[l], 0);
+        return before + st::lane_value64(m.upto[l], 0) - head * a.c.hkv;
+    }
+
+    __device__ __forceinline__ void place(Unit &u, int64_t head_start, int tile) const {
+        u.tile = uniform(tile);
+        if (u.tiles == 1) {
+            u.start = head_start, u.keys = min(max(u.len, u.rows), a.most);
+            return;
+        }
+        const int64_t from = keys_of(u.tile, u.tiles, u.rows, u.len);
+        u.start = head_start + from;
+        u.keys = uniform((int)(keys_of(u.tile + 1, u.tiles, u.rows, u.len) - from));
+    }
+
+    // The unit at `at` (not before the last one asked for).
+    __device__ __forceinline__ Unit unit_at(int64_t at) {
+        while (at >= before + inside) before += inside, s0 += 64, load();
+        const int l = __ffsll((unsigned long long)__ballot(before + m.upto[lane] > at)) - 1;
+        Unit u;
+        int64_t each;
+        const int64_t base = take(l, u, each);
+        u.head = uniform(quotient(at - base, each));
+        const int64_t off = at - base - u.head * each;
+        int lo = 0, hi = u.tiles - 1;  // the last tile whose start is not behind `off`
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (keys_of(mid, u.tiles, u.rows, u.len) <= off)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        place(u, base + u.head * each, lo);
+        return u;
+    }
+
+    // The unit of row `row` (a token) and query head `i`, and the row's place in its tile; false if no sequence has the row.
+    __device__ __forceinline__ bool unit_of(int row, int i, Unit &u, int &at) {
+        if (a.c.nseq > 64) s0 = 0, before = 0, load();
+        for (;;) {
+            const int first = m.first[lane];
+            const uint64_t hit = __ballot(first <= row && row < first + m.rows[lane]);
+            if (hit) {
+                const int l = __ffsll((unsigned long long)hit) - 1;
+                int64_t each;
+                const int64_t base = take(l, u, each);
+                u.head = uniform(quotient(i, a.share));
+                const int r = (row - u.first) * a.share + i - u.head * a.share, tile = uniform(quotient(r, a.tile_rows));
+                at = r - tile * a.tile_rows;
+                place(u, base + u.head * each, tile);
+                return true;
+            }
+            if (s0 + 64 >= a.c.nseq) return false;
+            before += inside, s0 += 64, load();
+        }
+    }
+
+    // Where a workgroup's stretch, ending at line position `end`, ends within a unit: at a multiple of 128 of its keys.
+    __device__ __forceinline__ int cut(const Unit &u, int64_t end) const {
+        const int64_t x = end - u.start;
+        if (x <= 0) return 0;
+        return u.keys <= WHOLE ? u.keys : (int)min((x + 127) & ~(int64_t)127, (int64_t)u.keys);
+    }
+};
 
 // The head's components in blocks of 128, 64 or 32: lane column c of a block of width W reads W / 16 components from
 // W / 16 c on, which lie in one word.
@@ -143,55 +227,94 @@ constexpr int block_width(int hd, int b) {
 }
 constexpr int blocks_of(int hd) { return block_width(hd, 1) ? 2 : 1; }
 
+// A wave's ring of tiles in LDS.  A tile (32 keys: their codes and (scale, lo) pairs, in two halves of 16 keys, which a page may
+// end between) is brought by DMA in chunks of 16 bytes: of K, then of V, then the pairs of K and of V.  A chunk's place is
+// 16 bytes times its number; which chunk of memory it is, is the lane's choice:
+//  - K of 128 and 256 components: in the order that lanes read their fragments in (lane (col, g) key col's 16 bytes from
+//    piece g, or 2 g + i, on), which no bank is hit twice by; else key by key;
+//  - V: rows in the order 0 4 8 12 1 5 .., so that the four keys that a read takes lie side by side.
 template <int HD>
-struct Tile {
+struct Ring {
     static constexpr int NW = HD / 32, NB = blocks_of(HD);
-    uint32_t k[2][NW];  // of each half of 16 keys: this lane's quarter of one key
-    uint32_t v[2][NB][4];
-    float4 ks[2][2], vs[2][2];  // (scale, lo) of the lane group's 4 keys
+    static constexpr int PER_KEY = HD / 32, HALF = 16 * PER_KEY;                    // chunks
+    static constexpr int LOADS = (2 * HD + 32 + 63) / 64, BYTES = 1024 * LOADS;    // of a tile
+    static constexpr bool EVEN = HD == 128 || HD == 256;                            // a load is of one half of K or of V
+    static constexpr int PAIRS = 32 * HD;                                           // byte offset of the pairs
+
+    // Source byte offset of chunk `n` of a half of K or V.
+    static __device__ __forceinline__ int source(int n, bool v) {
+        if (v) {
+            const int slot = n / PER_KEY;
+            return (4 * (slot & 3) + (slot >> 2)) * (HD / 2) + 16 * (n % PER_KEY);
+        }
+        if (HD == 128) return (n & 15) * (HD / 2) + 16 * (n >> 4);
+        if (HD == 256) return (n & 15) * (HD / 2) + 16 * (2 * ((n >> 4) & 3) + (n >> 6));
+        return n / PER_KEY * (HD / 2) + 16 * (n % PER_KEY);
+    }
+
+    // This lane's words of K's half `half`.
+    static __device__ __forceinline__ void k_words(const char *tile, int half, int lane, uint32_t (&w)[NW]) {
+        typedef uint32_t v2 __attribute__((ext_vector_type(2)));
+        const int col = lane & 15, g = lane >> 4;
+        if constexpr (EVEN) {
+#pragma unroll
+            for (int i = 0; i < NW; i += 4) {
+                const u4 x = *(const u4 *)(tile + 16 * (HALF * half + 16 * i + lane));
+                w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
+            }
+        } else {
+            const char *p = tile + 16 * HALF * half + col * (HD / 2) + g * (HD / 8);
+            if constexpr (NW % 2 == 0) {
+#pragma unroll
+                for (int i = 0; i < NW; i += 2) {
+                    const v2 x = *(const v2 *)(p + 4 * i);
+                    w[i] = x[0], w[i + 1] = x[1];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NW; i++) w[i] = *(const uint32_t *)(p + 4 * i);
+            }
+        }
+    }
+
+    // This lane's word of block b of value 4 g + r of half `half`.
+    static __device__ __forceinline__ uint32_t v_word(const char *tile, int half, int b, int r, int lane) {
+        const int col = lane & 15, g = lane >> 4, width = block_width(HD, b), start = b ? block_width(HD, 0) : 0;
+        const int off = start / 2 + 4 * (width == 128 ? col : width == 64 ? col >> 1 : col >> 2);
+        return *(const uint32_t *)(tile + 16 * (HD + HALF * half) + (4 * r + g) * (HD / 2) + off);
+    }
+
+    // The (scale, lo) pairs of keys (or values) 4 g + 2 i and the next of half `half`.
+    static __device__ __forceinline__ float4 pairs(const char *tile, bool v, int half, int i, int g) {
+        return *(const float4 *)(tile + PAIRS + 256 * v + 128 * half + 32 * g + 16 * i);
+    }
 };
 
-template <int NW>
-__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[NW]) {
-    typedef uint32_t v2 __attribute__((ext_vector_type(2)));
-    typedef uint32_t v3 __attribute__((ext_vector_type(3), aligned(4)));
-    if constexpr (NW % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < NW; i += 4) {
-            const u4 x = *(const u4 *)(p + 4 * i);
-            w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
-        }
-    } else if constexpr (NW % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < NW; i += 2) {
-            const v2 x = *(const v2 *)(p + 4 * i);
-            w[i] = x[0], w[i + 1] = x[1];
-        }
-    } else if constexpr (NW == 3) {
-        const v3 x = *(const v3 *)p;
-        w[0] = x[0], w[1] = x[1], w[2] = x[2];
-    } else {
-        w[0] = *(const uint32_t *)p;
-    }
+// 16 bytes a lane from scalar base + lane offset, or from a lane's address, to LDS from `to` on.  In assembly, so that the
+// compiler does not wait for every load in flight before any LDS read: a tile's loads are waited for by their number.
+__device__ __forceinline__ void bring(const void *base, uint32_t off, uint32_t to) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(off), "s"(base), "s"(to)
+        : "memory");
 }
-
-// Half a tile: 16 keys of page `page`, from slot `slot` on.
-template <int HD>
-__device__ __forceinline__ void load_half(const Cache &c, int h, int page, int slot, int half, int lane, Tile<HD> &t) {
-    const int64_t row = ((int64_t)page * c.hkv + h) * c.page + slot;
-    const uint8_t *kb = c.k_codes + row * (HD / 2), *vb = c.v_codes + row * (HD / 2);
-    const float4 *ks = (const float4 *)(c.k_scales + row), *vs = (const float4 *)(c.v_scales + row);
-    const int col = lane & 15, g = lane >> 4;
-    load_words(kb + (col * (HD / 2) + g * (HD / 8)), t.k[half]);
-#pragma unroll
-    for (int i = 0; i < 2; i++) t.ks[half][i] = ks[2 * g + i], t.vs[half][i] = vs[2 * g + i];
-#pragma unroll
-    for (int b = 0; b < Tile<HD>::NB; b++) {
-        const int width = block_width(HD, b), start = b ? block_width(HD, 0) : 0;
-        const int off = start / 2 + 4 * (width == 128 ? col : width == 64 ? col >> 1 : col >> 2);
-#pragma unroll
-        for (int r = 0; r < 4; r++) t.v[half][b][r] = *(const uint32_t *)(vb + ((4 * g + r) * (HD / 2) + off));
-    }
+__device__ __forceinline__ void bring(const void *at, uint32_t to) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, off\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(at), "s"(to)
+        : "memory");
 }
 
 __device__ __forceinline__ h8 as_h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -223,50 +346,124 @@ struct Taker {
 };
 
 template <int HD, int PARTS, int RT>
-__global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
-    constexpr int NW = HD / 32, NB = blocks_of(HD), WAVE_ROWS = 16 * RT, TILE_ROWS = 4 * WAVE_ROWS, LDO = HD + 4;
-    __shared__ float red[4][WAVE_ROWS][LDO];
+__global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attention4(const AttnArgs a) {
+    using R = Ring<HD>;
+    constexpr int NW = HD / 32, NB = blocks_of(HD), WAVE_ROWS = 16 * RT, LDO = HD + 4, STAGES = RT == 1 ? 2 : 3;
+    constexpr int RING = 4 * STAGES * R::BYTES, SUMS = 4 * WAVE_ROWS * LDO * 4;
+    __shared__ __align__(16) char mem[RING > SUMS ? RING : SUMS];  // the waves' rings, then their sums
     __shared__ float2 ml[4][WAVE_ROWS];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    __shared__ Rows row_mem[4];
+    float(*red)[WAVE_ROWS][LDO] = (float(*)[WAVE_ROWS][LDO])mem;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const Cache &c = a.c;
-    const int share = a.hq / c.hkv, cap = (int)(c.max_pages << c.page_log2);
-    const int chunk = chunk_keys(a, share, TILE_ROWS, cap, lane);
-    Place pl;
-    if (!place_of<true>(a, blockIdx.x, share, TILE_ROWS, cap, chunk, lane, pl)) return;
-    // Key heads beside each other (workgroups of one XCD share a head's pages), then the longest tiles first.
-    const int h = pl.index % c.hkv, rest = pl.index / c.hkv;
-    const int tile = pl.q.tiles - 1 - rest % pl.q.tiles, part = rest / pl.q.tiles;
-    if (pl.index < 0 || part >= pl.chunks) return;  // (row starts that do not ascend)
-    const int all_rows = pl.q.rows * share, row0 = tile * TILE_ROWS, rows = min(TILE_ROWS, all_rows - row0);
+    Line line(a, row_mem[wave], lane);
+    const int share = a.share, cap = a.cap;
+    // Neighbouring stretches to one XCD (workgroups go round the 8 of them): units of a head share its pages.
+    const int used = uniform(quotient(line.length + line.stretch - 1, line.stretch)), each = (used + 7) / 8;
+    const int64_t me = (int64_t)(blockIdx.x & 7) * each + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= each || me >= used) return;
+    const int64_t line_end = min((me + 1) * line.stretch, line.length);
+    const Taker take;
+    char *ring = mem + wave * STAGES * R::BYTES;
+    const uint32_t ring_at = uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)ring);
+
+  for (int64_t at = me * line.stretch; at < line_end;) {
+    const auto u = line.unit_at(at);
+    const int cut0 = uniform(line.cut(u, me * line.stretch)), cut1 = uniform(line.cut(u, line_end));
+    at = u.start + u.keys;
+    if (cut0 == cut1) continue;
+    // The tile's rows (a token's heads side by side) begin at head `rem0` of token tok0.
+    const int h = u.head, row0 = u.tile * a.tile_rows, rows = min(a.tile_rows, u.rows * share - row0);
+    const int tok0 = a.per ? u.tile * a.per : uniform(quotient(row0, share)), rem0 = a.per ? 0 : row0 - tok0 * share;
+    auto token_of = [&](int x) { return (int)(((float)(rem0 + x) + 0.5f) * a.inv_share); };  // of row x of the tile, from tok0 on
     const int groups = (rows + WAVE_ROWS - 1) / WAVE_ROWS, sharing = groups == 1 ? 4 : groups == 2 ? 2 : 1;
     const int group = wave / sharing, turn = wave % sharing;
     const bool busy = group < groups;
 
     // This lane's row of each 16, and the positions of the group's first and last.
     int pos[RT];
-    const int base = pl.q.len - pl.q.rows;  // position of the first row (negative: more rows than tokens)
-    const int first_row = row0 + group * WAVE_ROWS, last_row = min(first_row + WAVE_ROWS, all_rows) - 1;
-    const int pos_first = a.causal ? base + first_row / share : pl.q.len - 1;
-    const int pos_last = a.causal ? base + last_row / share : pl.q.len - 1;
+    const int base = u.len - u.rows + tok0;  // position of the first row (negative: more rows than tokens)
+    const int first_row = group * WAVE_ROWS, last_row = min(first_row + WAVE_ROWS, rows) - 1;
+    const int pos_first = uniform(a.causal ? base + token_of(first_row) : u.len - 1);
+    const int pos_last = uniform(a.causal ? base + token_of(last_row) : u.len - 1);
+
+    // The group's keys of this part: those that its first row may see up to those of its last, within the table.
+    const int tile_first = a.causal ? base : u.len - 1;
+    const int lo = a.window > 0 ? (int)(max((int64_t)0, (int64_t)tile_first + 1 - a.window) & ~31) : 0;
+    int begin = lo + cut0, end = min(pos_last + 1, cap);
+    if (cut1 < u.keys) end = min(end, lo + cut1);
+    if (a.window > 0) begin = max(begin, (int)(max((int64_t)0, (int64_t)pos_first + 1 - a.window) & ~31));
+    begin = uniform(begin), end = uniform(end);
+    const int first_key = uniform(begin + 32 * turn), step = 32 * sharing;
+    const int count = uniform(busy && c.pages > 0 && end > first_key ? (end - first_key + step - 1) / step : 0);
+    const bool no_pages = busy && c.pages == 0 && end > begin;
+
+    // Pages of the next 32 tiles' halves, a half a lane: -1 one outside the cache, 0 (not looked at) behind the end.
+    const int page_rows = c.hkv * c.page, head_row = h * c.page;
+    int entries = 0, entries_to = 0;
+    uint32_t bad = 0;  // of the tiles in the ring, two bits each
+    auto bring_tile = [&](int it, int slot) {
+        if (it >= entries_to) {
+            const int key = first_key + (it + (lane >> 1)) * step + 16 * (lane & 1);
+            entries = 0;
+            if (key < end) {
+                const int p = c.table[u.s * c.max_pages + (key >> c.page_log2)];
+                entries = p >= 0 && p < c.pages ? p : -1;
+            }
+            entries_to = it + 32;
+        }
+        const int key = first_key + it * step, i = 2 * (it + 32 - entries_to);
+        const int p0 = st::lane_value(entries, i), p1 = st::lane_value(entries, i + 1);
+        bad = (bad & ~(3u << (2 * slot))) | ((p0 < 0 ? 1u : 0u) | (p1 < 0 ? 2u : 0u)) << (2 * slot);
+        const int64_t row_0 = (int64_t)max(p0, 0) * page_rows + (head_row + (key & (c.page - 1)));
+        const int64_t row_1 = (int64_t)max(p1, 0) * page_rows + (head_row + ((key + 16) & (c.page - 1)));
+        const uint32_t to = ring_at + slot * R::BYTES;
+        const int64_t b0 = row_0 * (HD / 2), b1 = row_1 * (HD / 2);
+#pragma unroll
+        for (int i = 0; i < R::LOADS; i++) {
+            if (R::EVEN && i < HD / 32) {  // one half of K or V
+                const bool v = i >= HD / 64;
+                const int j = v ? i - HD / 64 : i, half = 64 * j / R::HALF;
+                bring((v ? c.v_codes : c.k_codes) + (half ? b1 : b0), R::source(64 * j % R::HALF + lane, v), to + 1024 * i);
+            } else {
+                int n = 64 * i + lane;
+                const char *from;
+                if (n < 2 * HD) {
+                    const bool v = n >= HD;
+                    n -= v ? HD : 0;
+                    from = (const char *)(v ? c.v_codes : c.k_codes) + (n >= R::HALF ? b1 : b0) + R::source(n % R::HALF, v);
+                } else {
+                    n = (n - 2 * HD) & 31;  // lanes without a chunk of their own repeat one into the tile's padding
+                    from = (const char *)(n >= 16 ? c.v_scales : c.k_scales) + (n & 8 ? row_1 : row_0) * 8 + 16 * (n & 7);
+                }
+                bring(from, to + 1024 * i);
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES; i++)
+        if (i < count) bring_tile(i, i);
+
     h8 qh[RT][NW], ql[PARTS == 2 ? RT : 1][PARTS == 2 ? NW : 1];
-    float unscale[RT], qsum[RT];
+    float unscale[RT], qsum[RT], qsum8[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const int r = first_row + 16 * rt + col;
-        pos[rt] = a.causal ? base + min(r, all_rows - 1) / share : pl.q.len - 1;
+        const int token = token_of(min(r, rows - 1));
+        pos[rt] = a.causal ? base + token : u.len - 1;
         float x[NW][8];
         float most = 0.f, sum = 0.f;
         bool finite = true;
-        if (busy && r < all_rows) {
-            const int64_t at = (int64_t)(pl.q.first + r / share) * a.q_stride + (int64_t)(h * share + r % share) * HD + g * (HD / 4);
+        if (busy && r < rows) {
+            const int64_t from = (int64_t)(u.first + tok0 + token) * a.q_stride + (h * share + rem0 + r - token * share) * HD + g * (HD / 4);
 #pragma unroll
             for (int w = 0; w < NW; w++) {
                 if (a.dtype == ST_F32)
-                    st::load8((const float *)a.q + at + 8 * w, a.vec_q, x[w]);
+                    st::load8((const float *)a.q + from + 8 * w, a.vec_q, x[w]);
                 else if (a.dtype == ST_F16)
-                    st::load8((const _Float16 *)a.q + at + 8 * w, a.vec_q, x[w]);
+                    st::load8((const _Float16 *)a.q + from + 8 * w, a.vec_q, x[w]);
                 else
-                    st::load8((const __bf16 *)a.q + at + 8 * w, a.vec_q, x[w]);
+                    st::load8((const __bf16 *)a.q + from + 8 * w, a.vec_q, x[w]);
             }
         } else {
 #pragma unroll
@@ -290,7 +487,7 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
         // The row's largest component to 2^14 .. 2^15.
         const int e = most > 0.f && __builtin_isfinite(most) ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
         unscale[rt] = __builtin_amdgcn_ldexpf(a.scale2, -e);
-        qsum[rt] = a.scale2 * sum;
+        qsum[rt] = a.scale2 * sum, qsum8[rt] = 8.f * qsum[rt];
 #pragma unroll
         for (int w = 0; w < NW; w++) {
             constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
@@ -302,13 +499,6 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
             }
         }
     }
-
-    // The group's keys of this chunk: those that its first row may see up to those of its last, within the table.
-    int begin = pl.q.lo + part * chunk, end = (int)min(min((int64_t)begin + chunk, (int64_t)pos_last + 1), (int64_t)cap);
-    if (a.window > 0) begin = max(begin, (int)(max((int64_t)0, (int64_t)pos_first + 1 - a.window) & ~31));
-    const int first_key = begin + 32 * turn, step = 32 * sharing;
-    const int count = busy && c.pages > 0 && end > first_key ? (end - first_key + step - 1) / step : 0;
-    const bool no_pages = busy && c.pages == 0 && end > begin;
 
     f4 o[RT][HD / 16];
     float ref[RT], total[RT], low[RT];  // sums in units of 2^ref
@@ -327,116 +517,102 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
             sel[b][i] = 0x0c000c00u | (uint32_t)(4 + byte) << 16 | (uint32_t)byte;
         }
 
-    const Taker take;
-    // Pages of the next 32 tiles' halves, a half a lane: -1 one outside the cache, 0 (not looked at) behind the end.
-    int entries = 0, entries_to = 0;
-    auto load_entries = [&](int it) {
-        const int key = first_key + (it + (lane >> 1)) * step + 16 * (lane & 1);
-        entries = 0;
-        if (key < end) {
-            const int p = c.table[pl.s * c.max_pages + (key >> c.page_log2)];
-            entries = p >= 0 && p < c.pages ? p : -1;
+    auto process = [&](char *tile, int it, int bad_halves) {
+        const int kt = first_key + it * step, key0 = kt + 4 * g;
+        const bool masked = kt + 31 > pos_first || kt + 31 >= end || (a.window > 0 && kt <= pos_last - a.window);
+        bool careful = false;
+        if (masked || bad_halves) {
+            // What lies behind the end counts nothing, whatever it holds; keys on a page outside the cache are NaN to the rows that
+            // see them; and a value that is not finite must not reach the rows that do not see it, as 0 times it.
+            const int k = lane & 31;
+            const bool gone = bad_halves & (k & 16 ? 2 : 1);
+            float2 *kp = (float2 *)(tile + R::PAIRS) + k, *vp = kp + 32;
+            const float2 v = *vp;
+            if (gone) *kp = make_float2(NAN, NAN);
+            if (gone || kt + k >= end) *vp = make_float2(0.f, 0.f);
+            careful = __any(!gone && kt + k < end && !__builtin_isfinite(v.x + v.y));
         }
-    };
-    auto load_tile = [&](int it, Tile<HD> &t, int &bad) {
-        if (it >= entries_to) load_entries(it), entries_to = it + 32;
-        const int key = first_key + it * step;
-        const int at = 2 * (it + 32 - entries_to), p0 = st::lane_value(entries, at), p1 = st::lane_value(entries, at + 1);
-        bad = (p0 < 0 ? 1 : 0) | (p1 < 0 ? 2 : 0);
-        load_half<HD>(c, h, max(p0, 0), key & (c.page - 1), 0, lane, t);
-        load_half<HD>(c, h, max(p1, 0), (key + 16) & (c.page - 1), 1, lane, t);
-    };
-
-    auto scores = [&](auto masked_, const f4 (&s)[RT][2], const float (&ak)[2][4], const float (&bk)[2][4], int key0, int rt,
-                      float shift, float (&z)[2][4]) {
-        constexpr bool masked = decltype(masked_)::value;
+        // Scores of the tile less `shift`, in log2.
+        auto scores = [&](const char *tile, const float (&shift)[RT], float (&z)[RT][2][4]) {
+            f4 s[RT][2];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+            for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                z[i][r] = __builtin_fmaf(ak[i][r], s[rt][i][r] * unscale[rt], __builtin_fmaf(bk[i][r], qsum[rt], shift));
-                if constexpr (masked) {
-                    const int key = key0 + 16 * i + r;
-                    const bool seen = key <= pos[rt] && (a.window <= 0 || key > pos[rt] - a.window);
-                    z[i][r] = seen ? z[i][r] : -INFINITY;
+            for (int i = 0; i < 2; i++) {
+                uint32_t kw[NW];
+                R::k_words(tile, i, lane, kw);
+#pragma unroll
+                for (int w = 0; w < NW; w++) {
+                    const h8 k8 = take.codes8(kw[w]);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        s[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[rt][w], s[rt][i], 0, 0, 0);
+                        if constexpr (PARTS == 2) s[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[rt][w], s[rt][i], 0, 0, 0);
+                    }
                 }
             }
-    };
-
-    auto work_on = [&](auto masked_, const Tile<HD> &t, int kt, int bad) {
-        constexpr bool masked = decltype(masked_)::value;
-        const int key0 = kt + 4 * g;
-        f4 s[RT][2];
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const h8 k8 = take.codes8(t.k[i][w]);
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    s[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[rt][w], s[rt][i], 0, 0, 0);
-                    if constexpr (PARTS == 2) s[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[rt][w], s[rt][i], 0, 0, 0);
-                }
-            }
-        float ak[2][4], bk[2][4], av[2][4], bv[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float4 x = t.ks[i][r >> 1], y = t.vs[i][r >> 1];
-                ak[i][r] = r & 1 ? x.z : x.x, bk[i][r] = r & 1 ? x.w : x.y;
-                av[i][r] = r & 1 ? y.z : y.x, bv[i][r] = r & 1 ? y.w : y.y;
-            }
-        if (bad) {  // keys on a page outside the cache: NaN to the rows that see them
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                if (bad & 1) ak[0][r] = NAN, av[0][r] = 0.f, bv[0][r] = 0.f;
-                if (bad & 2) ak[1][r] = NAN, av[1][r] = 0.f, bv[1][r] = 0.f;
-            }
-        }
-        if constexpr (masked) {  // what lies behind the end never counts, whatever it holds
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (key0 + 16 * i + r >= end) av[i][r] = bv[i][r] = 0.f;
-        }
+                for (int r = 0; r < 4; r += 2) {
+                    const float4 y = R::pairs(tile, false, i, r / 2, g);
 #pragma unroll
-        for (int i = 0; i < 2; i++)  // what a code of 8 stands for
+                    for (int rt = 0; rt < RT; rt++) {
+                        z[rt][i][r] = __builtin_fmaf(y.x, __builtin_fmaf(s[rt][i][r], unscale[rt], qsum8[rt]), __builtin_fmaf(y.y, qsum[rt], -shift[rt]));
+                        z[rt][i][r + 1] = __builtin_fmaf(y.z, __builtin_fmaf(s[rt][i][r + 1], unscale[rt], qsum8[rt]), __builtin_fmaf(y.w, qsum[rt], -shift[rt]));
+                    }
+                }
+            if (masked) {
 #pragma unroll
-            for (int r = 0; r < 4; r++) bk[i][r] = __builtin_fmaf(8.f, ak[i][r], bk[i][r]), bv[i][r] = __builtin_fmaf(8.f, av[i][r], bv[i][r]);
-        // p = 2^(z - R) and p aV of every row; R is raised where p aV would pass f16's range or p an f32's.
+                for (int rt = 0; rt < RT; rt++) {
+                    const int after = a.window > 0 ? pos[rt] - a.window : -1;
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int key = key0 + 16 * i + r;
+                            z[rt][i][r] = key <= pos[rt] && key > after ? z[rt][i][r] : -INFINITY;
+                        }
+                }
+            }
+        };
+        // p = 2^(z - R) and p aV of every row.  For the first tile, and where p aV would pass f16's range or p an f32's, the scores
+        // are taken again to set R: seldom, and the common tile holds no registers for it.
         float p[RT][2][4], x[RT][2][4];
-        float most_z = -INFINITY, most_x = 0.f;
-        auto weigh = [&](int rt) {
-            scores(masked_, s, ak, bk, key0, rt, -ref[rt], p[rt]);
+        float most_z = -INFINITY, most_x = INFINITY;
+        if (it > 0) {
+            scores(tile, ref, p);
+            most_x = 0.f;
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    most_z = fmaxf(most_z, p[rt][i][r]);
-                    p[rt][i][r] = __builtin_amdgcn_exp2f(p[rt][i][r]);
-                    x[rt][i][r] = p[rt][i][r] * av[i][r];
-                    if (masked && p[rt][i][r] == 0.f) x[rt][i][r] = 0.f;  // not 0 times a NaN
-                    most_x = fmaxf(most_x, x[rt][i][r]);
-                }
-        };
+                    const float4 y = R::pairs(tile, true, i, r / 2, g);
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) weigh(rt);
+                    for (int rt = 0; rt < RT; rt++) {
+                        most_z = fmaxf(most_z, p[rt][i][r]);
+                        p[rt][i][r] = __builtin_amdgcn_exp2f(p[rt][i][r]);
+                        x[rt][i][r] = p[rt][i][r] * (r & 1 ? y.z : y.x);
+                        most_x = fmaxf(most_x, x[rt][i][r]);
+                    }
+                }
+        }
         if (__any(most_z > MOST_P || most_x > MOST_X)) {
+            uint32_t from = uniform((uint32_t)(tile - mem));
+            asm volatile("" : "+s"(from));  // read again, not kept
+            const char *again = mem + from;
+            float zero[RT] = {};
+            scores(again, zero, p);
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
-                float z[2][4];
-                scores(masked_, s, ak, bk, key0, rt, 0.f, z);
                 float m = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float e = av[i][r] > 0.f ? (float)__builtin_amdgcn_frexp_expf(av[i][r]) : MIN_E;
-                        m = fmaxf(m, z[i][r] + fmaxf(e, MIN_E));
+                        const float4 y = R::pairs(again, true, i, r / 2, g);
+                        const float v = r & 1 ? y.z : y.x, e = v > 0.f ? (float)__builtin_amdgcn_frexp_expf(v) : MIN_E;
+                        m = fmaxf(m, p[rt][i][r] + fmaxf(e, MIN_E));
                     }
                 m = fmaxf(m, st::xor_lane(m, 16, lane));
                 m = fmaxf(m, st::xor_lane(m, 32, lane));
@@ -446,34 +622,51 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
 #pragma unroll
                 for (int j = 0; j < HD / 16; j++) o[rt][j] *= keep;
                 ref[rt] = m;
-                weigh(rt);
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float4 y = R::pairs(again, true, i, r / 2, g);
+                        // (A row without a reference sees nothing here: minus infinity less itself is no number.)
+                        p[rt][i][r] = m == -INFINITY && p[rt][i][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[rt][i][r] - m);
+                        x[rt][i][r] = p[rt][i][r] * (r & 1 ? y.z : y.x);
+                    }
             }
         }
         h8 ph[RT], pr[PARTS == 2 ? RT : 1];
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int r = 0; r < 4; r++) {
+                const float4 y = R::pairs(tile, true, i, r / 2, g);
+                const float v8 = __builtin_fmaf(8.f, r & 1 ? y.z : y.x, r & 1 ? y.w : y.y);  // what a code of 8 stands for
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
+                for (int rt = 0; rt < RT; rt++) {
+                    float &xx = x[rt][i][r];
                     total[rt] += p[rt][i][r];
-                    float y = p[rt][i][r] * bv[i][r];
-                    if (masked && p[rt][i][r] == 0.f) y = 0.f;
-                    low[rt] += y;
-                    ph[rt][4 * i + r] = (_Float16)x[rt][i][r];
-                    if constexpr (PARTS == 2) pr[rt][4 * i + r] = (_Float16)(x[rt][i][r] - (float)ph[rt][4 * i + r]);
+                    if (careful && p[rt][i][r] == 0.f)
+                        xx = 0.f;
+                    else
+                        low[rt] = __builtin_fmaf(p[rt][i][r], v8, low[rt]);
+                    ph[rt][4 * i + r] = (_Float16)xx;
+                    if constexpr (PARTS == 2) pr[rt][4 * i + r] = (_Float16)(xx - (float)ph[rt][4 * i + r]);
                 }
-        }
+            }
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             constexpr int first = block_width(HD, 0) / 16;
             const int bytes = block_width(HD, b) / 32;
+            uint32_t vw[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) vw[i][r] = R::v_word(tile, i, b, r, lane);
 #pragma unroll
             for (int i = 0; i < bytes; i++) {
-                const uint32_t x0 = __builtin_amdgcn_perm(t.v[0][b][1], t.v[0][b][0], sel[b][i]);
-                const uint32_t x1 = __builtin_amdgcn_perm(t.v[0][b][3], t.v[0][b][2], sel[b][i]);
-                const uint32_t x2 = __builtin_amdgcn_perm(t.v[1][b][1], t.v[1][b][0], sel[b][i]);
-                const uint32_t x3 = __builtin_amdgcn_perm(t.v[1][b][3], t.v[1][b][2], sel[b][i]);
+                const uint32_t x0 = __builtin_amdgcn_perm(vw[0][1], vw[0][0], sel[b][i]);
+                const uint32_t x1 = __builtin_amdgcn_perm(vw[0][3], vw[0][2], sel[b][i]);
+                const uint32_t x2 = __builtin_amdgcn_perm(vw[1][1], vw[1][0], sel[b][i]);
+                const uint32_t x3 = __builtin_amdgcn_perm(vw[1][3], vw[1][2], sel[b][i]);
                 const h8 even = as_h8(take.lower(x0), take.lower(x1), take.lower(x2), take.lower(x3));
                 const h8 odd = as_h8(take.upper(x0), take.upper(x1), take.upper(x2), take.upper(x3));
 #pragma unroll
@@ -490,29 +683,20 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
         }
     };
 
-    auto process = [&](const Tile<HD> &t, int it, int bad) {
-        const int kt = first_key + it * step;
-        if (kt + 31 > pos_first || kt + 31 >= end || (a.window > 0 && kt <= pos_last - a.window))
-            work_on(std::true_type(), t, kt, bad);
+    for (int it = 0, slot = 0; it < count; it++) {
+        // This tile's loads are over when only those of the STAGES - 1 behind it are under way (near the end: when none is).
+        if (it + STAGES <= count)
+            dma::wait_vm<(STAGES - 1) * R::LOADS>();
         else
-            work_on(std::false_type(), t, kt, bad);
-    };
-
-    if (count > 0) {
-        // The next tile's loads are in flight while one is worked on.  They are issued without a condition (the last tile again
-        // behind the end): the wait for a tile would else have to be one for everything.
-        Tile<HD> t0, t1;
-        int bad0, bad1;
-        load_tile(0, t0, bad0);
-        for (int it = 0; it < count; it += 2) {
-            load_tile(min(it + 1, count - 1), t1, bad1);
-            process(t0, it, bad0);
-            load_tile(min(it + 2, count - 1), t0, bad0);
-            if (it + 1 < count) process(t1, it + 1, bad1);
-        }
+            dma::wait_vm<0>();
+        asm volatile("" ::: "memory");
+        process(ring + slot * R::BYTES, it, (bad >> (2 * slot)) & 3);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the tile's last reads are over before it is overwritten
+        if (it + STAGES < count) bring_tile(it + STAGES, slot);
+        slot = slot + 1 == STAGES ? 0 : slot + 1;
     }
 
-    // Each wave's sums in true units against its own bound, then against the bound of the waves that share its rows.
+    // The sums of the waves that share rows, each against the wave's own reference, meet in LDS.
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         total[rt] += st::xor_lane(total[rt], 16, lane);
@@ -523,46 +707,50 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
         if (pos[rt] >= cap || no_pages) total[rt] = NAN;
         if (g == 0) ml[wave][16 * rt + col] = make_float2(ref[rt], total[rt]);
     }
-    __syncthreads();
+    __syncthreads();  // every ring is read
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        float m = -INFINITY;
-        for (int i = 0; i < sharing; i++) m = fmaxf(m, ml[group * sharing + i][16 * rt + col].x);
-        const float factor = ref[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref[rt] - m);
-        const float off = low[rt] * factor;
+    for (int rt = 0; rt < RT; rt++)
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             constexpr int first = block_width(HD, 0) / 16;
             const int per = block_width(HD, b) / 16, start = b ? block_width(HD, 0) : 0;
 #pragma unroll
-            for (int j = 0; j < per; j++)
+            for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    red[wave][16 * rt + col][start + per * (4 * g + r) + j] = __builtin_fmaf(o[rt][b * first + j][r], factor, off);
+                for (int j = 0; j < per; j++) red[wave][16 * rt + col][start + per * (4 * g + r) + j] = o[rt][b * first + j][r] + low[rt];
         }
-    }
     __syncthreads();
     for (int i = threadIdx.x; i < rows * (HD / 8); i += 256) {
-        const int x = i / (HD / 8), e = 8 * (i % (HD / 8)), w0 = x / WAVE_ROWS * sharing, y = x % WAVE_ROWS;
+        const int y = i / (HD / 8), e = 8 * (i % (HD / 8)), w0 = y / WAVE_ROWS * sharing, z = y % WAVE_ROWS;
+        float2 t[4];
         float m = -INFINITY, l = 0.f, v[8] = {};
-        for (int k = 0; k < sharing; k++) m = fmaxf(m, ml[w0 + k][y].x);
-        for (int k = 0; k < sharing; k++) {
-            const float2 t = ml[w0 + k][y];
-            l += t.y * (t.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t.x - m));
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] += red[w0 + k][y][e + j];
+        for (int k = 0; k < 4; k++) {
+            t[k] = ml[min(w0 + k, 3)][z];
+            if (k >= sharing) t[k] = make_float2(-INFINITY, 0.f);
+            m = fmaxf(m, t[k].x);
         }
-        const int r = row0 + x, head = h * share + r % share;
-        const int64_t row = ((int64_t)pl.q.first + r / share) * a.hq + head;
-        if (pl.chunks > 1) {
-            const int64_t slot = pl.part + ((int64_t)(r / share) * a.hq + head) * pl.chunks + part;
-            if (slot < 0 || slot >= a.part_rows) continue;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float f = t[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t[k].x - m);
+            l += t[k].y * f;
+            if (k < sharing) {
+                float w[8];
+                st::load8(&red[w0 + k][z][e], true, w);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(w[j], f, v[j]);
+            }
+        }
+        const int token = token_of(y);
+        const int64_t row = (int64_t)(u.first + tok0 + token) * a.hq + h * share + rem0 + y - token * share;
+        if (cut0 > 0 || cut1 < u.keys) {
+            const int64_t slot = (2 * me + (cut0 == 0 ? 1 : 0)) * a.part_rows + y;
             st::store8(a.part_o + slot * HD + e, true, v);
             if (e == 0) a.part_ml[slot] = make_float2(m, l);
             continue;
         }
         const float top = a.one ? fmaxf(m, 0.f) : m, f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-        const float sum = l * f + (a.one ? __builtin_amdgcn_exp2f(-top) : 0.f), inv = sum == 0.f ? 0.f : f / sum;
+        const float sum = l * f + (a.one ? __builtin_amdgcn_exp2f(-top) : 0.f), inv = sum == 0.f ? 0.f : f * __builtin_amdgcn_rcpf(sum);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] *= inv;
         if (a.dtype == ST_F32)
@@ -573,98 +761,124 @@ __global__ __launch_bounds__(256, 2) void k_attention4(const AttnArgs a) {
             st::store8((__bf16 *)a.out + row * HD + e, a.vec_out, v);
         if (a.lse && e == 0) a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
     }
+    __syncthreads();  // the sums are read before the rings are filled again
+  }
 }
 
-// Joins the chunks of the rows whose sequences have several: out = sum_c 2^(M_c - M) O_c / sum_c 2^(M_c - M) l_c.
-template <int HD>
-__global__ __launch_bounds__(256) void k_merge4(const AttnArgs a, int tile_rows) {
-    constexpr int LANES = HD / 4, GROUPS = 256 / LANES;
-    __shared__ float weight[MAX_CHUNKS];
-    __shared__ float red[GROUPS][HD], stat[8];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Cache &c = a.c;
-    const int share = a.hq / c.hkv, cap = (int)(c.max_pages << c.page_log2);
-    const int chunk = chunk_keys(a, share, tile_rows, cap, lane);
+// Joins the parts of units that several workgroups worked on: out = sum 2^(M_i - M) O_i / sum 2^(M_i - M) l_i over a row's parts.
+// WAVES waves take a row and head: the first part is in the odd slot of the workgroup that has the unit's start, the
+// others in the even slots of those behind it.
+template <int HD, int WAVES>
+__global__ __launch_bounds__(256) void k_merge4(const AttnArgs a) {
+    constexpr int LANES = HD / 4, GROUPS = 64 * WAVES / LANES, TEAMS = 4 / WAVES;
+    __shared__ float weights[TEAMS][MAX_GROUPS + 8];
+    __shared__ float red[TEAMS][GROUPS][HD], stat[8];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), team = wave / WAVES;
+    const int me = threadIdx.x - team * 64 * WAVES;
+    __shared__ Rows row_mem[4];
+    Line line(a, row_mem[wave], lane);
+    auto meet = [&] {
+        if constexpr (WAVES > 1)
+            __syncthreads();
+        else
+            __builtin_amdgcn_wave_barrier();
+    };
+    float *weight = weights[team];
     const int64_t pairs = (int64_t)a.n * a.hq;
-    for (int64_t pair = blockIdx.x; pair < pairs; pair += gridDim.x) {
-        const int row = (int)(pair / a.hq), head = (int)(pair - (int64_t)row * a.hq);
-        Place pl;
-        if (!place_of<false>(a, row, share, tile_rows, cap, chunk, lane, pl) || pl.chunks == 1 || pl.chunks > MAX_CHUNKS) continue;
-        const int64_t slot = pl.part + ((int64_t)(row - pl.q.first) * a.hq + head) * pl.chunks;
-        if (slot < 0 || slot + pl.chunks > a.part_rows) continue;
+    // A workgroup's waves go through as many pairs each, so that all meet.
+    for (int64_t p0 = (int64_t)blockIdx.x * TEAMS; p0 < pairs; p0 += (int64_t)gridDim.x * TEAMS) {
+        const int64_t pair = p0 + team;
+        Line::Unit u;
+        int place = 0;
+        const int row = (int)(min(pair, pairs - 1) / a.hq), head = (int)(min(pair, pairs - 1) - (int64_t)row * a.hq);
+        if (pair >= pairs || !line.unit_of(row, head, u, place) || u.keys <= WHOLE) continue;
+        const int w0 = uniform(quotient(u.start, line.stretch)), w1 = uniform(quotient(u.start + u.keys - 1, line.stretch));
+        if (w1 == w0) continue;
+        // The last one's share may be empty: its keys went to the one before.
+        const int parts = w1 - w0 + (line.cut(u, (int64_t)w1 * line.stretch) < u.keys ? 1 : 0);
+        if (parts == 1) continue;
+        auto slot = [&](int i) { return (2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0)) * a.part_rows + place; };
         float m = -INFINITY, l = 0.f;
-        for (int i = threadIdx.x; i < pl.chunks; i += 256) m = fmaxf(m, a.part_ml[slot + i].x);
+        for (int i = me; i < parts; i += 64 * WAVES) {
+            const float2 t = a.part_ml[slot(i)];
+            weight[i] = t.x;
+            m = fmaxf(m, t.x);
+            if (i < 64 * WAVES) l = t.y;
+        }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, st::xor_lane(m, o, lane));
-        __syncthreads();  // the last pair's readers are done
-        if (lane == 0) stat[wave] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
-        for (int i = threadIdx.x; i < pl.chunks; i += 256) {
-            const float2 t = a.part_ml[slot + i];
-            const float w = t.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t.x - m);
+        if constexpr (WAVES > 1) {
+            if (lane == 0) stat[wave] = m;
+            __syncthreads();
+            m = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
+        }
+        float sum = 0.f;
+        for (int i = me; i < parts; i += 64 * WAVES) {
+            const float w = weight[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(weight[i] - m);
             weight[i] = w;
-            l += t.y * w;
+            sum += w * (i < 64 * WAVES ? l : a.part_ml[slot(i)].y);
         }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) l += st::xor_lane(l, o, lane);
-        if (lane == 0) stat[4 + wave] = l;
-        __syncthreads();
-        l = (stat[4] + stat[5]) + (stat[6] + stat[7]);
-        const int gr = threadIdx.x / LANES, e = 4 * (threadIdx.x % LANES);
+        for (int o = 32; o > 0; o >>= 1) sum += st::xor_lane(sum, o, lane);
+        if constexpr (WAVES > 1) {
+            if (lane == 0) stat[4 + wave] = sum;
+        }
+        meet();
+        if constexpr (WAVES > 1) sum = (stat[4] + stat[5]) + (stat[6] + stat[7]);
+        const int gr = me / LANES, e = 4 * (me % LANES);
         if (gr < GROUPS) {
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int i = gr; i < pl.chunks; i += GROUPS) {
+#pragma unroll 8
+            for (int i = gr; i < parts; i += GROUPS) {
                 const float w = weight[i];
-                const float4 x = *(const float4 *)(a.part_o + (slot + i) * HD + e);
+                const float4 x = *(const float4 *)(a.part_o + slot(i) * HD + e);
                 v.x += w * x.x, v.y += w * x.y, v.z += w * x.z, v.w += w * x.w;
             }
-            *(float4 *)&red[gr][e] = v;
+            *(float4 *)&red[team][gr][e] = v;
         }
-        __syncthreads();
+        meet();
         const float top = a.one ? fmaxf(m, 0.f) : m, f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-        const float sum = l * f + (a.one ? __builtin_amdgcn_exp2f(-top) : 0.f), inv = sum == 0.f ? 0.f : f / sum;
-        if ((int)threadIdx.x < HD) {
+        const float all = sum * f + (a.one ? __builtin_amdgcn_exp2f(-top) : 0.f), inv = all == 0.f ? 0.f : f / all;
+        for (int d = me; d < HD; d += 64 * WAVES) {
             float v = 0.f;
 #pragma unroll
-            for (int i = 0; i < GROUPS; i++) v += red[i][threadIdx.x];
+            for (int i = 0; i < GROUPS; i++) v += red[team][i][d];
             v *= inv;
-            const int64_t at = pair * HD + threadIdx.x;
+            const int64_t to = pair * HD + d;
             if (a.dtype == ST_F32)
-                ((float *)a.out)[at] = v;
+                ((float *)a.out)[to] = v;
             else if (a.dtype == ST_F16)
-                ((_Float16 *)a.out)[at] = (_Float16)v;
+                ((_Float16 *)a.out)[to] = (_Float16)v;
             else
-                ((__bf16 *)a.out)[at] = (__bf16)v;
+                ((__bf16 *)a.out)[to] = (__bf16)v;
         }
-        if (a.lse && threadIdx.x == 0) a.lse[pair] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+        if (a.lse && me == 0) a.lse[pair] = all == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(all)) * 0.693147180559945309f;
+        meet();  // the sums are read before the next pair's are written
     }
 }
 
-// How a call is cut: rows per wave, workgroups to aim at, and the partial rows that it can need.
+// How a call is cut: rows per wave, workgroups, and rows of a slot for parts (0: no unit is shared).
 struct Cut {
-    int rt, target;
-    int64_t part_rows;
+    int rt, groups, part_rows;
 };
 
 Cut cut_of(int64_t n, int64_t nseq, int64_t hq, int64_t hkv, int64_t hd, int64_t max_pages, int64_t page) {
     Cut c;
     // Sequences of many rows: 32 rows a wave, which share the work of taking codes apart.
     c.rt = hd <= 128 && n * (hq / hkv) >= 64 * nseq ? 2 : 1;
-    c.target = 4 * st::device_cus();
-    const int64_t keys = max_pages * page, tile = 64 * c.rt;
-    const int64_t chunks = std::min<int64_t>((keys + MIN_CHUNK - 1) / MIN_CHUNK, c.target + 2);
-    // A sequence of `chunks` > 1 chunks has at most twice as many as its share of the target.
-    c.part_rows = keys <= MIN_CHUNK ? 0 : std::min<int64_t>(n * hq * chunks, (int64_t)2 * c.target * tile + tile);
+    c.groups = std::min((c.rt == 1 && hd <= 128 ? 3 : 2) * st::device_cus(), MAX_GROUPS) & ~7;
+    c.part_rows = max_pages * page <= WHOLE ? 0 : (int)std::min<int64_t>(64 * c.rt, n * (hq / hkv));
     return c;
 }
+
+int64_t work_of(const Cut &c, int64_t hd) { return (int64_t)2 * c.groups * c.part_rows * (hd + 2) * 4; }
 
 }  // namespace
 
 extern "C" int64_t st_kv_attention_4bit_bytes(int64_t n, int64_t nseq, int64_t hq, int64_t hkv, int64_t hd, int64_t max_pages,
                                               int64_t page) {
     if (n <= 0 || nseq <= 0 || hkv <= 0 || hq < hkv || max_pages <= 0) return 0;
-    return cut_of(n, nseq, hq, hkv, hd, max_pages, page).part_rows * (hd + 2) * 4;
+    return work_of(cut_of(n, nseq, hq, hkv, hd, max_pages, page), hd);
 }
 
 extern "C" st_status st_kv_attention_4bit(const void *q, int32_t dtype, int64_t n, int64_t hq, int64_t hkv, int64_t hd,
@@ -687,41 +901,53 @@ extern "C" st_status st_kv_attention_4bit(const void *q, int32_t dtype, int64_t 
     const int64_t size = st::dtype_size(dtype);
     if (((uintptr_t)q | (uintptr_t)out) & (size - 1)) return st::fail(ST_ERR_INVALID, "%s: q or out not aligned to its elements", name);
     const Cut cut = cut_of(n, nseq, hq, hkv, hd, max_pages, page);
-    if (cut.part_rows > 0 && (!work || ((uintptr_t)work & 15) || work_bytes < cut.part_rows * (hd + 2) * 4))
+    if (cut.part_rows > 0 && (!work || ((uintptr_t)work & 15) || work_bytes < work_of(cut, hd)))
         return st::fail(ST_ERR_INVALID, "%s: work is %lld bytes of 16-byte aligned device memory, got %lld", name,
-                        (long long)(cut.part_rows * (hd + 2) * 4), (long long)(work ? work_bytes : 0));
+                        (long long)work_of(cut, hd), (long long)(work ? work_bytes : 0));
     if (!st::device_ok()) return ST_ERR_NO_DEVICE;
     a.q = q, a.out = out, a.lse = lse, a.q_start = q_start, a.kv_len = kv_len;
-    a.part_o = (float *)work, a.part_ml = (float2 *)((float *)work + cut.part_rows * hd), a.part_rows = cut.part_rows;
+    a.part_o = (float *)work, a.part_ml = (float2 *)((float *)work + (int64_t)2 * cut.groups * cut.part_rows * hd);
     a.q_stride = q_stride;
     a.scale2 = scale * 1.44269504088896341f;
     a.n = (int32_t)n, a.hq = (int32_t)hq, a.dtype = dtype, a.causal = causal != 0, a.one = one != 0;
     a.window = window > INT32_MAX / 2 ? 0 : (int32_t)window;
-    a.target = cut.target;
+    a.groups = cut.groups, a.part_rows = cut.part_rows;
+    a.share = (int32_t)(hq / hkv), a.cap = (int32_t)(max_pages * page);
+    a.per = a.share <= 64 * cut.rt ? 64 * cut.rt / a.share : 0;
+    a.tile_rows = a.per ? a.per * a.share : 64 * cut.rt;
+    const int64_t room = std::max(a.cap, 1);
+    a.most = (int32_t)(a.window > 0 ? std::min<int64_t>(room, (int64_t)a.window + std::max(a.per, 1) + 31) : room);
+    a.small = nseq <= 64 && (room + 64 * cut.rt) * hkv * nseq < INT32_MAX;
+    a.inv_share = 1.f / (float)a.share, a.inv_groups = 1.f / (float)cut.groups;
     a.vec_q = st::rows_aligned(q, q_stride, size), a.vec_out = ((uintptr_t)out & 15) == 0;
-    const int64_t tile = 64 * cut.rt, share = hq / hkv;
-    // Every tile once, and the target's worth of further chunks (a little more for the rounding of the f32 total).
-    const int64_t grid = hkv * (n * share / tile + nseq) + (cut.part_rows > 0 ? cut.target + cut.target / 64 + 64 : 0);
-    if (grid > INT32_MAX) return st::fail(ST_ERR_INVALID, "%s: %lld rows and %lld sequences are too many for one call", name, (long long)n, (long long)nseq);
     auto go = [&](auto hd_) -> st_status {
         constexpr int HD = decltype(hd_)::value;
         const hipStream_t s = st::stream_of(stream);
+        const uint32_t grid = cut.groups, pairs = (uint32_t)(n * hq);
+        // Few rows: a workgroup's four waves join one together; many: a wave each.
+        auto merge = [&] {
+            if (cut.part_rows == 0) return;
+            if (pairs <= 2048)
+                k_merge4<HD, 4><<<pairs, 256, 0, s>>>(a);
+            else
+                k_merge4<HD, 1><<<std::min(pairs / 4 + 1, 8 * grid), 256, 0, s>>>(a);
+        };
         if (cut.rt == 1) {
             if (dtype == ST_F32)
-                k_attention4<HD, 2, 1><<<(uint32_t)grid, 256, 0, s>>>(a);
+                k_attention4<HD, 2, 1><<<grid, 256, 0, s>>>(a);
             else
-                k_attention4<HD, 1, 1><<<(uint32_t)grid, 256, 0, s>>>(a);
+                k_attention4<HD, 1, 1><<<grid, 256, 0, s>>>(a);
+            ST_LAUNCH_CHECK();
+            merge();
         } else if constexpr (HD <= 128) {
             if (dtype == ST_F32)
-                k_attention4<HD, 2, 2><<<(uint32_t)grid, 256, 0, s>>>(a);
+                k_attention4<HD, 2, 2><<<grid, 256, 0, s>>>(a);
             else
-                k_attention4<HD, 1, 2><<<(uint32_t)grid, 256, 0, s>>>(a);
+                k_attention4<HD, 1, 2><<<grid, 256, 0, s>>>(a);
+            ST_LAUNCH_CHECK();
+            merge();
         }
         ST_LAUNCH_CHECK();
-        if (cut.part_rows > 0) {
-            k_merge4<HD><<<(uint32_t)std::min<int64_t>(n * hq, 8 * st::device_cus()), 256, 0, s>>>(a, (int)tile);
-            ST_LAUNCH_CHECK();
-        }
         return ST_OK;
     };
     switch (hd) {

@@ -99,6 +99,10 @@ __device__ __forceinline__ int32_t wave_incl_scan(int32_t x) {
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, int src) { return (uint32_t)__builtin_amdgcn_readlane((int)v, src); }
 __device__ __forceinline__ int32_t lane_value(int32_t v, int src) { return __builtin_amdgcn_readlane(v, src); }
 
+__device__ __forceinline__ int64_t lane_value64(int64_t v, int src) {
+    return (int64_t)((uint64_t)lane_value((uint32_t)((uint64_t)v >> 32), src) << 32 | lane_value((uint32_t)v, src));
+}
+
 // This lane's index in its wave64.
 __device__ __forceinline__ int lane_id() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
 
