@@ -428,8 +428,8 @@ st_status st_kv_append_4bit(const void *q, const void *k, const void *v, int32_t
 
 /* Bytes of device memory that st_kv_attention_4bit needs for these sizes (0:
  * none): partial results where a sequence's keys are shared among workgroups. */
-int64_t st_kv_attention_4bit_bytes(int64_t n, int64_t nseq, int64_t hq, int64_t hkv, int64_t hd,
-                                   int64_t max_pages, int64_t page);
+int64_t st_kv_attention_4bit_bytes(int32_t dtype, int64_t n, int64_t nseq, int64_t hq, int64_t hkv,
+                                   int64_t hd, int64_t max_pages, int64_t page);
 
 /* Attention of rows q [n, hq, hd] (rotated, q_stride elements apart) over the
  * cache: out[t, h] = softmax(scale q k^T) v with head h reading key head

@@ -473,6 +473,7 @@ extern "C" {
     ) -> st_status;
     /// Bytes of `work` that `st_kv_attention_4bit` needs.
     pub fn st_kv_attention_4bit_bytes(
+        dtype: i32,
         n: i64,
         nseq: i64,
         hq: i64,

@@ -945,9 +945,10 @@ impl<'a, H: DeviceBuffer + ?Sized> KvCache4bit<'a, H> {
     }
 
     /// Bytes of device memory that [`KvCache4bit::attention`] needs for n rows of hq heads.
-    pub fn attention_bytes(&self, n: usize, hq: usize) -> usize {
+    pub fn attention_bytes(&self, dtype: Dtype, n: usize, hq: usize) -> usize {
         unsafe {
             sys::st_kv_attention_4bit_bytes(
+                dtype.code(),
                 n as i64,
                 self.nseq as i64,
                 hq as i64,

@@ -89,7 +89,7 @@ SIGNATURES = {
     "st_matvec_4bit": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _vp],
     "st_kv_append_4bit": [_vp, _vp, _vp, _i32] + 7 * [_i64] + [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i32]
     + 8 * [_vp],
-    "st_kv_attention_4bit_bytes": 7 * [_i64],
+    "st_kv_attention_4bit_bytes": [_i32] + 7 * [_i64],
     "st_kv_attention_4bit": [_vp, _i32] + 5 * [_i64] + [_vp, _vp, _i64, _vp, _i64, _i64, _i64] + 4 * [_vp]
     + [_f32, _i32, _i64, _i32, _vp, _vp, _vp, _i64, _vp],
     "st_device_info": [_vp, _vp, _vp, _vp],

@@ -5,26 +5,29 @@
 //   z_j = scale (aK_j (q . (cK_j - 8)) + b8K_j sum q)       the score of key j
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(z_j log2 e - M),  M a reference of the row
 //   sum_j p_j v_j = sum_j (p_j aV_j) (cV_j - 8) + sum_j p_j b8V_j
-// Both products run on the matrix cores (v_mfma_f32_16x16x32_f16), codes as f16 integers from -8 to 7 (exact, a VALU
-// operation per code): around 0, so that the rounding of the weights p aV to f16 is not multiplied by an offset.  (Nibbles
-// masked in place are f16 subnormals n 2^-24, half the work, and the matrix cores take them; but they line up the sums
-// by the exponent that subnormals share, and lose the 6 to 10 bits that n leaves unused: 4e-5 off in f32.)
+// Both products run on the matrix cores, codes as f16 integers from -8 to 7 (exact, a VALU operation per code): around 0, so
+// that the rounding of the weights p aV to f16 is not multiplied by an offset.  (Nibbles masked in place are f16 subnormals n
+// 2^-24, half the work, and the matrix cores take them; but they line up the sums by the exponent that subnormals share,
+// and lose the 6 to 10 bits that n leaves unused: 4e-5 off in f32.)
 // Rows are scaled by a power of two to f16 (f32 rows, PARTS = 2, as two f16 parts, 22 bits), scores and sums are f32; the
-// weights are rounded to f16, in two parts for f32 rows.
+// weights are rounded to f16, in two parts for f32 rows.  A row's reference M is no running maximum of its scores but follows
+// max(z log2 e + log2 aV), so that p aV stays inside f16's normal range whatever the sizes of the values; it is raised only
+// where p aV would pass 2^15, so the common tile has no reduction over lanes at all.
 //
-// A wave holds 16 RT rows (queries x the heads that share a key head) and takes 32 keys at a time: S^T = K Q^T gives
-// each lane 8 scores of one row, which are its B operand of O^T = V^T P^T without a move between lanes.  A row's
-// reference M is no running maximum of its scores but follows max(z log2 e + log2 aV), so that p aV stays inside f16's
-// normal range whatever the sizes of the values; it is raised only where p aV would pass 2^15, so the common tile has no
-// reduction over lanes at all.
-// V's operand wants 8 keys of one component in a lane: a lane reads a word (8 components) of 8 keys and v_perm pairs
-// their bytes.
+// Two kernels.  What they spend is the taking apart of codes, about a VALU operation each for K and for V, and the
+// scores' arithmetic; both would leave memory waiting, so the rest is arranged around them:
+//  - k_attention4 (prompts, many rows): a wave has 16 RT rows and takes 32 keys at a time.  S^T = K Q^T (16x16x32) gives a lane
+//    8 scores of one row, which are its B operand of O^T = V^T P^T without a move between lanes.
+//  - k_decode4 (up to 8 rows: a token or two of a sequence): in 16 columns most would stand empty, and their scores cost
+//    the same.  S = Q K^T as 16 blocks of 4x4x4: a lane has one of 64 keys and its scores of 4 rows, all of them wanted.
+// V's operand wants 8 keys of one component in a lane: a lane reads a word (8 components) of 8 keys and v_perm pairs their
+// bytes.  Tiles come by LDS DMA into a ring of each wave's own, two ahead and waited for by their number, no barrier.
 //
-// Work is cut on the device, where the lengths are.  A unit is a tile of up to 64 RT rows of one sequence and key head with
-// the keys that it sees; the units of all sequences stand one behind the other on a line of keys, which the launch's
-// workgroups (two to a CU) divide evenly.  A workgroup of 4 waves goes through its stretch of the line unit by unit; waves
-// without rows of their own share the unit's keys (a single token's rows: all four).  What a workgroup has of a unit
-// that others work on too goes to its slots in `work`, and k_merge4 joins the parts.
+// Work is cut on the device, where the lengths are.  A unit is a tile of rows of one sequence and key head with the keys that
+// it sees; the units of all sequences stand one behind the other on a line of keys (each with a lead for what its start
+// costs), which the launch's workgroups, as many as are resident at once, divide evenly.  A workgroup of 4 waves goes
+// through its stretch of the line unit by unit; waves without rows of their own share the unit's keys.  What a workgroup
+// has of a unit that others work on too goes to its slots in `work`, and k_merge4 joins the parts.
 #include <algorithm>
 #include <cmath>
 
@@ -43,11 +46,22 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int MIN_STRETCH = 128;  // keys of a workgroup's stretch: less is not worth its start
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+constexpr int MIN_STRETCH = 256;  // of the line for a workgroup at least
+// What a unit's start costs (finding it, its rows, its first loads, its end), in keys: 64 ragged sequences take 122, 98, 88, 82
+// and 87 us at 0, 256, 512, 768 and 1536 with k_decode4; prompts, whose keys cost more, 591, 558 and 588 us at 256, 512 and 768.
+constexpr int LEAD_DECODE = 768, LEAD_ROWS = 512;
 constexpr int WHOLE = 512;        // units of up to so many keys are not shared among workgroups: a merge would cost more
 constexpr int MAX_GROUPS = 1024;  // workgroups of a launch
 constexpr float BASE = 7.f, MOST_X = 32768.f;  // p aV is set to 2^7 at most, and may grow to 2^15
 constexpr float MIN_E = -86.f, MOST_P = 101.f;  // values below 2^-86 of scale count as that for the reference: p <= 2^93, 2^101
+
+// What k_merge4 joins: a unit's rows, the first of them head `head` of token `token`; the first part is in the odd slot of the
+// workgroup that this stands under, the others in the even slots of those behind it.
+struct Joint {
+    int parts, rows, token, head;
+};
 
 struct AttnArgs {
     Cache c;
@@ -57,11 +71,13 @@ struct AttnArgs {
     const int32_t *q_start, *kv_len;
     float *part_o;    // [2 groups, part_rows, hd] sums of parts of units
     float2 *part_ml;  // [2 groups, part_rows] their references and totals
+    Joint *joints;    // [groups]
     int64_t q_stride;
     float scale2;  // scale log2 e
     int32_t n, hq, dtype, causal, window, one, groups, part_rows;
     int32_t share, cap;      // query heads of a key head, tokens of a table's row
     int32_t per, tile_rows;  // tokens (0: less than one) and rows of a tile
+    int32_t lead;            // of each unit on the line
     int32_t most, small;     // the most keys that a tile sees; whether the line's positions fit 32 bits
     float inv_share, inv_groups;
     bool vec_q, vec_out;
@@ -78,21 +94,32 @@ __device__ __forceinline__ int quotient(int64_t x, int64_t y) {
     return q;
 }
 
-// A wave's copy, in LDS, of what the line's position needs of 64 sequences: registers are for tiles.
+// What the line's position needs of 64 sequences.
 struct Rows {
-    int64_t upto[64], head[64];  // keys on the line up to a sequence's end from the first of the 64 on, and those of one head
+    int64_t upto[64], head[64];  // the line up to a sequence's end from the first of the 64 on, and of one of its heads
     int first[64], rows[64], len[64], tiles[64];
 };
 
-// The line of keys: how units lie on it.
+// What a workgroup does next: keys cut0 .. cut1 of a unit (none: it is done).  `parts`: of how many workgroups the unit is, where
+// this one has its first part and not all of it, else 0.
+struct Task {
+    int cut0, cut1, keys, first, rows, len, head, tile, me, parts, s;
+};
+constexpr int TASK_WORDS = sizeof(Task) / 4;
+
+// The line of keys, how units lie on it, and the workgroup's stretch of it.  Its first wave's.
 struct Line {
     const AttnArgs &a;
     Rows &m;
     int lane;
-    // `m` holds the 64 sequences from s0 on, `before` the line's keys before them, `inside` theirs.
+    // `m` holds the 64 sequences from s0 on, `before` the line before them, `inside` theirs.
     int64_t s0 = 0, before = 0, inside = 0, length = 0, stretch = 0;
+    int64_t at = 0, from = 0, to = 0, me = 0;
+    int slot = 0;  // of the launch's workgroups, those without a stretch too
 
-    __device__ __forceinline__ Line(const AttnArgs &args, Rows &mem, int lane_) : a(args), m(mem), lane(lane_) {
+    __device__ __forceinline__ Line(const AttnArgs &args, Rows &mem, int lane_) : a(args), m(mem), lane(lane_) {}
+
+    __device__ __forceinline__ void lay() {
         for (;; s0 += 64) {
             load();
             length += inside;
@@ -105,14 +132,15 @@ struct Line {
         if (s0 > 0) s0 = 0, load();
     }
 
-    // Keys of a sequence's first j tiles of `tiles` (an upper bound where a window or rows without keys make it less; a tile has
-    // one at least, so that each is some workgroup's).
-    __device__ __forceinline__ int64_t keys_of(int j, int tiles, int rows, int len) const {
+    // The line's part of a sequence's first j tiles of `tiles`: their leads and their keys (an upper bound where a window or rows
+    // without keys make it less; a tile has one at least, so that each is some workgroup's).
+    __device__ __forceinline__ int64_t part_of(int j, int tiles, int rows, int len) const {
         const int base = max(len - rows, 0), all = base + rows, most = a.most;
-        if (!a.causal || a.per == 0 || tiles == 1) return (int64_t)j * min(all, most);
+        const int64_t leads = (int64_t)j * a.lead;
+        if (!a.causal || a.per == 0 || tiles == 1) return leads + (int64_t)j * min(all, most);
         // Tile i ends at token min((i + 1) per, rows) and sees base + that many keys, `most` of them.
-        int64_t sum = 0;
-        if (j == tiles) sum = min(all, most), j--;
+        int64_t sum = leads;
+        if (j == tiles) sum += min(all, most), j--;
         const int64_t grow = min(j, most > base ? (most - base) / a.per : 0);
         return sum + grow * base + a.per * (grow * (grow + 1) / 2) + (j - grow) * most;
     }
@@ -130,11 +158,11 @@ struct Line {
         int64_t upto;
         if (a.small && !__any(rows > a.per)) {  // a tile each at most, and 32 bits suffice: a decoding step
             tiles = rows > 0 ? 1 : 0;
-            head = tiles ? min(max(len, rows), a.most) : 0;
+            head = tiles ? min(max(len, rows), a.most) + a.lead : 0;
             upto = st::wave_incl_scan((int)head * a.c.hkv);
         } else {
             tiles = a.per ? (rows + a.per - 1) / a.per : (int)(((int64_t)rows * a.share + a.tile_rows - 1) / a.tile_rows);
-            if (tiles > 0) head = keys_of(tiles, tiles, rows, len);
+            if (tiles > 0) head = part_of(tiles, tiles, rows, len);
             // Prefix sums in two halves of 20 and more bits.
             const int64_t here = head * a.c.hkv;
             const int lo = st::wave_incl_scan((int)(here & 0xFFFFF)), hi = st::wave_incl_scan((int)(here >> 20));
@@ -147,11 +175,11 @@ struct Line {
 
     // A unit on the line.
     struct Unit {
-        int64_t s, start;  // sequence, first position
+        int64_t s, start;  // sequence, position of its first key
         int keys, first, rows, len, tiles, head, tile;
     };
 
-    // Fills in `u` what goes by its sequence (the l-th of the 64): returns its first position, and the keys of a head.
+    // Fills in `u` what goes by its sequence (the l-th of the 64): returns its first position, and the line's part of a head.
     __device__ __forceinline__ int64_t take(int l, Unit &u, int64_t &head) const {
         u.s = s0 + l;
         u.first = uniform(m.first[l]), u.rows = uniform(m.rows[l]), u.len = uniform(m.len[l]), u.tiles = uniform(m.tiles[l]);
@@ -162,27 +190,27 @@ struct Line {
     __device__ __forceinline__ void place(Unit &u, int64_t head_start, int tile) const {
         u.tile = uniform(tile);
         if (u.tiles == 1) {
-            u.start = head_start, u.keys = min(max(u.len, u.rows), a.most);
+            u.start = head_start + a.lead, u.keys = min(max(u.len, u.rows), a.most);
             return;
         }
-        const int64_t from = keys_of(u.tile, u.tiles, u.rows, u.len);
-        u.start = head_start + from;
-        u.keys = uniform((int)(keys_of(u.tile + 1, u.tiles, u.rows, u.len) - from));
+        const int64_t ahead = part_of(u.tile, u.tiles, u.rows, u.len);
+        u.start = head_start + ahead + a.lead;
+        u.keys = uniform((int)(part_of(u.tile + 1, u.tiles, u.rows, u.len) - ahead) - a.lead);
     }
 
-    // The unit at `at` (not before the last one asked for).
-    __device__ __forceinline__ Unit unit_at(int64_t at) {
-        while (at >= before + inside) before += inside, s0 += 64, load();
-        const int l = __ffsll((unsigned long long)__ballot(before + m.upto[lane] > at)) - 1;
+    // The unit that position `x` belongs to (not before the last one asked for).
+    __device__ __forceinline__ Unit unit_at(int64_t x) {
+        while (x >= before + inside) before += inside, s0 += 64, load();
+        const int l = __ffsll((unsigned long long)__ballot(before + m.upto[lane] > x)) - 1;
         Unit u;
         int64_t each;
         const int64_t base = take(l, u, each);
-        u.head = uniform(quotient(at - base, each));
-        const int64_t off = at - base - u.head * each;
-        int lo = 0, hi = u.tiles - 1;  // the last tile whose start is not behind `off`
+        u.head = uniform(quotient(x - base, each));
+        const int64_t off = x - base - u.head * each;
+        int lo = 0, hi = u.tiles - 1;  // the last tile whose lead does not begin behind `off`
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
-            if (keys_of(mid, u.tiles, u.rows, u.len) <= off)
+            if (part_of(mid, u.tiles, u.rows, u.len) <= off)
                 lo = mid;
             else
                 hi = mid - 1;
@@ -191,34 +219,138 @@ struct Line {
         return u;
     }
 
-    // The unit of row `row` (a token) and query head `i`, and the row's place in its tile; false if no sequence has the row.
-    __device__ __forceinline__ bool unit_of(int row, int i, Unit &u, int &at) {
-        if (a.c.nseq > 64) s0 = 0, before = 0, load();
-        for (;;) {
-            const int first = m.first[lane];
-            const uint64_t hit = __ballot(first <= row && row < first + m.rows[lane]);
-            if (hit) {
-                const int l = __ffsll((unsigned long long)hit) - 1;
-                int64_t each;
-                const int64_t base = take(l, u, each);
-                u.head = uniform(quotient(i, a.share));
-                const int r = (row - u.first) * a.share + i - u.head * a.share, tile = uniform(quotient(r, a.tile_rows));
-                at = r - tile * a.tile_rows;
-                place(u, base + u.head * each, tile);
-                return true;
-            }
-            if (s0 + 64 >= a.c.nseq) return false;
-            before += inside, s0 += 64, load();
-        }
-    }
-
-    // Where a workgroup's stretch, ending at line position `end`, ends within a unit: at a multiple of 128 of its keys.
+    // Where a stretch that ends at position `end` ends within a unit: at a multiple of 128 of its keys.
     __device__ __forceinline__ int cut(const Unit &u, int64_t end) const {
         const int64_t x = end - u.start;
         if (x <= 0) return 0;
         return u.keys <= WHOLE ? u.keys : (int)min((x + 127) & ~(int64_t)127, (int64_t)u.keys);
     }
+
+    // The workgroup's stretch.  Neighbouring ones go to one XCD (workgroups go round the 8 of them): units of a head share pages.
+    __device__ __forceinline__ void begin() {
+        lay();
+        const int used = uniform(quotient(length + stretch - 1, stretch)), each = (used + 7) / 8, row = blockIdx.x >> 3;
+        me = (int64_t)(blockIdx.x & 7) * each + row;
+        if (row >= each || me >= used) {
+            slot = row < each ? (int)me : (int)blockIdx.x;
+            return;
+        }
+        slot = (int)me;
+        from = at = me * stretch;
+        to = min(from + stretch, length);
+    }
+
+    __device__ __forceinline__ void next(Task &t) {
+        Unit u = {};
+        int cut0 = 0, cut1 = 0, parts = 0;
+        while (at < to && cut0 == cut1) {
+            u = unit_at(at);
+            at = u.start + u.keys;
+            cut0 = uniform(cut(u, from)), cut1 = uniform(cut(u, to));
+        }
+        if (cut0 == 0 && cut1 > 0 && cut1 < u.keys) {
+            const int last = quotient(u.start + u.keys - 1, stretch);
+            // The last one's share may be empty: its keys went to the one before.
+            parts = uniform(last - (int)me + (cut(u, last * stretch) < u.keys ? 1 : 0));
+        }
+        if (lane == 0) t = {cut0, cut1, u.keys, u.first, u.rows, u.len, u.head, u.tile, (int)me, parts, (int)u.s};
+    }
 };
+
+// The rows of a task's tile (a token's heads side by side, from head rem0 of token tok0 on) and the first key that they see.
+struct Span {
+    int rows, tok0, rem0, base, lo;
+    float inv_share;
+
+    __device__ __forceinline__ Span(const AttnArgs &a, const Task &u) : inv_share(a.inv_share) {
+        const int row0 = u.tile * a.tile_rows;
+        rows = min(a.tile_rows, u.rows * a.share - row0);
+        tok0 = a.per ? u.tile * a.per : uniform(quotient(row0, a.share)), rem0 = a.per ? 0 : row0 - tok0 * a.share;
+        base = u.len - u.rows + tok0;  // position of the first row (negative: more rows than tokens)
+        lo = a.window > 0 ? (int)(max((int64_t)0, (int64_t)base + 1 - a.window) & ~63) : 0;  // down to a tile's start
+    }
+    __device__ __forceinline__ int token_of(int x) const { return (int)(((float)(rem0 + x) + 0.5f) * inv_share); }  // of row x, from tok0 on
+    __device__ __forceinline__ int pos_of(const AttnArgs &a, const Task &u, int x) const { return a.causal ? base + token_of(x) : u.len - 1; }
+    // Element offset of row x in q, and its index in out's [n, hq].
+    __device__ __forceinline__ int64_t q_at(const AttnArgs &a, const Task &u, int x, int hd) const {
+        const int token = token_of(x);
+        return (int64_t)(u.first + tok0 + token) * a.q_stride + (int64_t)(u.head * a.share + rem0 + x - token * a.share) * hd;
+    }
+    __device__ __forceinline__ int64_t row_at(const AttnArgs &a, const Task &u, int x) const {
+        const int token = token_of(x);
+        return (int64_t)(u.first + tok0 + token) * a.hq + u.head * a.share + rem0 + x - token * a.share;
+    }
+};
+
+// The task from LDS, each word to a scalar register.
+__device__ __forceinline__ Task read_task(const Task &t, int lane) {
+    const int word = ((const int *)&t)[min(lane, TASK_WORDS - 1)];
+    Task u;
+#pragma unroll
+    for (int i = 0; i < TASK_WORDS; i++) ((int *)&u)[i] = st::lane_value(word, i);
+    return u;
+}
+
+__device__ __forceinline__ void load_q(const AttnArgs &a, int64_t at, float (&x)[8]) {
+    if (a.dtype == ST_F32)
+        st::load8((const float *)a.q + at, a.vec_q, x);
+    else if (a.dtype == ST_F16)
+        st::load8((const _Float16 *)a.q + at, a.vec_q, x);
+    else
+        st::load8((const __bf16 *)a.q + at, a.vec_q, x);
+}
+
+// The largest component's exponent in `most` (0 where it is 0 or not finite): a row is scaled by 2^(15 - it).
+__device__ __forceinline__ int lift_of(float most) {
+    return most > 0.f && __builtin_isfinite(most) ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+}
+
+// The waves' sums of a tile's rows, each against the wave's own reference, joined: to out, or to the workgroup's slot of a
+// unit that others work on too.  `sums` [4 waves][wave_rows][hd + 4], `ml` [4][wave_rows]; `sharing` waves have the same rows.
+template <int HD>
+__device__ __forceinline__ void finish(const AttnArgs &a, const Task &u, const Span &span, const float *sums, const float2 *ml, int wave_rows,
+                                       int sharing) {
+    for (int i = threadIdx.x; i < span.rows * (HD / 8); i += 256) {
+        const int y = i / (HD / 8), e = 8 * (i % (HD / 8)), w0 = y / wave_rows * sharing, z = y % wave_rows;
+        float2 t[4];
+        float m = -INFINITY, l = 0.f, v[8] = {};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            t[k] = ml[min(w0 + k, 3) * wave_rows + z];
+            if (k >= sharing) t[k] = make_float2(-INFINITY, 0.f);
+            m = fmaxf(m, t[k].x);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float f = t[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t[k].x - m);
+            l += t[k].y * f;
+            if (k < sharing) {
+                float w[8];
+                st::load8(sums + ((w0 + k) * wave_rows + z) * (HD + 4) + e, true, w);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(w[j], f, v[j]);
+            }
+        }
+        if (u.cut0 > 0 || u.cut1 < u.keys) {
+            const int64_t slot = (2 * (int64_t)u.me + (u.cut0 == 0 ? 1 : 0)) * a.part_rows + y;
+            st::store8(a.part_o + slot * HD + e, true, v);
+            if (e == 0) a.part_ml[slot] = make_float2(m, l);
+            continue;
+        }
+        const int64_t row = span.row_at(a, u, y);
+        const float top = a.one ? fmaxf(m, 0.f) : m, f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        const float sum = l * f + (a.one ? __builtin_amdgcn_exp2f(-top) : 0.f), inv = sum == 0.f ? 0.f : f * __builtin_amdgcn_rcpf(sum);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] *= inv;
+        if (a.dtype == ST_F32)
+            st::store8((float *)a.out + row * HD + e, a.vec_out, v);
+        else if (a.dtype == ST_F16)
+            st::store8((_Float16 *)a.out + row * HD + e, a.vec_out, v);
+        else
+            st::store8((__bf16 *)a.out + row * HD + e, a.vec_out, v);
+        if (a.lse && e == 0) a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+    }
+}
 
 // The head's components in blocks of 128, 64 or 32: lane column c of a block of width W reads W / 16 components from
 // W / 16 c on, which lie in one word.
@@ -226,69 +358,6 @@ constexpr int block_width(int hd, int b) {
     return b == 0 ? (hd >= 128 ? 128 : hd >= 64 ? 64 : 32) : hd == 96 ? 32 : hd == 192 ? 64 : hd == 256 ? 128 : 0;
 }
 constexpr int blocks_of(int hd) { return block_width(hd, 1) ? 2 : 1; }
-
-// A wave's ring of tiles in LDS.  A tile (32 keys: their codes and (scale, lo) pairs, in two halves of 16 keys, which a page may
-// end between) is brought by DMA in chunks of 16 bytes: of K, then of V, then the pairs of K and of V.  A chunk's place is
-// 16 bytes times its number; which chunk of memory it is, is the lane's choice:
-//  - K of 128 and 256 components: in the order that lanes read their fragments in (lane (col, g) key col's 16 bytes from
-//    piece g, or 2 g + i, on), which no bank is hit twice by; else key by key;
-//  - V: rows in the order 0 4 8 12 1 5 .., so that the four keys that a read takes lie side by side.
-template <int HD>
-struct Ring {
-    static constexpr int NW = HD / 32, NB = blocks_of(HD);
-    static constexpr int PER_KEY = HD / 32, HALF = 16 * PER_KEY;                    // chunks
-    static constexpr int LOADS = (2 * HD + 32 + 63) / 64, BYTES = 1024 * LOADS;    // of a tile
-    static constexpr bool EVEN = HD == 128 || HD == 256;                            // a load is of one half of K or of V
-    static constexpr int PAIRS = 32 * HD;                                           // byte offset of the pairs
-
-    // Source byte offset of chunk `n` of a half of K or V.
-    static __device__ __forceinline__ int source(int n, bool v) {
-        if (v) {
-            const int slot = n / PER_KEY;
-            return (4 * (slot & 3) + (slot >> 2)) * (HD / 2) + 16 * (n % PER_KEY);
-        }
-        if (HD == 128) return (n & 15) * (HD / 2) + 16 * (n >> 4);
-        if (HD == 256) return (n & 15) * (HD / 2) + 16 * (2 * ((n >> 4) & 3) + (n >> 6));
-        return n / PER_KEY * (HD / 2) + 16 * (n % PER_KEY);
-    }
-
-    // This lane's words of K's half `half`.
-    static __device__ __forceinline__ void k_words(const char *tile, int half, int lane, uint32_t (&w)[NW]) {
-        typedef uint32_t v2 __attribute__((ext_vector_type(2)));
-        const int col = lane & 15, g = lane >> 4;
-        if constexpr (EVEN) {
-#pragma unroll
-            for (int i = 0; i < NW; i += 4) {
-                const u4 x = *(const u4 *)(tile + 16 * (HALF * half + 16 * i + lane));
-                w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
-            }
-        } else {
-            const char *p = tile + 16 * HALF * half + col * (HD / 2) + g * (HD / 8);
-            if constexpr (NW % 2 == 0) {
-#pragma unroll
-                for (int i = 0; i < NW; i += 2) {
-                    const v2 x = *(const v2 *)(p + 4 * i);
-                    w[i] = x[0], w[i + 1] = x[1];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < NW; i++) w[i] = *(const uint32_t *)(p + 4 * i);
-            }
-        }
-    }
-
-    // This lane's word of block b of value 4 g + r of half `half`.
-    static __device__ __forceinline__ uint32_t v_word(const char *tile, int half, int b, int r, int lane) {
-        const int col = lane & 15, g = lane >> 4, width = block_width(HD, b), start = b ? block_width(HD, 0) : 0;
-        const int off = start / 2 + 4 * (width == 128 ? col : width == 64 ? col >> 1 : col >> 2);
-        return *(const uint32_t *)(tile + 16 * (HD + HALF * half) + (4 * r + g) * (HD / 2) + off);
-    }
-
-    // The (scale, lo) pairs of keys (or values) 4 g + 2 i and the next of half `half`.
-    static __device__ __forceinline__ float4 pairs(const char *tile, bool v, int half, int i, int g) {
-        return *(const float4 *)(tile + PAIRS + 256 * v + 128 * half + 32 * g + 16 * i);
-    }
-};
 
 // 16 bytes a lane from scalar base + lane offset, or from a lane's address, to LDS from `to` on.  In assembly, so that the
 // compiler does not wait for every load in flight before any LDS read: a tile's loads are waited for by their number.
@@ -345,53 +414,158 @@ struct Taker {
     __device__ __forceinline__ h8 codes8(uint32_t w) const { return as_h8(lower(w), upper(w), lower(w >> 8), upper(w >> 8)); }
 };
 
+// O^T += V^T P^T for 32 keys: `word(b, i)` is this lane's word of block b of the i-th of its 8 keys, ph (and pr, the weights'
+// second parts) its 8 weights of each 16 rows.
+template <int HD, int PARTS, int RT, class Word>
+__device__ __forceinline__ void weigh_values(const Taker &take, const Word &word, const h8 (&ph)[RT], const h8 (&pr)[PARTS == 2 ? RT : 1], int col,
+                                             f4 (&o)[RT][HD / 16]) {
+#pragma unroll
+    for (int b = 0; b < blocks_of(HD); b++) {
+        constexpr int first = block_width(HD, 0) / 16;
+        const int width = block_width(HD, b);
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = word(b, i);
+#pragma unroll
+        for (int i = 0; i < width / 32; i++) {
+            const int byte = width == 128 ? i : width == 64 ? 2 * (col & 1) + i : col & 3;
+            const uint32_t sel = 0x0c000c00u | (uint32_t)(4 + byte) << 16 | (uint32_t)byte;
+            const uint32_t x0 = __builtin_amdgcn_perm(w[1], w[0], sel), x1 = __builtin_amdgcn_perm(w[3], w[2], sel);
+            const uint32_t x2 = __builtin_amdgcn_perm(w[5], w[4], sel), x3 = __builtin_amdgcn_perm(w[7], w[6], sel);
+            const h8 even = as_h8(take.lower(x0), take.lower(x1), take.lower(x2), take.lower(x3));
+            const h8 odd = as_h8(take.upper(x0), take.upper(x1), take.upper(x2), take.upper(x3));
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                f4 &e = o[rt][b * first + 2 * i], &d = o[rt][b * first + 2 * i + 1];
+                e = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph[rt], e, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph[rt], d, 0, 0, 0);
+                if constexpr (PARTS == 2) {
+                    e = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pr[rt], e, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pr[rt], d, 0, 0, 0);
+                }
+            }
+        }
+    }
+}
+
+// This lane's byte offset in a row of codes of its word of block b.
+template <int HD>
+__device__ __forceinline__ int word_at(int b, int col) {
+    const int width = block_width(HD, b), start = b ? block_width(HD, 0) : 0;
+    return start / 2 + 4 * (width == 128 ? col : width == 64 ? col >> 1 : col >> 2);
+}
+
+// Puts o [col = row][components] and `low`, which goes to every component of the row, to a row of a wave's sums.
+template <int HD>
+__device__ __forceinline__ void put_sums(float *row, const f4 (&o)[HD / 16], float low, int g) {
+#pragma unroll
+    for (int b = 0; b < blocks_of(HD); b++) {
+        constexpr int first = block_width(HD, 0) / 16;
+        const int per = block_width(HD, b) / 16, start = b ? block_width(HD, 0) : 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int j = 0; j < per; j++) row[start + per * (4 * g + r) + j] = o[b * first + j][r] + low;
+    }
+}
+
+// A wave's ring of tiles in LDS.  A tile (32 keys: their codes and (scale, lo) pairs, in two halves of 16 keys, which a page may
+// end between) is brought by DMA in chunks of 16 bytes: of K, then of V, then the pairs of K and of V.  A chunk's place is
+// 16 bytes times its number; which chunk of memory it is, is the lane's choice:
+//  - K of 128 and 256 components: in the order that lanes read their fragments in (lane (col, g) key col's 16 bytes from
+//    piece g, or 2 g + i, on), which no bank is hit twice by; else key by key;
+//  - V: rows in the order 0 4 8 12 1 5 .., so that the four keys that a read takes lie side by side.
+template <int HD>
+struct Ring {
+    static constexpr int NW = HD / 32;
+    static constexpr int PER_KEY = HD / 32, HALF = 16 * PER_KEY;                    // chunks
+    static constexpr int LOADS = (2 * HD + 32 + 63) / 64, BYTES = 1024 * LOADS;    // of a tile
+    static constexpr bool EVEN = HD == 128 || HD == 256;                            // a load is of one half of K or of V
+    static constexpr int PAIRS = 32 * HD;                                           // byte offset of the pairs
+
+    // Source byte offset of chunk `n` of a half of K or V.
+    static __device__ __forceinline__ int source(int n, bool v) {
+        if (v) {
+            const int slot = n / PER_KEY;
+            return (4 * (slot & 3) + (slot >> 2)) * (HD / 2) + 16 * (n % PER_KEY);
+        }
+        if (HD == 128) return (n & 15) * (HD / 2) + 16 * (n >> 4);
+        if (HD == 256) return (n & 15) * (HD / 2) + 16 * (2 * ((n >> 4) & 3) + (n >> 6));
+        return n / PER_KEY * (HD / 2) + 16 * (n % PER_KEY);
+    }
+
+    // This lane's words of K's half `half`.
+    static __device__ __forceinline__ void k_words(const char *tile, int half, int lane, uint32_t (&w)[NW]) {
+        typedef uint32_t v2 __attribute__((ext_vector_type(2)));
+        const int col = lane & 15, g = lane >> 4;
+        if constexpr (EVEN) {
+#pragma unroll
+            for (int i = 0; i < NW; i += 4) {
+                const u4 x = *(const u4 *)(tile + 16 * (HALF * half + 16 * i + lane));
+                w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
+            }
+        } else {
+            const char *p = tile + 16 * HALF * half + col * (HD / 2) + g * (HD / 8);
+            if constexpr (NW % 2 == 0) {
+#pragma unroll
+                for (int i = 0; i < NW; i += 2) {
+                    const v2 x = *(const v2 *)(p + 4 * i);
+                    w[i] = x[0], w[i + 1] = x[1];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NW; i++) w[i] = *(const uint32_t *)(p + 4 * i);
+            }
+        }
+    }
+
+    // The (scale, lo) pairs of keys (or values) 4 g + 2 i and the next of half `half`.
+    static __device__ __forceinline__ float4 pairs(const char *tile, bool v, int half, int i, int g) {
+        return *(const float4 *)(tile + PAIRS + 256 * v + 128 * half + 32 * g + 16 * i);
+    }
+};
+
 template <int HD, int PARTS, int RT>
 __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attention4(const AttnArgs a) {
     using R = Ring<HD>;
-    constexpr int NW = HD / 32, NB = blocks_of(HD), WAVE_ROWS = 16 * RT, LDO = HD + 4, STAGES = RT == 1 ? 2 : 3;
+    constexpr int NW = HD / 32, WAVE_ROWS = 16 * RT, LDO = HD + 4, STAGES = RT == 1 ? 2 : 3;
     constexpr int RING = 4 * STAGES * R::BYTES, SUMS = 4 * WAVE_ROWS * LDO * 4;
     __shared__ __align__(16) char mem[RING > SUMS ? RING : SUMS];  // the waves' rings, then their sums
     __shared__ float2 ml[4][WAVE_ROWS];
-    __shared__ Rows row_mem[4];
-    float(*red)[WAVE_ROWS][LDO] = (float(*)[WAVE_ROWS][LDO])mem;
+    __shared__ Rows row_mem;
+    __shared__ Task task;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const Cache &c = a.c;
-    Line line(a, row_mem[wave], lane);
-    const int share = a.share, cap = a.cap;
-    // Neighbouring stretches to one XCD (workgroups go round the 8 of them): units of a head share its pages.
-    const int used = uniform(quotient(line.length + line.stretch - 1, line.stretch)), each = (used + 7) / 8;
-    const int64_t me = (int64_t)(blockIdx.x & 7) * each + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= each || me >= used) return;
-    const int64_t line_end = min((me + 1) * line.stretch, line.length);
     const Taker take;
     char *ring = mem + wave * STAGES * R::BYTES;
     const uint32_t ring_at = uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)ring);
+    Line line(a, row_mem, lane);
+    Joint joint = {};
+    if (wave == 0) line.begin();
 
-  for (int64_t at = me * line.stretch; at < line_end;) {
-    const auto u = line.unit_at(at);
-    const int cut0 = uniform(line.cut(u, me * line.stretch)), cut1 = uniform(line.cut(u, line_end));
-    at = u.start + u.keys;
-    if (cut0 == cut1) continue;
-    // The tile's rows (a token's heads side by side) begin at head `rem0` of token tok0.
-    const int h = u.head, row0 = u.tile * a.tile_rows, rows = min(a.tile_rows, u.rows * share - row0);
-    const int tok0 = a.per ? u.tile * a.per : uniform(quotient(row0, share)), rem0 = a.per ? 0 : row0 - tok0 * share;
-    auto token_of = [&](int x) { return (int)(((float)(rem0 + x) + 0.5f) * a.inv_share); };  // of row x of the tile, from tok0 on
+  for (;;) {
+    if (wave == 0) line.next(task);
+    __syncthreads();
+    const Task u = read_task(task, lane);
+    if (u.cut0 == u.cut1) {
+        if (threadIdx.x == 0 && a.part_rows) a.joints[line.slot] = joint;
+        return;
+    }
+    const Span span(a, u);
+    if (u.parts > 1) joint = {u.parts, span.rows, u.first + span.tok0, u.head * a.share + span.rem0};
+    const int rows = uniform(span.rows), cap = a.cap;
     const int groups = (rows + WAVE_ROWS - 1) / WAVE_ROWS, sharing = groups == 1 ? 4 : groups == 2 ? 2 : 1;
     const int group = wave / sharing, turn = wave % sharing;
     const bool busy = group < groups;
 
     // This lane's row of each 16, and the positions of the group's first and last.
     int pos[RT];
-    const int base = u.len - u.rows + tok0;  // position of the first row (negative: more rows than tokens)
     const int first_row = group * WAVE_ROWS, last_row = min(first_row + WAVE_ROWS, rows) - 1;
-    const int pos_first = uniform(a.causal ? base + token_of(first_row) : u.len - 1);
-    const int pos_last = uniform(a.causal ? base + token_of(last_row) : u.len - 1);
+    const int pos_first = uniform(span.pos_of(a, u, first_row)), pos_last = uniform(span.pos_of(a, u, last_row));
 
     // The group's keys of this part: those that its first row may see up to those of its last, within the table.
-    const int tile_first = a.causal ? base : u.len - 1;
-    const int lo = a.window > 0 ? (int)(max((int64_t)0, (int64_t)tile_first + 1 - a.window) & ~31) : 0;
-    int begin = lo + cut0, end = min(pos_last + 1, cap);
-    if (cut1 < u.keys) end = min(end, lo + cut1);
+    int begin = span.lo + u.cut0, end = min(pos_last + 1, cap);
+    if (u.cut1 < u.keys) end = min(end, span.lo + u.cut1);
     if (a.window > 0) begin = max(begin, (int)(max((int64_t)0, (int64_t)pos_first + 1 - a.window) & ~31));
     begin = uniform(begin), end = uniform(end);
     const int first_key = uniform(begin + 32 * turn), step = 32 * sharing;
@@ -399,7 +573,7 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
     const bool no_pages = busy && c.pages == 0 && end > begin;
 
     // Pages of the next 32 tiles' halves, a half a lane: -1 one outside the cache, 0 (not looked at) behind the end.
-    const int page_rows = c.hkv * c.page, head_row = h * c.page;
+    const int page_rows = c.hkv * c.page, head_row = u.head * c.page;
     int entries = 0, entries_to = 0;
     uint32_t bad = 0;  // of the tiles in the ring, two bits each
     auto bring_tile = [&](int it, int slot) {
@@ -407,7 +581,7 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
             const int key = first_key + (it + (lane >> 1)) * step + 16 * (lane & 1);
             entries = 0;
             if (key < end) {
-                const int p = c.table[u.s * c.max_pages + (key >> c.page_log2)];
+                const int p = c.table[(int64_t)u.s * c.max_pages + (key >> c.page_log2)];
                 entries = p >= 0 && p < c.pages ? p : -1;
             }
             entries_to = it + 32;
@@ -449,27 +623,18 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const int r = first_row + 16 * rt + col;
-        const int token = token_of(min(r, rows - 1));
-        pos[rt] = a.causal ? base + token : u.len - 1;
+        pos[rt] = span.pos_of(a, u, min(r, rows - 1));
         float x[NW][8];
         float most = 0.f, sum = 0.f;
         bool finite = true;
+#pragma unroll
+        for (int w = 0; w < NW; w++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[w][i] = 0.f;
         if (busy && r < rows) {
-            const int64_t from = (int64_t)(u.first + tok0 + token) * a.q_stride + (h * share + rem0 + r - token * share) * HD + g * (HD / 4);
+            const int64_t from = span.q_at(a, u, r, HD) + g * (HD / 4);
 #pragma unroll
-            for (int w = 0; w < NW; w++) {
-                if (a.dtype == ST_F32)
-                    st::load8((const float *)a.q + from + 8 * w, a.vec_q, x[w]);
-                else if (a.dtype == ST_F16)
-                    st::load8((const _Float16 *)a.q + from + 8 * w, a.vec_q, x[w]);
-                else
-                    st::load8((const __bf16 *)a.q + from + 8 * w, a.vec_q, x[w]);
-            }
-        } else {
-#pragma unroll
-            for (int w = 0; w < NW; w++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[w][i] = 0.f;
+            for (int w = 0; w < NW; w++) load_q(a, from + 8 * w, x[w]);
         }
 #pragma unroll
         for (int w = 0; w < NW; w++)
@@ -485,7 +650,7 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
         sum += st::xor_lane(sum, 16, lane);
         sum += st::xor_lane(sum, 32, lane);
         // The row's largest component to 2^14 .. 2^15.
-        const int e = most > 0.f && __builtin_isfinite(most) ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+        const int e = lift_of(most);
         unscale[rt] = __builtin_amdgcn_ldexpf(a.scale2, -e);
         qsum[rt] = a.scale2 * sum, qsum8[rt] = 8.f * qsum[rt];
 #pragma unroll
@@ -508,15 +673,6 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
 #pragma unroll
         for (int j = 0; j < HD / 16; j++) o[rt][j] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    uint32_t sel[NB][4];
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int width = block_width(HD, b), byte = width == 128 ? i : width == 64 ? 2 * (col & 1) + (i & 1) : col & 3;
-            sel[b][i] = 0x0c000c00u | (uint32_t)(4 + byte) << 16 | (uint32_t)byte;
-        }
-
     auto process = [&](char *tile, int it, int bad_halves) {
         const int kt = first_key + it * step, key0 = kt + 4 * g;
         const bool masked = kt + 31 > pos_first || kt + 31 >= end || (a.window > 0 && kt <= pos_last - a.window);
@@ -652,35 +808,9 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
                     if constexpr (PARTS == 2) pr[rt][4 * i + r] = (_Float16)(xx - (float)ph[rt][4 * i + r]);
                 }
             }
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            constexpr int first = block_width(HD, 0) / 16;
-            const int bytes = block_width(HD, b) / 32;
-            uint32_t vw[2][4];
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) vw[i][r] = R::v_word(tile, i, b, r, lane);
-#pragma unroll
-            for (int i = 0; i < bytes; i++) {
-                const uint32_t x0 = __builtin_amdgcn_perm(vw[0][1], vw[0][0], sel[b][i]);
-                const uint32_t x1 = __builtin_amdgcn_perm(vw[0][3], vw[0][2], sel[b][i]);
-                const uint32_t x2 = __builtin_amdgcn_perm(vw[1][1], vw[1][0], sel[b][i]);
-                const uint32_t x3 = __builtin_amdgcn_perm(vw[1][3], vw[1][2], sel[b][i]);
-                const h8 even = as_h8(take.lower(x0), take.lower(x1), take.lower(x2), take.lower(x3));
-                const h8 odd = as_h8(take.upper(x0), take.upper(x1), take.upper(x2), take.upper(x3));
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    f4 &e = o[rt][b * first + 2 * i], &d = o[rt][b * first + 2 * i + 1];
-                    e = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph[rt], e, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph[rt], d, 0, 0, 0);
-                    if constexpr (PARTS == 2) {
-                        e = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pr[rt], e, 0, 0, 0);
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pr[rt], d, 0, 0, 0);
-                    }
-                }
-            }
-        }
+        weigh_values<HD, PARTS, RT>(take, [&](int b, int i) {  // keys 4 g .. of each half, whose rows lie in the order 0 4 8 12 1 ..
+            return *(const uint32_t *)(tile + 16 * (HD + R::HALF * (i >> 2)) + (4 * (i & 3) + g) * (HD / 2) + word_at<HD>(b, col));
+        }, ph, pr, col, o);
     };
 
     for (int it = 0, slot = 0; it < count; it++) {
@@ -708,177 +838,431 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
         if (g == 0) ml[wave][16 * rt + col] = make_float2(ref[rt], total[rt]);
     }
     __syncthreads();  // every ring is read
+    float *sums = (float *)mem;
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            constexpr int first = block_width(HD, 0) / 16;
-            const int per = block_width(HD, b) / 16, start = b ? block_width(HD, 0) : 0;
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int j = 0; j < per; j++) red[wave][16 * rt + col][start + per * (4 * g + r) + j] = o[rt][b * first + j][r] + low[rt];
-        }
+    for (int rt = 0; rt < RT; rt++) put_sums<HD>(sums + (wave * WAVE_ROWS + 16 * rt + col) * LDO, o[rt], low[rt], g);
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * (HD / 8); i += 256) {
-        const int y = i / (HD / 8), e = 8 * (i % (HD / 8)), w0 = y / WAVE_ROWS * sharing, z = y % WAVE_ROWS;
-        float2 t[4];
-        float m = -INFINITY, l = 0.f, v[8] = {};
+    finish<HD>(a, u, span, sums, &ml[0][0], WAVE_ROWS, sharing);
+    __syncthreads();  // the sums are read before the rings are filled again
+  }
+}
+
+// A wave's ring of tiles of 64 keys.  Chunks of 16 bytes: of K, of V, then the pairs of K and of V, a key's (lane's) 8 bytes each.
+//  - K: key by key, a lane reads its key's chunks; which of them comes first goes by the key, so that 8 lanes' reads of a
+//    chunk meet 8 different groups of banks;
+//  - V: rows of each 16 in the order 0 4 8 12 1 5 .., so that the four keys that a read takes lie side by side.
+template <int HD>
+struct Ring64 {
+    static constexpr int PER_KEY = HD / 32, LOADS = HD / 16 + 1, BYTES = 1024 * LOADS, VALUES = 32 * HD, PAIRS = 64 * HD;
+    static constexpr bool EVEN = PER_KEY == 4;  // a load is of 16 keys, which a page holds together
+
+    static __device__ __forceinline__ int turn(int key) { return PER_KEY == 4 ? (key >> 1) & 3 : PER_KEY == 2 ? (key >> 2) & 1 : 0; }
+    // Key and byte offset in its row of chunk n of K or V.
+    static __device__ __forceinline__ int key_of(int n, bool v) {
+        const int row = n / PER_KEY;
+        return v ? (row & ~15) + 4 * (row & 3) + ((row >> 2) & 3) : row;
+    }
+    static __device__ __forceinline__ int byte_of(int n, bool v) { return 16 * ((n % PER_KEY) ^ (v ? 0 : turn(n / PER_KEY))); }
+};
+
+// Up to 4 RG rows (RG = 1, 2) of a sequence over 64 keys at a time, a key a lane.
+template <int HD, int PARTS, int RG>
+__global__ __launch_bounds__(256, 2) void k_decode4(const AttnArgs a) {
+    using R = Ring64<HD>;
+    constexpr int ROWS = 4 * RG, LDO = HD + 4, STAGES = 2, LDP = 72;  // f16 of a row of weights
+    constexpr int RING = 4 * STAGES * R::BYTES, SUMS = 4 * ROWS * LDO * 4;
+    static_assert(RING >= SUMS && R::BYTES >= ROWS * HD * 2 * PARTS);
+    __shared__ __align__(16) char mem[RING];  // the waves' rings (at first their rows, at last their sums)
+    __shared__ __align__(16) _Float16 weights[4][PARTS][ROWS][LDP];
+    __shared__ float2 ml[4][ROWS];
+    __shared__ Rows row_mem;
+    __shared__ Task task;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    const Cache &c = a.c;
+    const Taker take;
+    char *ring = mem + wave * STAGES * R::BYTES;
+    const uint32_t ring_at = uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)ring);
+    Line line(a, row_mem, lane);
+    Joint joint = {};
+    if (wave == 0) line.begin();
+
+  for (;;) {
+    if (wave == 0) line.next(task);
+    __syncthreads();
+    const Task u = read_task(task, lane);
+    if (u.cut0 == u.cut1) {
+        if (threadIdx.x == 0 && a.part_rows) a.joints[line.slot] = joint;
+        return;
+    }
+    const Span span(a, u);
+    if (u.parts > 1) joint = {u.parts, span.rows, u.first + span.tok0, u.head * a.share + span.rem0};
+    const int rows = uniform(span.rows), cap = a.cap;
+    int pos[ROWS];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            t[k] = ml[min(w0 + k, 3)][z];
-            if (k >= sharing) t[k] = make_float2(-INFINITY, 0.f);
-            m = fmaxf(m, t[k].x);
+    for (int r = 0; r < ROWS; r++) pos[r] = uniform(span.pos_of(a, u, min(r, rows - 1)));
+    const int pos_first = pos[0], pos_last = uniform(span.pos_of(a, u, rows - 1));
+    int end = min(pos_last + 1, cap);
+    if (u.cut1 < u.keys) end = min(end, span.lo + u.cut1);
+    end = uniform(end);
+    const int first_key = uniform(span.lo + u.cut0 + 64 * wave);
+    const int count = uniform(c.pages > 0 && end > first_key ? (end - first_key + 255) / 256 : 0);
+    const bool no_pages = c.pages == 0 && end > span.lo + u.cut0;
+
+    // Pages of the next 16 tiles' quarters, a quarter a lane: -1 one outside the cache, 0 (not looked at) behind the end.
+    const int page_rows = c.hkv * c.page, head_row = u.head * c.page;
+    int entries = 0, entries_to = 0;
+    uint32_t bad = 0;  // of the tiles in the ring, four bits each
+    auto bring_tile = [&](int it, int slot) {
+        if (it >= entries_to) {
+            const int key = first_key + (it + (lane >> 2)) * 256 + 16 * (lane & 3);
+            entries = 0;
+            if (key < end) {
+                const int p = c.table[(int64_t)u.s * c.max_pages + (key >> c.page_log2)];
+                entries = p >= 0 && p < c.pages ? p : -1;
+            }
+            entries_to = it + 16;
         }
+        const int key = first_key + it * 256, i0 = 4 * (it + 16 - entries_to);
+        bad = (bad & ~(15u << (4 * slot))) | (uint32_t)((__ballot(entries < 0) >> i0) & 15) << (4 * slot);
+        int64_t row[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float f = t[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t[k].x - m);
-            l += t[k].y * f;
-            if (k < sharing) {
-                float w[8];
-                st::load8(&red[w0 + k][z][e], true, w);
+        for (int i = 0; i < 4; i++)
+            row[i] = (int64_t)max(st::lane_value(entries, i0 + i), 0) * page_rows + (head_row + ((key + 16 * i) & (c.page - 1)));
+        const uint32_t to = ring_at + slot * R::BYTES;
+        const bool one_page = c.page >= 64;
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(w[j], f, v[j]);
+        for (int i = 0; i < R::LOADS - 1; i++) {
+            const bool v = i >= HD / 32;
+            const int n = 64 * (v ? i - HD / 32 : i);
+            const uint8_t *codes = v ? c.v_codes : c.k_codes;
+            if constexpr (R::EVEN) {  // 16 keys of one quarter
+                bring(codes + row[n / 64] * (HD / 2), (R::key_of(n + lane, v) & 15) * (HD / 2) + R::byte_of(n + lane, v), to + 1024 * i);
+            } else if (one_page) {
+                bring(codes + row[0] * (HD / 2), R::key_of(n + lane, v) * (HD / 2) + R::byte_of(n + lane, v), to + 1024 * i);
+            } else {
+                const int k = R::key_of(n + lane, v), q = k >> 4;
+                const int64_t at = (q & 2 ? q & 1 ? row[3] : row[2] : q & 1 ? row[1] : row[0]) + (k & 15);
+                bring(codes + at * (HD / 2) + R::byte_of(n + lane, v), to + 1024 * i);
             }
         }
-        const int token = token_of(y);
-        const int64_t row = (int64_t)(u.first + tok0 + token) * a.hq + h * share + rem0 + y - token * share;
-        if (cut0 > 0 || cut1 < u.keys) {
-            const int64_t slot = (2 * me + (cut0 == 0 ? 1 : 0)) * a.part_rows + y;
-            st::store8(a.part_o + slot * HD + e, true, v);
-            if (e == 0) a.part_ml[slot] = make_float2(m, l);
-            continue;
-        }
-        const float top = a.one ? fmaxf(m, 0.f) : m, f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-        const float sum = l * f + (a.one ? __builtin_amdgcn_exp2f(-top) : 0.f), inv = sum == 0.f ? 0.f : f * __builtin_amdgcn_rcpf(sum);
+        const int q = (lane & 31) >> 3;
+        const int64_t at = (q & 2 ? q & 1 ? row[3] : row[2] : q & 1 ? row[1] : row[0]) + 2 * (lane & 7);
+        bring((lane < 32 ? c.k_scales : c.v_scales) + at, to + 1024 * (R::LOADS - 1));
+    };
+    // Rows: 16 lanes share one's components, find its largest, and leave it in LDS scaled to f16 for all lanes to read.
+    // Lane (block, row) of the 4 x 4 x 4 products holds row lane % 4 of each 4.
+    h4 qh[RG][HD / 4], ql[PARTS == 2 ? RG : 1][PARTS == 2 ? HD / 4 : 1];
+    float unscale[ROWS], qsum[ROWS];
+    {
+        _Float16 *stage = (_Float16 *)(ring + R::BYTES);  // the second tile's place, not yet under way
+        float xs[RG][8] = {};
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] *= inv;
-        if (a.dtype == ST_F32)
-            st::store8((float *)a.out + row * HD + e, a.vec_out, v);
-        else if (a.dtype == ST_F16)
-            st::store8((_Float16 *)a.out + row * HD + e, a.vec_out, v);
-        else
-            st::store8((__bf16 *)a.out + row * HD + e, a.vec_out, v);
-        if (a.lse && e == 0) a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+        for (int rg = 0; rg < RG; rg++) {
+            const int r = 4 * rg + (lane & 3), e0 = 8 * (lane >> 2);
+            if (r < rows && e0 < HD) load_q(a, span.q_at(a, u, r, HD) + e0, xs[rg]);
+        }
+        if (count > 0) bring_tile(0, 0);
+
+#pragma unroll
+        for (int rg = 0; rg < RG; rg++) {
+            const int r = 4 * rg + (lane & 3), block = lane >> 2, e0 = 8 * block;
+            const float(&x)[8] = xs[rg];
+            float most = 0.f, sum = 0.f;
+            bool finite = true;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                most = fmaxf(most, fabsf(x[i]));
+                sum += x[i];
+                finite = finite && __builtin_isfinite(x[i]);
+            }
+            sum = finite ? sum : NAN;  // a row that is not finite: its scores, and so its sums, are NaN
+#pragma unroll
+            for (int o = 4; o < 64; o <<= 1) most = fmaxf(most, st::xor_lane(most, o, lane)), sum += st::xor_lane(sum, o, lane);
+            const int e = lift_of(most);
+            const float un = __builtin_amdgcn_ldexpf(a.scale2, -e), qs = a.scale2 * sum;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {  // (lane i has row i)
+                unscale[4 * rg + i] = __builtin_bit_cast(float, st::lane_value(__builtin_bit_cast(uint32_t, un), i));
+                qsum[4 * rg + i] = __builtin_bit_cast(float, st::lane_value(__builtin_bit_cast(uint32_t, qs), i));
+            }
+            if (e0 < HD) {
+                constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+                h8 hi, lo_;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float y = __builtin_amdgcn_ldexpf(x[order[i]], e);
+                    hi[i] = (_Float16)y;
+                    lo_[i] = (_Float16)(y - (float)hi[i]);
+                }
+                *(h8 *)(stage + r * HD + e0) = hi;
+                if constexpr (PARTS == 2) *(h8 *)(stage + ROWS * HD + r * HD + e0) = lo_;
+            }
+        }
+
+#pragma unroll
+        for (int rg = 0; rg < RG; rg++)
+#pragma unroll
+            for (int w = 0; w < HD / 8; w++) {
+                const int r = 4 * rg + (lane & 3);
+                const h8 y = *(const h8 *)(stage + r * HD + 8 * w);
+                qh[rg][2 * w] = h4{y[0], y[1], y[2], y[3]}, qh[rg][2 * w + 1] = h4{y[4], y[5], y[6], y[7]};
+                if constexpr (PARTS == 2) {
+                    const h8 z = *(const h8 *)(stage + ROWS * HD + r * HD + 8 * w);
+                    ql[rg][2 * w] = h4{z[0], z[1], z[2], z[3]}, ql[rg][2 * w + 1] = h4{z[4], z[5], z[6], z[7]};
+                }
+            }
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the rows are read
+        asm volatile("" ::: "memory");
     }
+    if (count > 1) bring_tile(1, 1);
+
+    f4 o[1][HD / 16];
+    float ref[ROWS], total[ROWS], low[ROWS];  // sums in units of 2^ref (the same in all lanes), of this lane's keys
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) ref[r] = -INFINITY, total[r] = low[r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < HD / 16; j++) o[0][j] = f4{0.f, 0.f, 0.f, 0.f};
+
+    auto process = [&](char *tile, int it, int bad_quarters) {
+        const int kt = first_key + it * 256, key = kt + lane;
+        const bool masked = kt + 63 > pos_first || kt + 63 >= end || (a.window > 0 && kt <= pos_last - a.window);
+        float2 kp = *(const float2 *)(tile + R::PAIRS + 8 * lane), vp = *(const float2 *)(tile + R::PAIRS + 512 + 8 * lane);
+        bool careful = false;
+        if (masked || bad_quarters) {
+            // What lies behind the end counts nothing, whatever it holds; keys on a page outside the cache are NaN to the rows that
+            // see them; and a value that is not finite must not reach the rows that do not see it, as 0 times it.
+            const bool gone = bad_quarters >> (lane >> 4) & 1;
+            if (gone) kp = make_float2(NAN, NAN);
+            if (gone || key >= end) vp = make_float2(0.f, 0.f);
+            careful = __any(!__builtin_isfinite(vp.x + vp.y));
+        }
+        kp.y = __builtin_fmaf(8.f, kp.x, kp.y), vp.y = __builtin_fmaf(8.f, vp.x, vp.y);  // what a code of 8 stands for
+        // This key's scores of all rows, in log2.
+        auto scores = [&](const char *from, float (&z)[ROWS]) {
+            f4 s[RG];
+#pragma unroll
+            for (int rg = 0; rg < RG; rg++) s[rg] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int p = 0; p < R::PER_KEY; p++) {
+                const u4 w = *(const u4 *)(from + 16 * (lane * R::PER_KEY + (p ^ R::turn(lane))));
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const h8 k8 = take.codes8(w[j]);
+                    const h4 k0 = {k8[0], k8[1], k8[2], k8[3]}, k1 = {k8[4], k8[5], k8[6], k8[7]};
+#pragma unroll
+                    for (int rg = 0; rg < RG; rg++) {
+                        s[rg] = __builtin_amdgcn_mfma_f32_4x4x4f16(qh[rg][2 * (4 * p + j)], k0, s[rg], 0, 0, 0);
+                        s[rg] = __builtin_amdgcn_mfma_f32_4x4x4f16(qh[rg][2 * (4 * p + j) + 1], k1, s[rg], 0, 0, 0);
+                        if constexpr (PARTS == 2) {
+                            s[rg] = __builtin_amdgcn_mfma_f32_4x4x4f16(ql[rg][2 * (4 * p + j)], k0, s[rg], 0, 0, 0);
+                            s[rg] = __builtin_amdgcn_mfma_f32_4x4x4f16(ql[rg][2 * (4 * p + j) + 1], k1, s[rg], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) z[r] = __builtin_fmaf(kp.x, s[r >> 2][r & 3] * unscale[r], kp.y * qsum[r]);
+            if (masked) {
+#pragma unroll
+                for (int r = 0; r < ROWS; r++) z[r] = key <= pos[r] && key > (a.window > 0 ? pos[r] - a.window : -1) ? z[r] : -INFINITY;
+            }
+        };
+        // p = 2^(z - R) and p aV.  For the first tile, and where p aV would pass f16's range or p an f32's, the scores set R.
+        float p[ROWS], x[ROWS];
+        scores(tile, p);
+        float most_z = -INFINITY, most_x = 0.f;
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            x[r] = p[r] - ref[r];
+            most_z = fmaxf(most_z, x[r]);
+            x[r] = __builtin_amdgcn_exp2f(x[r]) * vp.x;
+            most_x = fmaxf(most_x, x[r]);
+        }
+        if (it == 0 || __any(most_z > MOST_P || most_x > MOST_X)) {
+            const float e = vp.x > 0.f ? fmaxf((float)__builtin_amdgcn_frexp_expf(vp.x), MIN_E) : MIN_E;
+            float mine = 1.f;  // what the sums of row `col` keep
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+                float m = p[r] + e;
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, st::xor_lane(m, o, lane));
+                m = fmaxf(ref[r], m - BASE);
+                const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref[r] - m);
+                total[r] *= keep, low[r] *= keep;
+                mine = col == r ? keep : mine;
+                ref[r] = m;
+            }
+#pragma unroll
+            for (int j = 0; j < HD / 16; j++) o[0][j] *= mine;
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            // (A row without a reference sees nothing here: minus infinity less itself is no number.)
+            float w = __builtin_amdgcn_exp2f(p[r] - ref[r]);
+            if (masked && p[r] == -INFINITY) w = 0.f;
+            total[r] += w;
+            float y = w * vp.x;
+            if (careful && w == 0.f)
+                y = 0.f;
+            else
+                low[r] = __builtin_fmaf(w, vp.y, low[r]);
+            const _Float16 hi = (_Float16)y;
+            weights[wave][0][r][lane] = hi;
+            if constexpr (PARTS == 2) weights[wave][1][r][lane] = (_Float16)(y - (float)hi);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; s++) {  // 32 keys: 4 g .. of two quarters
+            h8 ph[1], pr[1];
+            auto read = [&](int part) {
+                const _Float16 *from = &weights[wave][part][col % ROWS][32 * s + 4 * g];
+                const h4 lo = *(const h4 *)from, hi = *(const h4 *)(from + 16);
+                return h8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            };
+            ph[0] = read(0);
+            if constexpr (PARTS == 2) pr[0] = read(1);
+            weigh_values<HD, PARTS, 1>(take, [&](int b, int i) {
+                return *(const uint32_t *)(tile + R::VALUES + (16 * (2 * s + (i >> 2)) + 4 * (i & 3) + g) * (HD / 2) + word_at<HD>(b, col));
+            }, ph, pr, col, o);
+        }
+    };
+
+    for (int it = 0, slot = 0; it < count; it++, slot ^= 1) {
+        // This tile's loads are over when only those of the one behind it are under way (the last: when none is).
+        if (it + STAGES <= count)
+            dma::wait_vm<(STAGES - 1) * R::LOADS>();
+        else
+            dma::wait_vm<0>();
+        asm volatile("" ::: "memory");
+        process(ring + slot * R::BYTES, it, (bad >> (4 * slot)) & 15);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the tile's last reads are over before it is overwritten
+        if (it + STAGES < count) bring_tile(it + STAGES, slot);
+    }
+
+    float mine = 0.f;  // of row `col`
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) total[r] += st::xor_lane(total[r], o, lane), low[r] += st::xor_lane(low[r], o, lane);
+        // A row whose own token lies past the table (or that sees a token of a cache without pages).
+        if (pos[r] >= cap || no_pages) total[r] = NAN;
+        if (lane == r) ml[wave][r] = make_float2(ref[r], total[r]);
+        mine = col == r ? low[r] : mine;
+    }
+    __syncthreads();  // every ring is read
+    float *sums = (float *)mem;
+    if (col < ROWS) put_sums<HD>(sums + (wave * ROWS + col) * LDO, o[0], mine, g);
+    __syncthreads();
+    finish<HD>(a, u, span, sums, &ml[0][0], ROWS, 4);
     __syncthreads();  // the sums are read before the rings are filled again
   }
 }
 
 // Joins the parts of units that several workgroups worked on: out = sum 2^(M_i - M) O_i / sum 2^(M_i - M) l_i over a row's parts.
-// WAVES waves take a row and head: the first part is in the odd slot of the workgroup that has the unit's start, the
-// others in the even slots of those behind it.
+// Workgroup (i, j) has the unit that begins in the launch's workgroup i, and WAVES waves to each of its rows from j 4 / WAVES on.
 template <int HD, int WAVES>
 __global__ __launch_bounds__(256) void k_merge4(const AttnArgs a) {
     constexpr int LANES = HD / 4, GROUPS = 64 * WAVES / LANES, TEAMS = 4 / WAVES;
     __shared__ float weights[TEAMS][MAX_GROUPS + 8];
     __shared__ float red[TEAMS][GROUPS][HD], stat[8];
+    const Joint joint = a.joints[blockIdx.x];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), team = wave / WAVES;
-    const int me = threadIdx.x - team * 64 * WAVES;
-    __shared__ Rows row_mem[4];
-    Line line(a, row_mem[wave], lane);
-    auto meet = [&] {
-        if constexpr (WAVES > 1)
-            __syncthreads();
-        else
-            __builtin_amdgcn_wave_barrier();
-    };
+    const int me = threadIdx.x - team * 64 * WAVES, y = blockIdx.y * TEAMS + team, parts = min(joint.parts, MAX_GROUPS);
+    if (parts < 2 || y >= joint.rows || y >= a.part_rows) return;
     float *weight = weights[team];
-    const int64_t pairs = (int64_t)a.n * a.hq;
-    // A workgroup's waves go through as many pairs each, so that all meet.
-    for (int64_t p0 = (int64_t)blockIdx.x * TEAMS; p0 < pairs; p0 += (int64_t)gridDim.x * TEAMS) {
-        const int64_t pair = p0 + team;
-        Line::Unit u;
-        int place = 0;
-        const int row = (int)(min(pair, pairs - 1) / a.hq), head = (int)(min(pair, pairs - 1) - (int64_t)row * a.hq);
-        if (pair >= pairs || !line.unit_of(row, head, u, place) || u.keys <= WHOLE) continue;
-        const int w0 = uniform(quotient(u.start, line.stretch)), w1 = uniform(quotient(u.start + u.keys - 1, line.stretch));
-        if (w1 == w0) continue;
-        // The last one's share may be empty: its keys went to the one before.
-        const int parts = w1 - w0 + (line.cut(u, (int64_t)w1 * line.stretch) < u.keys ? 1 : 0);
-        if (parts == 1) continue;
-        auto slot = [&](int i) { return (2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0)) * a.part_rows + place; };
-        float m = -INFINITY, l = 0.f;
-        for (int i = me; i < parts; i += 64 * WAVES) {
-            const float2 t = a.part_ml[slot(i)];
-            weight[i] = t.x;
-            m = fmaxf(m, t.x);
-            if (i < 64 * WAVES) l = t.y;
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, st::xor_lane(m, o, lane));
-        if constexpr (WAVES > 1) {
-            if (lane == 0) stat[wave] = m;
-            __syncthreads();
-            m = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
-        }
-        float sum = 0.f;
-        for (int i = me; i < parts; i += 64 * WAVES) {
-            const float w = weight[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(weight[i] - m);
-            weight[i] = w;
-            sum += w * (i < 64 * WAVES ? l : a.part_ml[slot(i)].y);
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) sum += st::xor_lane(sum, o, lane);
-        if constexpr (WAVES > 1) {
-            if (lane == 0) stat[4 + wave] = sum;
-        }
-        meet();
-        if constexpr (WAVES > 1) sum = (stat[4] + stat[5]) + (stat[6] + stat[7]);
-        const int gr = me / LANES, e = 4 * (me % LANES);
-        if (gr < GROUPS) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int i = gr; i < parts; i += GROUPS) {
-                const float w = weight[i];
-                const float4 x = *(const float4 *)(a.part_o + slot(i) * HD + e);
-                v.x += w * x.x, v.y += w * x.y, v.z += w * x.z, v.w += w * x.w;
-            }
-            *(float4 *)&red[team][gr][e] = v;
-        }
-        meet();
-        const float top = a.one ? fmaxf(m, 0.f) : m, f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-        const float all = sum * f + (a.one ? __builtin_amdgcn_exp2f(-top) : 0.f), inv = all == 0.f ? 0.f : f / all;
-        for (int d = me; d < HD; d += 64 * WAVES) {
-            float v = 0.f;
-#pragma unroll
-            for (int i = 0; i < GROUPS; i++) v += red[team][i][d];
-            v *= inv;
-            const int64_t to = pair * HD + d;
-            if (a.dtype == ST_F32)
-                ((float *)a.out)[to] = v;
-            else if (a.dtype == ST_F16)
-                ((_Float16 *)a.out)[to] = (_Float16)v;
-            else
-                ((__bf16 *)a.out)[to] = (__bf16)v;
-        }
-        if (a.lse && me == 0) a.lse[pair] = all == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(all)) * 0.693147180559945309f;
-        meet();  // the sums are read before the next pair's are written
+    auto slot = [&](int i) { return (2 * (int64_t)min((int)blockIdx.x + i, a.groups - 1) + (i == 0 ? 1 : 0)) * a.part_rows + y; };
+    float m = -INFINITY, l = 0.f;
+    for (int i = me; i < parts; i += 64 * WAVES) {
+        const float2 t = a.part_ml[slot(i)];
+        weight[i] = t.x;
+        m = fmaxf(m, t.x);
+        if (i < 64 * WAVES) l = t.y;
     }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, st::xor_lane(m, o, lane));
+    if constexpr (WAVES > 1) {
+        if (lane == 0) stat[wave] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
+    }
+    float sum = 0.f;
+    for (int i = me; i < parts; i += 64 * WAVES) {
+        const float w = weight[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(weight[i] - m);
+        weight[i] = w;
+        sum += w * (i < 64 * WAVES ? l : a.part_ml[slot(i)].y);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += st::xor_lane(sum, o, lane);
+    if constexpr (WAVES > 1) {
+        if (lane == 0) stat[4 + wave] = sum;
+        __syncthreads();
+        sum = (stat[4] + stat[5]) + (stat[6] + stat[7]);
+    }
+    const int gr = me / LANES, e = 4 * (me % LANES);
+    if (gr < GROUPS) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = gr; i0 < parts; i0 += 8 * GROUPS) {  // eight loads under way
+            float4 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = *(const float4 *)(a.part_o + slot(min(i0 + k * GROUPS, parts - 1)) * HD + e);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float w = i0 + k * GROUPS < parts ? weight[i0 + k * GROUPS] : 0.f;
+                if (w != 0.f) v.x += w * x[k].x, v.y += w * x[k].y, v.z += w * x[k].z, v.w += w * x[k].w;
+            }
+        }
+        *(float4 *)&red[team][gr][e] = v;
+    }
+    if constexpr (WAVES > 1) __syncthreads();
+    const float top = a.one ? fmaxf(m, 0.f) : m, f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float all = sum * f + (a.one ? __builtin_amdgcn_exp2f(-top) : 0.f), inv = all == 0.f ? 0.f : f / all;
+    const int token = (int)(((float)(joint.head % a.share + y) + 0.5f) * a.inv_share);
+    const int64_t row = (int64_t)(joint.token + token) * a.hq + joint.head + y - token * a.share;
+    for (int d = me; d < HD; d += 64 * WAVES) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < GROUPS; i++) v += red[team][i][d];
+        v *= inv;
+        const int64_t to = row * HD + d;
+        if (a.dtype == ST_F32)
+            ((float *)a.out)[to] = v;
+        else if (a.dtype == ST_F16)
+            ((_Float16 *)a.out)[to] = (_Float16)v;
+        else
+            ((__bf16 *)a.out)[to] = (__bf16)v;
+    }
+    if (a.lse && me == 0) a.lse[row] = all == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(all)) * 0.693147180559945309f;
 }
 
-// How a call is cut: rows per wave, workgroups, and rows of a slot for parts (0: no unit is shared).
+// How a call is cut: the kernel (rows of a tile: 4 or 8 for k_decode4, else 64 rt), workgroups, and rows of a slot for parts of
+// units (0: none is shared).
 struct Cut {
-    int rt, groups, part_rows;
+    int rows, rt, groups, part_rows;
 };
 
-Cut cut_of(int64_t n, int64_t nseq, int64_t hq, int64_t hkv, int64_t hd, int64_t max_pages, int64_t page) {
+Cut cut_of(int32_t dtype, int64_t n, int64_t nseq, int64_t hq, int64_t hkv, int64_t hd, int64_t max_pages, int64_t page) {
     Cut c;
-    // Sequences of many rows: 32 rows a wave, which share the work of taking codes apart.
-    c.rt = hd <= 128 && n * (hq / hkv) >= 64 * nseq ? 2 : 1;
-    c.groups = std::min((c.rt == 1 && hd <= 128 ? 3 : 2) * st::device_cus(), MAX_GROUPS) & ~7;
-    c.part_rows = max_pages * page <= WHOLE ? 0 : (int)std::min<int64_t>(64 * c.rt, n * (hq / hkv));
+    const int64_t share = hq / hkv, parts = dtype == ST_F32 ? 2 : 1;
+    // By the rows of a sequence on average.  k_decode4 holds its rows in hd / 2 registers for each 4 of them and each part.
+    if (share <= 8 && n * share <= 4 * nseq && hd <= 128)
+        c.rows = 4, c.rt = 0;
+    else if (share <= 8 && n * share <= 8 * nseq && hd * parts <= 128)
+        c.rows = 8, c.rt = 0;
+    else
+        c.rt = hd <= 128 && n * share >= 64 * nseq ? 2 : 1, c.rows = 64 * c.rt;  // many rows: 32 a wave, which share the work of taking codes apart
+    const int per_cu = c.rt == 1 && hd <= 128 ? 3 : 2;
+    c.groups = std::min(per_cu * st::device_cus(), MAX_GROUPS) & ~7;
+    c.part_rows = max_pages * page <= WHOLE ? 0 : (int)std::min<int64_t>(c.rows, n * share);
     return c;
 }
 
-int64_t work_of(const Cut &c, int64_t hd) { return (int64_t)2 * c.groups * c.part_rows * (hd + 2) * 4; }
+int64_t work_of(const Cut &c, int64_t hd) { return c.part_rows ? (int64_t)2 * c.groups * c.part_rows * (hd + 2) * 4 + c.groups * sizeof(Joint) : 0; }
 
 }  // namespace
 
-extern "C" int64_t st_kv_attention_4bit_bytes(int64_t n, int64_t nseq, int64_t hq, int64_t hkv, int64_t hd, int64_t max_pages,
-                                              int64_t page) {
+extern "C" int64_t st_kv_attention_4bit_bytes(int32_t dtype, int64_t n, int64_t nseq, int64_t hq, int64_t hkv, int64_t hd,
+                                              int64_t max_pages, int64_t page) {
     if (n <= 0 || nseq <= 0 || hkv <= 0 || hq < hkv || max_pages <= 0) return 0;
-    return work_of(cut_of(n, nseq, hq, hkv, hd, max_pages, page), hd);
+    return work_of(cut_of(dtype, n, nseq, hq, hkv, hd, max_pages, page), hd);
 }
 
 extern "C" st_status st_kv_attention_4bit(const void *q, int32_t dtype, int64_t n, int64_t hq, int64_t hkv, int64_t hd,
@@ -900,53 +1284,60 @@ extern "C" st_status st_kv_attention_4bit(const void *q, int32_t dtype, int64_t 
     if (!q || !q_start || !kv_len || !out) return st::fail(ST_ERR_INVALID, "%s: NULL buffer", name);
     const int64_t size = st::dtype_size(dtype);
     if (((uintptr_t)q | (uintptr_t)out) & (size - 1)) return st::fail(ST_ERR_INVALID, "%s: q or out not aligned to its elements", name);
-    const Cut cut = cut_of(n, nseq, hq, hkv, hd, max_pages, page);
+    const Cut cut = cut_of(dtype, n, nseq, hq, hkv, hd, max_pages, page);
     if (cut.part_rows > 0 && (!work || ((uintptr_t)work & 15) || work_bytes < work_of(cut, hd)))
         return st::fail(ST_ERR_INVALID, "%s: work is %lld bytes of 16-byte aligned device memory, got %lld", name,
                         (long long)work_of(cut, hd), (long long)(work ? work_bytes : 0));
     if (!st::device_ok()) return ST_ERR_NO_DEVICE;
     a.q = q, a.out = out, a.lse = lse, a.q_start = q_start, a.kv_len = kv_len;
     a.part_o = (float *)work, a.part_ml = (float2 *)((float *)work + (int64_t)2 * cut.groups * cut.part_rows * hd);
+    a.joints = (Joint *)(a.part_ml + (int64_t)2 * cut.groups * cut.part_rows);
     a.q_stride = q_stride;
     a.scale2 = scale * 1.44269504088896341f;
     a.n = (int32_t)n, a.hq = (int32_t)hq, a.dtype = dtype, a.causal = causal != 0, a.one = one != 0;
     a.window = window > INT32_MAX / 2 ? 0 : (int32_t)window;
     a.groups = cut.groups, a.part_rows = cut.part_rows;
     a.share = (int32_t)(hq / hkv), a.cap = (int32_t)(max_pages * page);
-    a.per = a.share <= 64 * cut.rt ? 64 * cut.rt / a.share : 0;
-    a.tile_rows = a.per ? a.per * a.share : 64 * cut.rt;
+    a.per = a.share <= cut.rows ? cut.rows / a.share : 0;
+    a.tile_rows = a.per ? a.per * a.share : cut.rows;
     const int64_t room = std::max(a.cap, 1);
-    a.most = (int32_t)(a.window > 0 ? std::min<int64_t>(room, (int64_t)a.window + std::max(a.per, 1) + 31) : room);
-    a.small = nseq <= 64 && (room + 64 * cut.rt) * hkv * nseq < INT32_MAX;
+    a.most = (int32_t)(a.window > 0 ? std::min<int64_t>(room, (int64_t)a.window + std::max(a.per, 1) + 63) : room);
+    a.lead = cut.rt == 0 ? LEAD_DECODE : LEAD_ROWS;
+    a.small = nseq <= 64 && (room + a.tile_rows + a.lead) * hkv * nseq < INT32_MAX;
     a.inv_share = 1.f / (float)a.share, a.inv_groups = 1.f / (float)cut.groups;
     a.vec_q = st::rows_aligned(q, q_stride, size), a.vec_out = ((uintptr_t)out & 15) == 0;
     auto go = [&](auto hd_) -> st_status {
         constexpr int HD = decltype(hd_)::value;
         const hipStream_t s = st::stream_of(stream);
-        const uint32_t grid = cut.groups, pairs = (uint32_t)(n * hq);
-        // Few rows: a workgroup's four waves join one together; many: a wave each.
+        const uint32_t grid = cut.groups;
+        // Few rows in a tile: a workgroup's four waves join one together; many: a wave each.
         auto merge = [&] {
             if (cut.part_rows == 0) return;
-            if (pairs <= 2048)
-                k_merge4<HD, 4><<<pairs, 256, 0, s>>>(a);
+            if (cut.part_rows <= 16)
+                k_merge4<HD, 4><<<dim3(grid, cut.part_rows), 256, 0, s>>>(a);
             else
-                k_merge4<HD, 1><<<std::min(pairs / 4 + 1, 8 * grid), 256, 0, s>>>(a);
+                k_merge4<HD, 1><<<dim3(grid, (cut.part_rows + 3) / 4), 256, 0, s>>>(a);
+        };
+        auto with = [&](auto kernel_f32, auto kernel) {
+            if (dtype == ST_F32)
+                kernel_f32<<<grid, 256, 0, s>>>(a);
+            else
+                kernel<<<grid, 256, 0, s>>>(a);
         };
         if (cut.rt == 1) {
-            if (dtype == ST_F32)
-                k_attention4<HD, 2, 1><<<grid, 256, 0, s>>>(a);
-            else
-                k_attention4<HD, 1, 1><<<grid, 256, 0, s>>>(a);
-            ST_LAUNCH_CHECK();
-            merge();
+            with(k_attention4<HD, 2, 1>, k_attention4<HD, 1, 1>);
         } else if constexpr (HD <= 128) {
-            if (dtype == ST_F32)
-                k_attention4<HD, 2, 2><<<grid, 256, 0, s>>>(a);
+            if (cut.rt == 2)
+                with(k_attention4<HD, 2, 2>, k_attention4<HD, 1, 2>);
+            else if (cut.rows == 4)
+                with(k_decode4<HD, 2, 1>, k_decode4<HD, 1, 1>);
+            else if constexpr (HD <= 64)
+                with(k_decode4<HD, 2, 2>, k_decode4<HD, 1, 2>);
             else
-                k_attention4<HD, 1, 2><<<grid, 256, 0, s>>>(a);
-            ST_LAUNCH_CHECK();
-            merge();
+                k_decode4<HD, 1, 2><<<grid, 256, 0, s>>>(a);
         }
+        ST_LAUNCH_CHECK();
+        merge();
         ST_LAUNCH_CHECK();
         return ST_OK;
     };

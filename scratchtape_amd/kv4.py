@@ -149,7 +149,7 @@ class KvCache4bit:
             if out is None:
                 out = torch.empty((n, hq, 2 * half), dtype=q.dtype, device=q.device)
             stats = torch.empty((n, hq), dtype=torch.float32, device=q.device) if lse else None
-            nbytes = int(_lib.lib().st_kv_attention_4bit_bytes(n, nseq, hq, heads, 2 * half, max_pages, page))
+            nbytes = int(_lib.lib().st_kv_attention_4bit_bytes(dtype, n, nseq, hq, heads, 2 * half, max_pages, page))
             work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
             _lib.call("st_kv_attention_4bit", q.data_ptr(), dtype, n, hq, heads, 2 * half, q_stride, q_start.data_ptr(),
                       kv_len.data_ptr(), nseq, table.data_ptr(), max_pages, pages, page,

@@ -322,8 +322,10 @@ def test_views_and_rows_of_no_sequence(dev, t):
         out = torch.full((12, 4, 64), 8.0, dtype=t, device=dev)
         assert cache.attention(q, table, start, ints(lens, dev), out=out) is out
         assert bool((out[:2] == 8).all()) and bool((out[6:] == 8).all())
-        want = cache.attention(q[2:6].contiguous(), table, ints([0, 3, 4], dev), ints(lens, dev))
-        assert torch.equal(out[2:6], want)
+        # (Which kernel runs goes by rows a sequence, n / sequences, so that a call of the four rows alone may add in another order:
+        # against 64 bits, not against its bits.)
+        part = 2 if t == torch.float32 else 1
+        check(out[2:6], None, oracle.attention(q[2:6], cache, table, ints([0, 3, 4], dev), ints(lens, dev), 64 ** -0.5, parts=part))
     assert cache.attention(fused[:0, :256].unflatten(-1, (4, 64)), table, ints([0, 0, 0], dev), ints(lens, dev)).shape == (0, 4, 64)
 
 
