@@ -1,5 +1,6 @@
 // 4-bit weights: the quantiser (the format is in quant4.h) and the products of a few rows with them.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "lanes.h"
@@ -30,36 +31,231 @@ __global__ __launch_bounds__(256) void k_quantise4(const T *__restrict__ x, int6
     }
 }
 
-// One wave per output: lane l takes every 64th run of 8 weights.
+// Products of 16 MB rows of x with 16 NT rows of weights a workgroup, the sums over k shared by its four waves.
+//
+// y = sum over groups of s (sum x c) + lo (sum x).  The first sum runs on the matrix cores (16x16x32, f32 sums): x is one
+// operand as it lies in memory (f16 and bf16), and a code is the f16 or bf16 number 16 + c, its four bits put under the
+// exponent of 16 by a shift and a v_and_or (a VALU operation per code), so that sum x c = sum x (16 + c) - 16 sum x loses two
+// bits of the f32 sum and not seven, as 1024 + c or 128 + c would.  sum x is one more product, with ones, which comes out
+// in the lanes that want it.  f32 rows are three bf16 parts of 8 bits each, taken off one after the other without rounding.
+//
+// Lane (i, q) of a wave reads 16 bytes (32 codes) of weight row i: 64 bytes of each of 16 rows a load.  For groups of 32
+// and 64 a product over 32 k has to stay inside a group: the four lanes of a row exchange words (a 4 x 4 transposition by
+// v_permlane swaps), so that lane q has the q-th 8 codes of each 32.  The lane of a row holds its scales; nothing goes
+// through LDS but the four waves' sums at the end.
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+constexpr int STEP = 128;  // k of a wave's step
+
 template <class T>
-__global__ __launch_bounds__(256) void k_matvec4(const T *__restrict__ x, int64_t m, int64_t k, int64_t x_stride,
-                                                 bool vec, const uint32_t *__restrict__ codes,
-                                                 const float2 *__restrict__ scales, int64_t group, int64_t n,
-                                                 const float *__restrict__ bias, bool relu, T *__restrict__ out,
-                                                 int64_t out_stride) {
-    const int64_t col = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (col >= n) return;
-    for (int64_t row = blockIdx.y; row < m; row += gridDim.y) {
-        float acc = 0.f;
-        for (int64_t i = lane; i < k / 8; i += 64) {
-            float v[8];
-            st::load8(x + row * x_stride + i * 8, vec, v);
-            const uint32_t c = codes[col * (k / 8) + i];
-            const float2 s = scales[col * (k / group) + i * 8 / group];
-            float dot = 0.f, sum = 0.f;
+constexpr int parts_of() { return sizeof(T) == 4 ? 3 : 1; }
+
+// One step's loads of a wave.
+template <class T, int GROUP, int NT, int MB>
+struct Step {
+    u4 codes[NT];
+    float2 scales[NT][STEP / GROUP];
+    u4 x[MB][4][sizeof(T) / 2];  // 8 elements for each of the four products
+};
+
+template <class T>
+__device__ __forceinline__ f4 product(u4 a, u4 b, f4 c) {
+    if constexpr (std::is_same_v<T, _Float16>)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+// Elements 0 1 .. 7 to the order 0 4 1 5 2 6 3 7 that a word's codes come out in.
+__device__ __forceinline__ u4 in_code_order(u4 x) {
+    return u4{__builtin_amdgcn_perm(x[2], x[0], 0x05040100), __builtin_amdgcn_perm(x[2], x[0], 0x07060302),
+              __builtin_amdgcn_perm(x[3], x[1], 0x05040100), __builtin_amdgcn_perm(x[3], x[1], 0x07060302)};
+}
+
+// The upper halves (bf16 parts) of two f32 words, the first below.
+__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
+
+template <class T, int GROUP, int NT, int MB>
+__global__ __launch_bounds__(256, 2) void k_matvec4(const T *__restrict__ x, int32_t m, int32_t k, int64_t x_stride, bool vec,
+                                                    const uint8_t *__restrict__ codes, const float2 *__restrict__ scales,
+                                                    int64_t n, const float *__restrict__ bias, bool relu, T *__restrict__ out,
+                                                    int64_t out_stride) {
+    constexpr int PARTS = parts_of<T>(), G = STEP / GROUP;
+    __shared__ float sums[4][16 * MB][16 * NT + 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16 * NT;
+    const int m0 = blockIdx.y * 16 * MB;
+    const int steps = (k + STEP - 1) / STEP, first = steps * wave / 4, last = steps * (wave + 1) / 4;
+
+    // Where this lane's weights, scales and rows of x begin (rows past the end repeat the last one and are not stored).
+    const uint8_t *w[NT];
+    const float2 *sc[NT];
+    const T *xr[MB];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                dot += v[j] * (float)((c >> (4 * j)) & 15);
-                sum += v[j];
+    for (int t = 0; t < NT; t++) {
+        const int64_t row = min(n0 + 16 * t + col, n - 1);
+        w[t] = codes + row * (k / 2);
+        sc[t] = scales + row * (k / GROUP);
+    }
+#pragma unroll
+    for (int b = 0; b < MB; b++) xr[b] = x + min(m0 + 16 * b + col, m - 1) * x_stride;
+
+    auto load = [&](int step, Step<T, GROUP, NT, MB> &s) {
+        const int k0 = step * STEP + 32 * q;
+        const bool in = k0 < k;  // (k and the groups are multiples of 32)
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            s.codes[t] = in ? *(const u4 *)(w[t] + k0 / 2) : u4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < G; i++) {
+                const int at = step * STEP + i * GROUP;
+                s.scales[t][i] = at < k ? sc[t][at / GROUP] : make_float2(0.f, 0.f);
             }
-            acc += s.x * dot + s.y * sum;
         }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) acc += st::xor_lane(acc, o, lane);
-        if (bias) acc += bias[col];
-        if (relu && acc < 0.f) acc = 0.f;
-        if (lane == 0) out[row * out_stride + col] = (T)acc;
+        for (int b = 0; b < MB; b++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                // Product j's 8 elements of this lane: the j-th 8 of its 32 codes, or after the exchange the q-th of the j-th 32.
+                const int at = step * STEP + (GROUP == STEP ? 32 * q + 8 * j : 32 * j + 8 * q);
+#pragma unroll
+                for (int h = 0; h < (int)sizeof(T) / 2; h++) s.x[b][j][h] = u4{0, 0, 0, 0};
+                if (at < k) {
+                    if (vec) {
+#pragma unroll
+                        for (int h = 0; h < (int)sizeof(T) / 2; h++) s.x[b][j][h] = *(const u4 *)((const char *)(xr[b] + at) + 16 * h);
+                    } else {
+                        T e[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) e[i] = xr[b][at + i];
+                        __builtin_memcpy(s.x[b][j], e, sizeof e);
+                    }
+                }
+            }
+    };
+
+    uint32_t mask, bias16, ones;
+    if constexpr (std::is_same_v<T, _Float16>) {  // 16 + c: exponent of 16, c in the upper four bits of the mantissa
+        asm("s_mov_b32 %0, 0x03C003C0" : "=s"(mask));
+        asm("v_mov_b32 %0, 0x4C004C00" : "=v"(bias16));
+        ones = 0x3C003C00;
+    } else {
+        asm("s_mov_b32 %0, 0x00780078" : "=s"(mask));
+        asm("v_mov_b32 %0, 0x41804180" : "=v"(bias16));
+        ones = 0x3F803F80;
+    }
+    auto numbers = [&](uint32_t c) {
+        if constexpr (std::is_same_v<T, _Float16>)
+            return u4{((c << 6) & mask) | bias16, ((c << 2) & mask) | bias16, ((c >> 2) & mask) | bias16, ((c >> 6) & mask) | bias16};
+        else
+            return u4{((c << 3) & mask) | bias16, ((c >> 1) & mask) | bias16, ((c >> 5) & mask) | bias16, ((c >> 9) & mask) | bias16};
+    };
+
+    f4 acc[NT][MB];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int b = 0; b < MB; b++) acc[t][b] = f4{0.f, 0.f, 0.f, 0.f};
+
+    auto compute = [&](const Step<T, GROUP, NT, MB> &s) {
+        u4 c[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            c[t] = s.codes[t];
+            if constexpr (GROUP < STEP) {
+                const auto a = __builtin_amdgcn_permlane32_swap(c[t][0], c[t][2], false, false);
+                const auto d = __builtin_amdgcn_permlane32_swap(c[t][1], c[t][3], false, false);
+                const auto e = __builtin_amdgcn_permlane16_swap(a[0], d[0], false, false);
+                const auto f = __builtin_amdgcn_permlane16_swap(a[1], d[1], false, false);
+                c[t] = u4{(uint32_t)e[0], (uint32_t)e[1], (uint32_t)f[0], (uint32_t)f[1]};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            f4 dot[NT][MB], sum[MB];
+#pragma unroll
+            for (int b = 0; b < MB; b++) {
+                sum[b] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < NT; t++) dot[t][b] = f4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int j = i * (4 / G); j < (i + 1) * (4 / G); j++) {
+                u4 xs[MB][PARTS];
+#pragma unroll
+                for (int b = 0; b < MB; b++) {
+                    if constexpr (PARTS == 1) {
+                        xs[b][0] = in_code_order(s.x[b][j][0]);
+                    } else {
+                        constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+                        uint32_t r[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) r[e] = s.x[b][j][order[e] >> 2][order[e] & 3];
+#pragma unroll
+                        for (int p = 0; p < 3; p++) {
+                            xs[b][p] = u4{upper_halves(r[0], r[1]), upper_halves(r[2], r[3]), upper_halves(r[4], r[5]), upper_halves(r[6], r[7])};
+                            if (p < 2) {
+#pragma unroll
+                                for (int e = 0; e < 8; e++)
+                                    r[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, r[e]) - __builtin_bit_cast(float, r[e] & 0xFFFF0000u));
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                    for (int b = 0; b < MB; b++) sum[b] = product<T>(xs[b][p], u4{ones, ones, ones, ones}, sum[b]);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const u4 y = numbers(c[t][j]);
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                        for (int b = 0; b < MB; b++) dot[t][b] = product<T>(xs[b][p], y, dot[t][b]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const float scale = s.scales[t][i].x, lo = __builtin_fmaf(-16.f, scale, s.scales[t][i].y);
+#pragma unroll
+                for (int b = 0; b < MB; b++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[t][b][r] = __builtin_fmaf(scale, dot[t][b][r], __builtin_fmaf(lo, sum[b][r], acc[t][b][r]));
+            }
+        }
+    };
+
+    // The next step's loads are under way while one is worked on (the last one again behind the end).
+    if (first < last) {
+        Step<T, GROUP, NT, MB> s0, s1;
+        load(first, s0);
+        for (int i = first; i < last; i += 2) {
+            load(min(i + 1, last - 1), s1);
+            compute(s0);
+            load(min(i + 2, last - 1), s0);
+            if (i + 1 < last) compute(s1);
+        }
+    }
+
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int b = 0; b < MB; b++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) sums[wave][16 * b + 4 * q + r][16 * t + col] = acc[t][b][r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * MB * 16 * NT; i += 256) {
+        const int b = i / (16 * NT), j = i % (16 * NT);
+        if (m0 + b >= m) break;
+        if (n0 + j >= n) continue;
+        float y = (sums[0][b][j] + sums[1][b][j]) + (sums[2][b][j] + sums[3][b][j]);
+        if (bias) y += bias[n0 + j];
+        if (relu && y < 0.f) y = 0.f;
+        out[(m0 + b) * out_stride + n0 + j] = (T)y;
     }
 }
 
@@ -108,8 +304,8 @@ extern "C" st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int
     if (group != 32 && group != 64 && group != 128)
         return st::fail(ST_ERR_INVALID, "matvec_4bit: group %lld is none of 32, 64, 128", (long long)group);
     if (k % group) return st::fail(ST_ERR_INVALID, "matvec_4bit: k %lld is not a multiple of the group %lld", (long long)k, (long long)group);
-    if (k > 1 << 20 || m > 1 << 20 || n > (int64_t)1 << 31)
-        return st::fail(ST_ERR_INVALID, "matvec_4bit: m %lld, k %lld (up to 2^20 each), n %lld (up to 2^31)", (long long)m, (long long)k, (long long)n);
+    if (k > 1 << 20 || m > 1 << 20 || n > INT32_MAX)
+        return st::fail(ST_ERR_INVALID, "matvec_4bit: m %lld, k %lld (up to 2^20 each), n %lld (below 2^31)", (long long)m, (long long)k, (long long)n);
     if (x_stride < k || out_stride < n)
         return st::fail(ST_ERR_INVALID, "matvec_4bit: rows of %lld and %lld elements lie %lld and %lld apart", (long long)k, (long long)n, (long long)x_stride, (long long)out_stride);
     if (dtype < ST_F32 || dtype > ST_BF16) return st::fail(ST_ERR_INVALID, "matvec_4bit: dtype %d is none of ST_F32, ST_F16, ST_BF16", (int)dtype);
@@ -123,9 +319,26 @@ extern "C" st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int
     const bool vec = st::rows_aligned(x, x_stride, size);
     return st::with_dtype(dtype, [&](auto *t) -> st_status {
         using T = std::remove_pointer_t<decltype(t)>;
-        k_matvec4<T><<<dim3((uint32_t)((n + 3) / 4), (uint32_t)std::min<int64_t>(m, 65535)), 256, 0, st::stream_of(stream)>>>(
-            (const T *)x, m, k, x_stride, vec, (const uint32_t *)codes, (const float2 *)scales, group, n, bias, relu != 0,
-            (T *)out, out_stride);
+        auto go = [&](auto kernel, int nt, int mb) {
+            const dim3 grid((uint32_t)((n + 16 * nt - 1) / (16 * nt)), (uint32_t)((m + 16 * mb - 1) / (16 * mb)));
+            kernel<<<grid, 256, 0, st::stream_of(stream)>>>((const T *)x, (int32_t)m, (int32_t)k, x_stride, vec, codes, (const float2 *)scales, n,
+                                                            bias, relu != 0, (T *)out, out_stride);
+        };
+        auto pick = [&](auto group_) {
+            constexpr int GROUP = decltype(group_)::value;
+            if (m > 16)
+                go(k_matvec4<T, GROUP, 2, 2>, 2, 2);
+            else if (n >= 8192)
+                go(k_matvec4<T, GROUP, 2, 1>, 2, 1);
+            else
+                go(k_matvec4<T, GROUP, 1, 1>, 1, 1);
+        };
+        if (group == 32)
+            pick(std::integral_constant<int, 32>());
+        else if (group == 64)
+            pick(std::integral_constant<int, 64>());
+        else
+            pick(std::integral_constant<int, 128>());
         ST_LAUNCH_CHECK();
         return ST_OK;
     });
