@@ -390,9 +390,9 @@ st_status st_quantize_4bit(const void *x, int32_t dtype, int64_t n, int64_t k, i
 /* out[i, j] = sum over l of x[i, l] w[j, l] + bias[j] (f32, NULL: none), then
  * ReLU where relu != 0, for m rows x [m, k] and weights w [n, k] as
  * st_quantize_4bit writes them (codes 16-byte aligned): the Linear layer
- * x @ w^T of a decoding step.  m, k <= 2^20, n < 2^31; every 32 rows read the weights
- * once, so large batches belong in st_matmul over dequantised weights.  out may
- * not overlap x. */
+ * x @ w^T of a decoding step.  m <= 2^19, k <= 2^20, n <= 2^28; every 32 rows
+ * (f32: 16) read the weights once, so large batches belong in st_matmul over
+ * dequantised weights.  out may not overlap x. */
 st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int64_t k, int64_t x_stride,
                          const uint8_t *codes, const float *scales, int64_t group, int64_t n,
                          const float *bias, int32_t relu, void *out, int64_t out_stride,

@@ -41,8 +41,9 @@ __global__ __launch_bounds__(256) void k_quantise4(const T *__restrict__ x, int6
 //
 // Lane (i, q) of a wave reads 16 bytes (32 codes) of weight row i: 64 bytes of each of 16 rows a load.  For groups of 32
 // and 64 a product over 32 k has to stay inside a group: the four lanes of a row exchange words (a 4 x 4 transposition by
-// v_permlane swaps), so that lane q has the q-th 8 codes of each 32.  The lane of a row holds its scales; nothing goes
-// through LDS but the four waves' sums at the end.
+// v_permlane swaps), so that lane q has the q-th 8 codes of each 32.  Lines of 128 bytes are read whole while they are there
+// (16 waves' rows are four times the L1 cache): two steps' codes at once, and a row's scales 16 groups at once, into LDS,
+// which the lanes of the row then read.
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -54,10 +55,9 @@ template <class T>
 constexpr int parts_of() { return sizeof(T) == 4 ? 3 : 1; }
 
 // One step's loads of a wave.
-template <class T, int GROUP, int NT, int MB>
+template <class T, int NT, int MB>
 struct Step {
     u4 codes[NT];
-    float2 scales[NT][STEP / GROUP];
     u4 x[MB][4][sizeof(T) / 2];  // 8 elements for each of the four products
 };
 
@@ -69,6 +69,29 @@ __device__ __forceinline__ f4 product(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
+// Codes as 16 + c in f16 or bf16: the exponent of 16, c in the upper four bits of the mantissa.
+template <class T>
+struct Numbers {
+    uint32_t mask, exponent, ones;
+    __device__ __forceinline__ Numbers() {
+        if constexpr (std::is_same_v<T, _Float16>) {
+            asm("s_mov_b32 %0, 0x03C003C0" : "=s"(mask));
+            asm("v_mov_b32 %0, 0x4C004C00" : "=v"(exponent));
+            ones = 0x3C003C00;
+        } else {
+            asm("s_mov_b32 %0, 0x00780078" : "=s"(mask));
+            asm("v_mov_b32 %0, 0x41804180" : "=v"(exponent));
+            ones = 0x3F803F80;
+        }
+    }
+    __device__ __forceinline__ u4 operator()(uint32_t c) const {
+        if constexpr (std::is_same_v<T, _Float16>)
+            return u4{((c << 6) & mask) | exponent, ((c << 2) & mask) | exponent, ((c >> 2) & mask) | exponent, ((c >> 6) & mask) | exponent};
+        else
+            return u4{((c << 3) & mask) | exponent, ((c >> 1) & mask) | exponent, ((c >> 5) & mask) | exponent, ((c >> 9) & mask) | exponent};
+    }
+};
+
 // Elements 0 1 .. 7 to the order 0 4 1 5 2 6 3 7 that a word's codes come out in.
 __device__ __forceinline__ u4 in_code_order(u4 x) {
     return u4{__builtin_amdgcn_perm(x[2], x[0], 0x05040100), __builtin_amdgcn_perm(x[2], x[0], 0x07060302),
@@ -78,17 +101,40 @@ __device__ __forceinline__ u4 in_code_order(u4 x) {
 // The upper halves (bf16 parts) of two f32 words, the first below.
 __device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
 
+// 8 elements as the products take them: in the codes' order, f32 in three parts.
+template <class T>
+__device__ __forceinline__ void parts8(const u4 (&x)[sizeof(T) / 2], u4 (&part)[parts_of<T>()]) {
+    if constexpr (sizeof(T) == 2) {
+        part[0] = in_code_order(x[0]);
+    } else {
+        constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+        uint32_t r[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) r[e] = x[order[e] >> 2][order[e] & 3];
+#pragma unroll
+        for (int p = 0; p < 3; p++) {
+            part[p] = u4{upper_halves(r[0], r[1]), upper_halves(r[2], r[3]), upper_halves(r[4], r[5]), upper_halves(r[6], r[7])};
+            if (p < 2) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    r[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, r[e]) - __builtin_bit_cast(float, r[e] & 0xFFFF0000u));
+            }
+        }
+    }
+}
+
 template <class T, int GROUP, int NT, int MB>
-__global__ __launch_bounds__(256, 2) void k_matvec4(const T *__restrict__ x, int32_t m, int32_t k, int64_t x_stride, bool vec,
-                                                    const uint8_t *__restrict__ codes, const float2 *__restrict__ scales,
-                                                    int64_t n, const float *__restrict__ bias, bool relu, T *__restrict__ out,
+__global__ __launch_bounds__(256, 2) void k_matvec4(const T *__restrict__ x, int32_t m, int32_t k, int64_t x_stride,
+                                                    const uint8_t *__restrict__ codes, const float2 *__restrict__ scales, int64_t n,
+                                                    const float *__restrict__ bias, bool relu, T *__restrict__ out,
                                                     int64_t out_stride) {
-    constexpr int PARTS = parts_of<T>(), G = STEP / GROUP;
+    constexpr int PARTS = parts_of<T>(), G = STEP / GROUP, PER_BLOCK = 16 / G;  // groups of a step, steps of 16 groups
     __shared__ float sums[4][16 * MB][16 * NT + 4];
+    __shared__ float2 block[4][NT][16][17];  // a wave's rows: 16 groups of each
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * 16 * NT;
     const int m0 = blockIdx.y * 16 * MB;
-    const int steps = (k + STEP - 1) / STEP, first = steps * wave / 4, last = steps * (wave + 1) / 4;
+    const int steps = k / STEP, first = steps * wave / 4, last = steps * (wave + 1) / 4;
 
     // Where this lane's weights, scales and rows of x begin (rows past the end repeat the last one and are not stored).
     const uint8_t *w[NT];
@@ -103,17 +149,14 @@ __global__ __launch_bounds__(256, 2) void k_matvec4(const T *__restrict__ x, int
 #pragma unroll
     for (int b = 0; b < MB; b++) xr[b] = x + min(m0 + 16 * b + col, m - 1) * x_stride;
 
-    auto load = [&](int step, Step<T, GROUP, NT, MB> &s) {
+    // (Rows of x need the alignment of their elements only: a load of 16 bytes may begin at any of them.)
+    typedef uint32_t X4 __attribute__((ext_vector_type(4), aligned(2)));
+    auto load = [&](auto tail_, int step, Step<T, NT, MB> &s) {
+        constexpr bool tail = decltype(tail_)::value;  // the step may reach past k (which is a multiple of 32)
         const int k0 = step * STEP + 32 * q;
-        const bool in = k0 < k;  // (k and the groups are multiples of 32)
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            s.codes[t] = in ? *(const u4 *)(w[t] + k0 / 2) : u4{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < G; i++) {
-                const int at = step * STEP + i * GROUP;
-                s.scales[t][i] = at < k ? sc[t][at / GROUP] : make_float2(0.f, 0.f);
-            }
+            s.codes[t] = tail && k0 >= k ? u4{0, 0, 0, 0} : *(const u4 *)(w[t] + k0 / 2);
         }
 #pragma unroll
         for (int b = 0; b < MB; b++)
@@ -122,37 +165,12 @@ __global__ __launch_bounds__(256, 2) void k_matvec4(const T *__restrict__ x, int
                 // Product j's 8 elements of this lane: the j-th 8 of its 32 codes, or after the exchange the q-th of the j-th 32.
                 const int at = step * STEP + (GROUP == STEP ? 32 * q + 8 * j : 32 * j + 8 * q);
 #pragma unroll
-                for (int h = 0; h < (int)sizeof(T) / 2; h++) s.x[b][j][h] = u4{0, 0, 0, 0};
-                if (at < k) {
-                    if (vec) {
-#pragma unroll
-                        for (int h = 0; h < (int)sizeof(T) / 2; h++) s.x[b][j][h] = *(const u4 *)((const char *)(xr[b] + at) + 16 * h);
-                    } else {
-                        T e[8];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) e[i] = xr[b][at + i];
-                        __builtin_memcpy(s.x[b][j], e, sizeof e);
-                    }
-                }
+                for (int h = 0; h < (int)sizeof(T) / 2; h++)
+                    s.x[b][j][h] = tail && at >= k ? u4{0, 0, 0, 0} : u4(*(const X4 *)((const char *)(xr[b] + at) + 16 * h));
             }
     };
 
-    uint32_t mask, bias16, ones;
-    if constexpr (std::is_same_v<T, _Float16>) {  // 16 + c: exponent of 16, c in the upper four bits of the mantissa
-        asm("s_mov_b32 %0, 0x03C003C0" : "=s"(mask));
-        asm("v_mov_b32 %0, 0x4C004C00" : "=v"(bias16));
-        ones = 0x3C003C00;
-    } else {
-        asm("s_mov_b32 %0, 0x00780078" : "=s"(mask));
-        asm("v_mov_b32 %0, 0x41804180" : "=v"(bias16));
-        ones = 0x3F803F80;
-    }
-    auto numbers = [&](uint32_t c) {
-        if constexpr (std::is_same_v<T, _Float16>)
-            return u4{((c << 6) & mask) | bias16, ((c << 2) & mask) | bias16, ((c >> 2) & mask) | bias16, ((c >> 6) & mask) | bias16};
-        else
-            return u4{((c << 3) & mask) | bias16, ((c >> 1) & mask) | bias16, ((c >> 5) & mask) | bias16, ((c >> 9) & mask) | bias16};
-    };
+    const Numbers<T> numbers;
 
     f4 acc[NT][MB];
 #pragma unroll
@@ -160,7 +178,8 @@ __global__ __launch_bounds__(256, 2) void k_matvec4(const T *__restrict__ x, int
 #pragma unroll
         for (int b = 0; b < MB; b++) acc[t][b] = f4{0.f, 0.f, 0.f, 0.f};
 
-    auto compute = [&](const Step<T, GROUP, NT, MB> &s) {
+    // `group`: of the block in LDS, the step's first.
+    auto compute = [&](const Step<T, NT, MB> &s, int group) {
         u4 c[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -187,28 +206,12 @@ __global__ __launch_bounds__(256, 2) void k_matvec4(const T *__restrict__ x, int
                 u4 xs[MB][PARTS];
 #pragma unroll
                 for (int b = 0; b < MB; b++) {
-                    if constexpr (PARTS == 1) {
-                        xs[b][0] = in_code_order(s.x[b][j][0]);
-                    } else {
-                        constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-                        uint32_t r[8];
-#pragma unroll
-                        for (int e = 0; e < 8; e++) r[e] = s.x[b][j][order[e] >> 2][order[e] & 3];
-#pragma unroll
-                        for (int p = 0; p < 3; p++) {
-                            xs[b][p] = u4{upper_halves(r[0], r[1]), upper_halves(r[2], r[3]), upper_halves(r[4], r[5]), upper_halves(r[6], r[7])};
-                            if (p < 2) {
-#pragma unroll
-                                for (int e = 0; e < 8; e++)
-                                    r[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, r[e]) - __builtin_bit_cast(float, r[e] & 0xFFFF0000u));
-                            }
-                        }
-                    }
+                    parts8<T>(s.x[b][j], xs[b]);
                 }
 #pragma unroll
                 for (int p = 0; p < PARTS; p++)
 #pragma unroll
-                    for (int b = 0; b < MB; b++) sum[b] = product<T>(xs[b][p], u4{ones, ones, ones, ones}, sum[b]);
+                    for (int b = 0; b < MB; b++) sum[b] = product<T>(xs[b][p], u4{numbers.ones, numbers.ones, numbers.ones, numbers.ones}, sum[b]);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     const u4 y = numbers(c[t][j]);
@@ -220,7 +223,8 @@ __global__ __launch_bounds__(256, 2) void k_matvec4(const T *__restrict__ x, int
             }
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                const float scale = s.scales[t][i].x, lo = __builtin_fmaf(-16.f, scale, s.scales[t][i].y);
+                const float2 pair = block[wave][t][col][group + i];
+                const float scale = pair.x, lo = __builtin_fmaf(-16.f, scale, pair.y);
 #pragma unroll
                 for (int b = 0; b < MB; b++)
 #pragma unroll
@@ -229,16 +233,50 @@ __global__ __launch_bounds__(256, 2) void k_matvec4(const T *__restrict__ x, int
         }
     };
 
-    // The next step's loads are under way while one is worked on (the last one again behind the end).
+    // 16 groups from `from` on (those past the row's end repeat its last): lane (i, q) has the q-th 4 of row i.
+    float2 coming[NT][4];
+    const int groups = k / GROUP;
+    auto load_block = [&](int from) {
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) coming[t][i] = sc[t][min(from + 4 * q + i, groups - 1)];
+    };
+    auto put_block = [&] {  // (a wave's LDS operations are carried out in order: no barrier)
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) block[wave][t][col][4 * q + i] = coming[t][i];
+    };
+    // The next two steps' loads are under way while two are worked on (the last one's again behind the end: a condition around
+    // them would make every wait one for all of them).
     if (first < last) {
-        Step<T, GROUP, NT, MB> s0, s1;
-        load(first, s0);
-        for (int i = first; i < last; i += 2) {
-            load(min(i + 1, last - 1), s1);
-            compute(s0);
-            load(min(i + 2, last - 1), s0);
-            if (i + 1 < last) compute(s1);
+        Step<T, NT, MB> s[2][2];
+        load_block(first * G);
+        load(std::false_type(), first, s[0][0]);
+        load(std::false_type(), min(first + 1, last - 1), s[0][1]);
+        for (int i = first; i < last; i += 4) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int at = i + 2 * j, group = (at - first) % PER_BLOCK * G;
+                if (at >= last) break;
+                if (group == 0) {
+                    put_block();
+                    load_block((at + PER_BLOCK) * G);
+                }
+                load(std::false_type(), min(at + 2, last - 1), s[1 - j][0]);
+                load(std::false_type(), min(at + 3, last - 1), s[1 - j][1]);
+                compute(s[j][0], group);
+                if (at + 1 < last) compute(s[j][1], group + G);
+            }
         }
+    }
+    if (wave == 3 && k % STEP) {  // (the groups of a part of a step are those of k's last)
+        Step<T, NT, MB> s;
+        load_block(k / STEP * G);
+        load(std::true_type(), k / STEP, s);
+        put_block();
+        compute(s, 0);
     }
 
 #pragma unroll
@@ -304,8 +342,8 @@ extern "C" st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int
     if (group != 32 && group != 64 && group != 128)
         return st::fail(ST_ERR_INVALID, "matvec_4bit: group %lld is none of 32, 64, 128", (long long)group);
     if (k % group) return st::fail(ST_ERR_INVALID, "matvec_4bit: k %lld is not a multiple of the group %lld", (long long)k, (long long)group);
-    if (k > 1 << 20 || m > 1 << 20 || n > INT32_MAX)
-        return st::fail(ST_ERR_INVALID, "matvec_4bit: m %lld, k %lld (up to 2^20 each), n %lld (below 2^31)", (long long)m, (long long)k, (long long)n);
+    if (m > 1 << 19 || k > 1 << 20 || n > 1 << 28)  // (a launch holds less than 2^32 threads along x, 2^16 workgroups along y)
+        return st::fail(ST_ERR_INVALID, "matvec_4bit: m %lld (up to 2^19), k %lld (up to 2^20), n %lld (up to 2^28)", (long long)m, (long long)k, (long long)n);
     if (x_stride < k || out_stride < n)
         return st::fail(ST_ERR_INVALID, "matvec_4bit: rows of %lld and %lld elements lie %lld and %lld apart", (long long)k, (long long)n, (long long)x_stride, (long long)out_stride);
     if (dtype < ST_F32 || dtype > ST_BF16) return st::fail(ST_ERR_INVALID, "matvec_4bit: dtype %d is none of ST_F32, ST_F16, ST_BF16", (int)dtype);
@@ -316,20 +354,24 @@ extern "C" st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int
     if (((uintptr_t)codes & 15) || ((uintptr_t)scales & 7) || ((uintptr_t)bias & 3))
         return st::fail(ST_ERR_INVALID, "matvec_4bit: codes are 16-byte, scales 8-byte, bias 4-byte aligned");
     if (!st::device_ok()) return ST_ERR_NO_DEVICE;
-    const bool vec = st::rows_aligned(x, x_stride, size);
     return st::with_dtype(dtype, [&](auto *t) -> st_status {
         using T = std::remove_pointer_t<decltype(t)>;
         auto go = [&](auto kernel, int nt, int mb) {
             const dim3 grid((uint32_t)((n + 16 * nt - 1) / (16 * nt)), (uint32_t)((m + 16 * mb - 1) / (16 * mb)));
-            kernel<<<grid, 256, 0, st::stream_of(stream)>>>((const T *)x, (int32_t)m, (int32_t)k, x_stride, vec, codes, (const float2 *)scales, n,
+            kernel<<<grid, 256, 0, st::stream_of(stream)>>>((const T *)x, (int32_t)m, (int32_t)k, x_stride, codes, (const float2 *)scales, n,
                                                             bias, relu != 0, (T *)out, out_stride);
         };
         auto pick = [&](auto group_) {
             constexpr int GROUP = decltype(group_)::value;
-            if (m > 16)
-                go(k_matvec4<T, GROUP, 2, 2>, 2, 2);
-            else if (n >= 8192)
-                go(k_matvec4<T, GROUP, 2, 1>, 2, 1);
+            // Rows of weights a workgroup (16 NT): with more of them x is read and summed less often, with fewer there are workgroups
+            // for every CU.  us at NT 1, 2, 4: 32768 x 8192 in groups of 128, one row of bf16: 48.8, 42.3, 38.8; 11003 x 4096 in groups
+            // of 32, 16 rows of f16: 23.9, 22.2, 20.2; 1024 x 256, one row of f32: 4.05 and 10.9 at NT 1 and 4.  f32's three parts
+            // leave registers for half as many tiles, and 16 rows of x at a time.
+            constexpr int WIDE = sizeof(T) == 2 ? 4 : 2;
+            if constexpr (sizeof(T) == 2)
+                if (m > 16) return go(k_matvec4<T, GROUP, 2, 2>, 2, 2);
+            if (n >= 8192)
+                go(k_matvec4<T, GROUP, WIDE, 1>, WIDE, 1);
             else
                 go(k_matvec4<T, GROUP, 1, 1>, 1, 1);
         };

@@ -37,7 +37,8 @@ def test_matvec_refusals():
                     (dict(out_stride=7), "apart"), (dict(dtype=7), "dtype"), (dict(x=None), "NULL"), (dict(codes=None), "NULL"),
                     (dict(scales=None), "NULL"), (dict(out=None), "NULL"), (dict(codes=FAKE + 8), "aligned"),
                     (dict(scales=FAKE + 4), "aligned"), (dict(bias=FAKE + 2), "aligned"), (dict(out=FAKE + 1), "aligned"),
-                    (dict(k=1 << 21, x_stride=1 << 21), "2^20"), (dict(m=1 << 21), "2^20")]:
+                    (dict(k=1 << 21, x_stride=1 << 21), "2^20"), (dict(m=(1 << 19) + 1), "2^19"),
+                    (dict(m=1 << 21), "2^20"), (dict(n=(1 << 28) + 1, out_stride=1 << 30), "2^28")]:
         refused("st_matvec_4bit", swap(ok, **kw), msg)
     for kw in (dict(m=0), dict(n=0)):
         assert _lib.lib().st_matvec_4bit(*swap(ok, x=None, out=None, codes=None, scales=None, **kw)) == _lib.ST_OK
