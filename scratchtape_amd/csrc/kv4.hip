@@ -14,7 +14,7 @@ using st::page_of;
 
 struct AppendArgs {
     int64_t n, q_stride, k_stride, v_stride;
-    int32_t hq, hd, half, interleaved;
+    int32_t hq, hd, half, interleaved, stretch;
     bool vec_q, vec_k, vec_v, vec_out;
     const int32_t *seq, *pos;
     const float *inv_freq;
@@ -23,66 +23,86 @@ struct AppendArgs {
     Cache cache;
 };
 
-// 8 components from e of a vector, the first 2 half of them rotated by the position's angles in 64 bits.
-template <class T>
-__device__ __forceinline__ void rotate8(const T *x, int e, bool vec, int half, bool interleaved, int32_t pos,
-                                        const float *inv_freq, float (&y)[8]) {
-    st::load8(x + e, vec, y);
-    if (e >= 2 * half) return;
-#pragma unroll 1
-    for (int i = 0; i < 8; i++) {
-        const int d = e + i;
-        if (d >= 2 * half) break;
-        const int j = interleaved ? d >> 1 : d < half ? d : d - half;
-        const bool second = interleaved ? d & 1 : d >= half;
-        const int other = interleaved ? d ^ 1 : second ? d - half : d + half;
-        double s, c;
-        sincos((double)pos * (double)inv_freq[j], &s, &c);
-        const double a = (double)(float)x[d], b = (double)(float)x[other];
-        y[i] = (float)(second ? a * c + b * s : a * c - b * s);
+// A lane's part of the rotation: component e + i becomes x[i] c[i] + other[i] s[i], `other` the second of its pair.
+struct Turn {
+    double c[8], s[8];
+    __device__ __forceinline__ Turn(const double2 *turn, int e, int half, bool interleaved) {  // turn: (cos, sin) of the pairs' angles
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int d = e + i;
+            const bool second = interleaved ? d & 1 : d >= half;
+            const double2 t = turn[d >= 2 * half ? 0 : interleaved ? d >> 1 : second ? d - half : d];
+            c[i] = t.x, s[i] = second ? t.y : -t.y;
+        }
     }
-}
+    // The components e .. e + 7 of the vector `from`, x; the first 2 half are rotated.
+    template <class T>
+    __device__ __forceinline__ void operator()(const T *from, int e, bool vec, int half, bool interleaved, float (&x)[8]) const {
+        if (e >= 2 * half) return;
+        float other[8];
+        if (interleaved) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) other[i] = x[i ^ 1];
+        } else if (half % 8 == 0) {  // the eight others lie side by side
+            st::load8(from + (e >= half ? e - half : e + half), vec, other);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) other[i] = e + i >= 2 * half ? 0.f : (float)from[e + i >= half ? e + i - half : e + i + half];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (e + i < 2 * half) x[i] = (float)((double)x[i] * c[i] + (double)other[i] * s[i]);
+    }
+};
 
-// Vectors of a token: hq of q, then hkv of k, then hkv of v; LANES lanes each, 8 components a lane.
+// A token's vectors (hq of q, then hkv of k, then hkv of v), `stretch` of them a workgroup, LANES lanes each, 8 components a
+// lane.  The cosines and sines are taken once a workgroup, in 64 bits; sequence, position and page are the same for all its lanes.
 template <class T, int LANES>
 __global__ __launch_bounds__(256) void k_append4(const T *__restrict__ q, const T *__restrict__ k,
                                                  const T *__restrict__ v, T *__restrict__ q_out, T *__restrict__ k_out,
                                                  T *__restrict__ v_out, AppendArgs a) {
-    const int per = a.hq + 2 * a.cache.hkv, hkv = a.cache.hkv;
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
-    const int64_t token = i / per;
-    const int head = (int)(i - token * per), e = (threadIdx.x % LANES) * 8;
-    bool used = token < a.n && e < a.hd;
-    int64_t s = 0, pos = 0;
-    if (used) {
-        s = a.seq[token], pos = a.pos[token];
-        used = s >= 0 && s < a.cache.nseq && pos >= 0;
-    }
-    const int64_t page = used ? page_of(a.cache, s, pos) : -1;
-    used = page >= 0;
-    float x[8] = {};
-    const bool is_q = head < a.hq, is_k = !is_q && head < a.hq + hkv;
-    if (used) {
-        if (is_q) {
-            rotate8(q + token * a.q_stride + (int64_t)head * a.hd, e, a.vec_q, a.half, a.interleaved, (int32_t)pos, a.inv_freq, x);
-            st::store8(q_out + (token * a.hq + head) * a.hd + e, a.vec_out, x);
-        } else if (is_k) {
-            rotate8(k + token * a.k_stride + (int64_t)(head - a.hq) * a.hd, e, a.vec_k, a.half, a.interleaved, (int32_t)pos, a.inv_freq, x);
-        } else {
-            st::load8(v + token * a.v_stride + (int64_t)(head - a.hq - hkv) * a.hd + e, a.vec_v, x);
+    __shared__ double2 turn[128];
+    const int hq = a.hq, hkv = a.cache.hkv, e = (threadIdx.x % LANES) * 8;
+    const int64_t token = (int64_t)blockIdx.z * gridDim.x + blockIdx.x;
+    if (token >= a.n) return;
+    const int64_t s = a.seq[token], pos = a.pos[token];
+    if (s < 0 || s >= a.cache.nseq || pos < 0) return;
+    const int64_t page = page_of(a.cache, s, pos);
+    if (page < 0) return;
+    const int begin = blockIdx.y * a.stretch, end = min(begin + a.stretch, hq + 2 * hkv);
+    if (a.half && begin < hq + hkv) {
+        if ((int)threadIdx.x < a.half) {
+            double si, co;
+            sincos((double)pos * (double)a.inv_freq[threadIdx.x], &si, &co);
+            turn[threadIdx.x] = make_double2(co, si);
         }
+        __syncthreads();
     }
-    float scale, lo;
-    const uint32_t codes = st::quantise8<LANES>(x, used, scale, lo);
-    if (!used || is_q) return;
-    const int h = head - a.hq - (is_k ? 0 : hkv);
-    const int64_t row = (page * hkv + h) * a.cache.page + (pos & (a.cache.page - 1));
-    *(uint32_t *)((is_k ? a.k_codes : a.v_codes) + row * (a.hd / 2) + e / 2) = codes;
-    if (e == 0) (is_k ? a.k_scales : a.v_scales)[row] = make_float2(scale, lo);
-    T *out = is_k ? k_out : v_out;
-    if (out) {
-        st::values8(codes, scale, lo, x);
-        st::store8(out + (token * hkv + h) * a.hd + e, a.vec_out, x);
+    const Turn rotate(turn, e, a.half, a.interleaved);
+    for (int first = begin; first < end; first += 256 / LANES) {
+        const int head = first + threadIdx.x / LANES;
+        const bool used = head < end && e < a.hd, is_q = head < hq, is_k = !is_q && head < hq + hkv;
+        const int h = is_q ? head : is_k ? head - hq : head - hq - hkv;
+        float x[8] = {};
+        if (used) {
+            const T *from = (is_q ? q + token * a.q_stride : is_k ? k + token * a.k_stride : v + token * a.v_stride) + (int64_t)h * a.hd;
+            const bool vec = is_q ? a.vec_q : is_k ? a.vec_k : a.vec_v;
+            st::load8(from + e, vec, x);
+            if (is_q || is_k) rotate(from, e, vec, a.half, a.interleaved, x);
+            if (is_q) st::store8(q_out + (token * hq + h) * a.hd + e, a.vec_out, x);
+        }
+        if (first + 256 / LANES <= hq) continue;  // queries only
+        float scale, lo;
+        const uint32_t codes = st::quantise8<LANES>(x, used, scale, lo);
+        if (!used || is_q) continue;
+        const int64_t row = (page * hkv + h) * a.cache.page + (pos & (a.cache.page - 1));
+        *(uint32_t *)((is_k ? a.k_codes : a.v_codes) + row * (a.hd / 2) + e / 2) = codes;
+        if (e == 0) (is_k ? a.k_scales : a.v_scales)[row] = make_float2(scale, lo);
+        T *out = is_k ? k_out : v_out;
+        if (out) {
+            st::values8(codes, scale, lo, x);
+            st::store8(out + (token * hkv + h) * a.hd + e, a.vec_out, x);
+        }
     }
 }
 
@@ -119,13 +139,17 @@ extern "C" st_status st_kv_append_4bit(const void *q, const void *k, const void 
     a.seq = seq, a.pos = pos, a.inv_freq = inv_freq;
     a.k_codes = k_codes, a.v_codes = v_codes, a.k_scales = (float2 *)k_scales, a.v_scales = (float2 *)v_scales;
     const int64_t lanes = hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32;
-    const int64_t blocks = (n * (queries + 2 * hkv) * lanes + 255) / 256;
-    if (blocks > INT32_MAX) return st::fail(ST_ERR_INVALID, "%s: %lld tokens of %lld heads are too many for one call", name, (long long)n, (long long)(queries + 2 * hkv));
+    // With tokens enough to fill the chip a workgroup takes a whole token (8191 tokens of 48 vectors of 128: 68 us, 98 with a pass
+    // of 16 vectors each, which take the sines three times); with few, one pass (64 tokens: 5.1 us, 6.2).
+    const int64_t vectors = queries + 2 * hkv, once = 256 / lanes;
+    a.stretch = (int32_t)(n >= 1024 ? vectors : once);
+    const int64_t along = std::min<int64_t>(n, 1 << 23);  // (a launch holds less than 2^32 threads along x)
+    const dim3 grid((uint32_t)along, (uint32_t)((vectors + a.stretch - 1) / a.stretch), (uint32_t)((n + along - 1) / along));
     return st::with_dtype(dtype, [&](auto *t) -> st_status {
         using T = std::remove_pointer_t<decltype(t)>;
         auto go = [&](auto kernel) {
-            kernel<<<(uint32_t)blocks, 256, 0, st::stream_of(stream)>>>((const T *)q, (const T *)k, (const T *)v, (T *)q_out, (T *)k_out,
-                                                                        (T *)v_out, a);
+            kernel<<<grid, 256, 0, st::stream_of(stream)>>>((const T *)q, (const T *)k, (const T *)v, (T *)q_out, (T *)k_out,
+                                                            (T *)v_out, a);
         };
         if (lanes == 4)
             go(k_append4<T, 4>);

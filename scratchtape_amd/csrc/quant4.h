@@ -69,37 +69,58 @@ __device__ __forceinline__ void store8(T *p, bool vec, const float (&x)[8]) {
 // The 4-bit form of a group spread over LANES neighbouring lanes (a power of two up to 64, the group starting at a
 // multiple of it), 8 values x a lane; lanes with used = false hold none of it.  Returns the lane's 8 codes, and scale
 // and lo, the same in every lane.  All lanes of the wave take part.
+//
+// Quotients by d = hi - lo are products with its reciprocal in 64 bits and one correction, q + (a - q d) / d, which is
+// a / d rounded (the reciprocal is).  For the codes f32 does as long as it leaves no doubt: (x - lo) (15 / d) in f32 is off by
+// no more than 4 roundings (d, 15 / d, the difference, the product) of a number up to 15, 4 x 15 x 2^-24 = 3.6e-6, so a
+// quotient more than 1e-5 from the middle of two codes has the code that 64 bits give it.  Where a wave has one that is nearer
+// (or d is so small or so large that these products would leave f32's normal numbers), it computes its codes again in 64.
 template <int LANES>
 __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], bool used, float &scale, float &lo) {
 #pragma clang fp contract(off)
     const int lane = lane_id();
     float mn = INFINITY, mx = -INFINITY;
-    bool finite = true;
     if (used) {
+        float zero = 0.f;  // NaN once a value is not finite
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             mn = fminf(mn, x[i]);
             mx = fmaxf(mx, x[i]);
-            finite = finite && __builtin_isfinite(x[i]);
+            zero = __builtin_fmaf(x[i], 0.f, zero);
         }
+        if (zero != 0.f) mn = -INFINITY;  // which then shows in the group's minimum
     }
-    mn = finite ? mn : -INFINITY;  // a value that is not finite shows in the group's minimum
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1) {
         mn = fminf(mn, xor_lane(mn, o, lane));
         mx = fmaxf(mx, xor_lane(mx, o, lane));
     }
-    const double d = (double)mx - (double)mn;
-    if (mn == -INFINITY) {
-        scale = lo = NAN;
-        return 0;
-    }
-    scale = (float)(d / 15.0);
-    lo = mn;
-    if (!(d > 0.0)) return 0;
+    const bool finite = mn != -INFINITY && used;
+    lo = finite ? mn : NAN;
+    const double d = finite ? (double)mx - (double)mn : 0.0;
+    const double third = d * (1.0 / 15.0);
+    const float fifteenth = (float)__builtin_fma(__builtin_fma(-15.0, third, d), 1.0 / 15.0, third);
+    scale = finite ? fifteenth : NAN;
+    const float f = 15.f / (float)d;  // (d 0: infinite, and not used)
+    const bool plain = d > 0x1p-100 && d < 0x1p100;
     uint32_t codes = 0;
+    float nearest = 0.5f;  // the least distance from the middle of two codes
 #pragma unroll
-    for (int i = 0; i < 8; i++) codes |= (uint32_t)(int)rint((((double)x[i] - (double)mn) * 15.0) / d) << (4 * i);
+    for (int i = 0; i < 8; i++) {
+        const float r = (x[i] - mn) * f, c = __builtin_rintf(r);
+        nearest = fminf(nearest, 0.5f - __builtin_fabsf(r - c));
+        codes |= (uint32_t)(int)c << (4 * i);
+    }
+    if (d == 0.0) codes = 0;
+    if (d > 0.0 && (!plain || !(nearest > 1e-5f))) {
+        const double reciprocal = 1.0 / d;
+        codes = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const double a = ((double)x[i] - (double)mn) * 15.0, q = a * reciprocal;
+            codes |= (uint32_t)(int)rint(__builtin_fma(__builtin_fma(-q, d, a), reciprocal, q)) << (4 * i);
+        }
+    }
     return codes;
 }
 

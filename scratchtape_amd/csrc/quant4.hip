@@ -8,23 +8,31 @@
 
 namespace {
 
-// One thread per 8 values; a group is 4, 8 or 16 neighbouring lanes.
+// One thread per 8 values; a group is 4, 8 or 16 neighbouring lanes.  `width`: 8-value units of a row (of all rows, where they
+// lie behind each other).
 template <class T, int GROUP>
-__global__ __launch_bounds__(256) void k_quantise4(const T *__restrict__ x, int64_t n, int64_t k, int64_t stride,
+__global__ __launch_bounds__(256) void k_quantise4(const T *__restrict__ x, int64_t total, int64_t width, int64_t stride,
                                                    bool vec, uint32_t *__restrict__ codes, float2 *__restrict__ scales,
                                                    T *__restrict__ values, bool vec_values) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = n * (k / 8);
+    const int64_t first = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256, i = first + threadIdx.x;
     const bool used = i < total;
     float v[8] = {};
     if (used) {
-        const int64_t row = i / (k / 8);
-        st::load8(x + row * stride + (i - row * (k / 8)) * 8, vec, v);
+        // The workgroup's first row is the same for all lanes (a scalar division); a lane's is a few rows on.
+        int64_t row = first / width, at = first - row * width + threadIdx.x;
+        if (width >= 256) {
+            if (at >= width) at -= width, row++;
+        } else {
+            const uint32_t more = (uint32_t)at / (uint32_t)width;
+            row += more, at -= more * width;
+        }
+        st::load8(x + row * stride + at * 8, vec, v);
     }
     float scale, lo;
     const uint32_t c = st::quantise8<GROUP / 8>(v, used, scale, lo);
     if (!used) return;
     codes[i] = c;
-    if (i % (GROUP / 8) == 0) scales[i / (GROUP / 8)] = make_float2(scale, lo);
+    if (threadIdx.x % (GROUP / 8) == 0) scales[i / (GROUP / 8)] = make_float2(scale, lo);
     if (values) {
         st::values8(c, scale, lo, v);
         st::store8(values + i * 8, vec_values, v);
@@ -316,12 +324,14 @@ extern "C" st_status st_quantize_4bit(const void *x, int32_t dtype, int64_t n, i
     if (((uintptr_t)codes & 3) || ((uintptr_t)scales & 7)) return st::fail(ST_ERR_INVALID, "quantize_4bit: codes are 4-byte, scales 8-byte aligned");
     if (!st::device_ok()) return ST_ERR_NO_DEVICE;
     const bool vec = st::rows_aligned(x, x_stride, size), vec_values = ((uintptr_t)values & 15) == 0;
-    const int64_t blocks = (n * (k / 8) + 255) / 256;
+    const int64_t total = n * (k / 8), blocks = (total + 255) / 256, along = std::min<int64_t>(blocks, 1 << 23);  // (below 2^32 threads)
+    const dim3 grid((uint32_t)along, (uint32_t)((blocks + along - 1) / along));
+    const int64_t width = x_stride == k ? total : k / 8;
     return st::with_dtype(dtype, [&](auto *t) -> st_status {
         using T = std::remove_pointer_t<decltype(t)>;
         auto go = [&](auto kernel) {
-            kernel<<<(uint32_t)blocks, 256, 0, st::stream_of(stream)>>>((const T *)x, n, k, x_stride, vec, (uint32_t *)codes,
-                                                                        (float2 *)scales, (T *)values, vec_values);
+            kernel<<<grid, 256, 0, st::stream_of(stream)>>>((const T *)x, total, width, x_stride, vec, (uint32_t *)codes,
+                                                            (float2 *)scales, (T *)values, vec_values);
         };
         if (group == 32)
             go(k_quantise4<T, 32>);
