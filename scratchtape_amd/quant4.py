@@ -29,21 +29,26 @@ def _dtype(t: torch.Tensor, what: str) -> int:
 
 def _rows(t: torch.Tensor, what: str) -> int:
     """Elements from a row to the next of a [rows, ...] tensor whose rows are contiguous."""
-    width, run = t[0].numel() if t.shape[0] else 0, 1
-    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+    shape, strides = t.shape, t.stride()
+    width = 1
+    for size in shape[1:]:
+        width *= size
+    if not shape[0] or t.is_contiguous():
+        return width
+    run = 1
+    for size, stride in zip(reversed(shape[1:]), reversed(strides[1:])):
         if size != 1 and width and stride != run:
-            raise ValueError(f"{what} has rows that are not contiguous (shape {list(t.shape)}, strides {list(t.stride())})")
+            raise ValueError(f"{what} has rows that are not contiguous (shape {list(shape)}, strides {list(strides)})")
         run *= size
-    stride = t.stride(0) if t.shape[0] > 1 else run
-    if stride < run:
-        raise ValueError(f"{what} has rows that overlap (shape {list(t.shape)}, strides {list(t.stride())})")
-    return stride
+    if shape[0] > 1 and strides[0] < run:
+        raise ValueError(f"{what} has rows that overlap (shape {list(shape)}, strides {list(strides)})")
+    return strides[0] if shape[0] > 1 else run
 
 
 def _plain(t: torch.Tensor, dtype: torch.dtype, shape, what: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} is a torch tensor")
-    if t.dtype != dtype or not t.is_contiguous() or tuple(t.shape) != tuple(shape):
+    if t.dtype != dtype or not t.is_contiguous() or t.shape != shape:
         raise ValueError(f"{what} is a contiguous {dtype} tensor {list(shape)}; got {t.dtype} {list(t.shape)}"
                          + ("" if t.is_contiguous() else " that is not contiguous"))
     return t
@@ -51,40 +56,62 @@ def _plain(t: torch.Tensor, dtype: torch.dtype, shape, what: str) -> torch.Tenso
 
 def _extent(t: torch.Tensor) -> Tuple[int, int]:
     """The first byte of a tensor and the one behind its last."""
+    start = t.data_ptr()
+    if t.is_contiguous():
+        return start, start + t.nbytes
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    return start, start + (last + 1) * t.element_size()
 
 
 def _apart(outs, ins) -> None:
     """No output shares memory with an input or with another output; (tensor or None, name) pairs."""
-    outs = [(*_extent(t), name) for t, name in outs if t is not None and t.numel()]
-    ins = [(*_extent(t), name) for t, name in ins if t is not None and t.numel()]
-    for i, (a, b, name) in enumerate(outs):
-        for c, d, other in ins + outs[:i]:
-            if a < d and c < b:
-                raise ValueError(f"{name} shares memory with {other}")
+    spans = [(*_extent(t), True, name) for t, name in outs if t is not None]
+    spans += [(*_extent(t), False, name) for t, name in ins if t is not None]
+    spans = [s for s in spans if s[0] < s[1]]
+    spans.sort()
+    # By their starts: an output may not start before the end of anything earlier, an input not before an output's.
+    end = out_end = 0
+    for a, b, out, name in spans:
+        if a < (end if out else out_end):
+            other = next(o for c, d, other_out, o in spans if c <= a < d and o != name and (out or other_out))
+            raise ValueError(f"{name} shares memory with {other}" if out else f"{other} shares memory with {name}")
+        end = max(end, b)
+        if out:
+            out_end = max(out_end, b)
 
 
 def _on_gpu(first: torch.Tensor, tensors) -> None:
     """Every given tensor on the GPU of the first."""
     if not first.is_cuda:
         raise ValueError("tensors live on the GPU")
+    index = first.get_device()
     for t, name in tensors:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"{name} is on {t.device}, the rest on {first.device}")
 
 
-@contextlib.contextmanager
-def _launch(device: torch.device, stream):
+class _launch:
     """Makes `device` current and, inside, gives the handle of the stream to launch on (the device's current one if
     `stream` is None); what is allocated inside belongs to that stream."""
-    with torch.cuda.device(device):
-        handle = _stream(stream)
-        if stream is None or handle == _stream(None):
-            yield handle
-        else:
-            with torch.cuda.stream(torch.cuda.ExternalStream(handle, device=device)):
-                yield handle
+    __slots__ = ("device", "stream", "inside")
+
+    def __init__(self, device: torch.device, stream):
+        self.device, self.stream, self.inside = device, stream, None
+
+    def __enter__(self) -> int:
+        if self.stream is None and torch.cuda.current_device() == self.device.index:
+            return _stream(None)
+        with contextlib.ExitStack() as stack:
+            stack.enter_context(torch.cuda.device(self.device))
+            handle = _stream(self.stream)
+            if self.stream is not None and handle != _stream(None):
+                stack.enter_context(torch.cuda.stream(torch.cuda.ExternalStream(handle, device=self.device)))
+            self.inside = stack.pop_all()
+        return handle
+
+    def __exit__(self, *error) -> None:
+        if self.inside is not None:
+            self.inside.__exit__(*error)
 
 
 def _addr(t: Optional[torch.Tensor]) -> int:
