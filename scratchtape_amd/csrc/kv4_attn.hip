@@ -56,6 +56,7 @@ constexpr int WHOLE = 512;        // units of up to so many keys are not shared 
 constexpr int MAX_GROUPS = 1024;  // workgroups of a launch
 constexpr float BASE = 7.f, MOST_X = 32768.f;  // p aV is set to 2^7 at most, and may grow to 2^15
 constexpr float MIN_E = -86.f, MOST_P = 101.f;  // values below 2^-86 of scale count as that for the reference: p <= 2^93, 2^101
+constexpr float MOST_SUM = 0x1p101f;
 
 // What k_merge4 joins: a unit's rows, the first of them head `head` of token `token`; the first part is in the odd slot of the
 // workgroup that this stands under, the others in the even slots of those behind it.
@@ -525,6 +526,14 @@ struct Ring {
     }
 };
 
+// A wave-uniform value in scalar registers of its own.  Kernel arguments arrive eight or sixteen words at a time, and where
+// scalar registers are short the compiler puts away and brings back all of those for one that a loop needs.
+template <class T>
+__device__ __forceinline__ T alone(T x) {
+    asm("" : "+s"(x));
+    return x;
+}
+
 template <int HD, int PARTS, int RT>
 __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attention4(const AttnArgs a) {
     using R = Ring<HD>;
@@ -573,7 +582,9 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
     const bool no_pages = busy && c.pages == 0 && end > begin;
 
     // Pages of the next 32 tiles' halves, a half a lane: -1 one outside the cache, 0 (not looked at) behind the end.
-    const int page_rows = c.hkv * c.page, head_row = u.head * c.page;
+    const int page_rows = alone(c.hkv * c.page), head_row = alone(u.head * c.page), page_mask = alone(c.page - 1), window = alone(a.window);
+    const uint8_t *const k_codes = alone(c.k_codes), *const v_codes = alone(c.v_codes);
+    const float2 *const k_scales = alone(c.k_scales), *const v_scales = alone(c.v_scales);
     int entries = 0, entries_to = 0;
     uint32_t bad = 0;  // of the tiles in the ring, two bits each
     auto bring_tile = [&](int it, int slot) {
@@ -589,8 +600,8 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
         const int key = first_key + it * step, i = 2 * (it + 32 - entries_to);
         const int p0 = st::lane_value(entries, i), p1 = st::lane_value(entries, i + 1);
         bad = (bad & ~(3u << (2 * slot))) | ((p0 < 0 ? 1u : 0u) | (p1 < 0 ? 2u : 0u)) << (2 * slot);
-        const int64_t row_0 = (int64_t)max(p0, 0) * page_rows + (head_row + (key & (c.page - 1)));
-        const int64_t row_1 = (int64_t)max(p1, 0) * page_rows + (head_row + ((key + 16) & (c.page - 1)));
+        const int64_t row_0 = (int64_t)max(p0, 0) * page_rows + (head_row + (key & page_mask));
+        const int64_t row_1 = (int64_t)max(p1, 0) * page_rows + (head_row + ((key + 16) & page_mask));
         const uint32_t to = ring_at + slot * R::BYTES;
         const int64_t b0 = row_0 * (HD / 2), b1 = row_1 * (HD / 2);
 #pragma unroll
@@ -598,17 +609,17 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
             if (R::EVEN && i < HD / 32) {  // one half of K or V
                 const bool v = i >= HD / 64;
                 const int j = v ? i - HD / 64 : i, half = 64 * j / R::HALF;
-                bring((v ? c.v_codes : c.k_codes) + (half ? b1 : b0), R::source(64 * j % R::HALF + lane, v), to + 1024 * i);
+                bring((v ? v_codes : k_codes) + (half ? b1 : b0), R::source(64 * j % R::HALF + lane, v), to + 1024 * i);
             } else {
                 int n = 64 * i + lane;
                 const char *from;
                 if (n < 2 * HD) {
                     const bool v = n >= HD;
                     n -= v ? HD : 0;
-                    from = (const char *)(v ? c.v_codes : c.k_codes) + (n >= R::HALF ? b1 : b0) + R::source(n % R::HALF, v);
+                    from = (const char *)(v ? v_codes : k_codes) + (n >= R::HALF ? b1 : b0) + R::source(n % R::HALF, v);
                 } else {
                     n = (n - 2 * HD) & 31;  // lanes without a chunk of their own repeat one into the tile's padding
-                    from = (const char *)(n >= 16 ? c.v_scales : c.k_scales) + (n & 8 ? row_1 : row_0) * 8 + 16 * (n & 7);
+                    from = (const char *)(n >= 16 ? v_scales : k_scales) + (n & 8 ? row_1 : row_0) * 8 + 16 * (n & 7);
                 }
                 bring(from, to + 1024 * i);
             }
@@ -675,7 +686,7 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
     }
     auto process = [&](char *tile, int it, int bad_halves) {
         const int kt = first_key + it * step, key0 = kt + 4 * g;
-        const bool masked = kt + 31 > pos_first || kt + 31 >= end || (a.window > 0 && kt <= pos_last - a.window);
+        const bool masked = kt + 31 > pos_first || kt + 31 >= end || (window > 0 && kt <= pos_last - window);
         bool careful = false;
         if (masked || bad_halves) {
             // What lies behind the end counts nothing, whatever it holds; keys on a page outside the cache are NaN to the rows that
@@ -721,7 +732,7 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
             if (masked) {
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
-                    const int after = a.window > 0 ? pos[rt] - a.window : -1;
+                    const int after = window > 0 ? pos[rt] - window : -1;
 #pragma unroll
                     for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -734,26 +745,48 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
         };
         // p = 2^(z - R) and p aV of every row.  For the first tile, and where p aV would pass f16's range or p an f32's, the scores
         // are taken again to set R: seldom, and the common tile holds no registers for it.
-        float p[RT][2][4], x[RT][2][4];
-        float most_z = -INFINITY, most_x = INFINITY;
-        if (it > 0) {
-            scores(tile, ref, p);
-            most_x = 0.f;
+        // (The tile's p are no larger than their sum.)
+        float p[RT][2][4], sum[RT];
+        h8 ph[RT], pr[PARTS == 2 ? RT : 1];
+        auto weights = [&](const char *tile) {  // p aV in f16, rounded once
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const float4 y = R::pairs(tile, true, i, r / 2, g);
+                    const float v = r & 1 ? y.z : y.x;
 #pragma unroll
                     for (int rt = 0; rt < RT; rt++) {
-                        most_z = fmaxf(most_z, p[rt][i][r]);
-                        p[rt][i][r] = __builtin_amdgcn_exp2f(p[rt][i][r]);
-                        x[rt][i][r] = p[rt][i][r] * (r & 1 ? y.z : y.x);
-                        most_x = fmaxf(most_x, x[rt][i][r]);
+                        ph[rt][4 * i + r] = (_Float16)__builtin_fmaf(p[rt][i][r], v, 0.f);
+                        if constexpr (PARTS == 2) pr[rt][4 * i + r] = (_Float16)__builtin_fmaf(p[rt][i][r], v, -(float)ph[rt][4 * i + r]);
                     }
                 }
+        };
+        bool past = true;
+        if (it > 0) {
+            scores(tile, ref, p);
+            float most_p = 0.f;
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                sum[rt] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        p[rt][i][r] = __builtin_amdgcn_exp2f(p[rt][i][r]);
+                        sum[rt] += p[rt][i][r];
+                    }
+                most_p = fmaxf(most_p, sum[rt]);
+            }
+            weights(tile);
+            h2 most_x = {};
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) most_x = __builtin_elementwise_max(most_x, h2{ph[rt][2 * i], ph[rt][2 * i + 1]});
+            past = most_p > MOST_SUM || (float)most_x[0] > MOST_X || (float)most_x[1] > MOST_X;
         }
-        if (__any(most_z > MOST_P || most_x > MOST_X)) {
+        if (__any(past)) {
             uint32_t from = uniform((uint32_t)(tile - mem));
             asm volatile("" : "+s"(from));  // read again, not kept
             const char *again = mem + from;
@@ -778,36 +811,46 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
 #pragma unroll
                 for (int j = 0; j < HD / 16; j++) o[rt][j] *= keep;
                 ref[rt] = m;
+                sum[rt] = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float4 y = R::pairs(again, true, i, r / 2, g);
                         // (A row without a reference sees nothing here: minus infinity less itself is no number.)
                         p[rt][i][r] = m == -INFINITY && p[rt][i][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[rt][i][r] - m);
-                        x[rt][i][r] = p[rt][i][r] * (r & 1 ? y.z : y.x);
+                        sum[rt] += p[rt][i][r];
                     }
             }
+            weights(again);
         }
-        h8 ph[RT], pr[PARTS == 2 ? RT : 1];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int rt = 0; rt < RT; rt++) total[rt] += sum[rt];
+        if (careful) {  // (a weight of 0 leaves even what is not a number out)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float4 y = R::pairs(tile, true, i, r / 2, g);
-                const float v8 = __builtin_fmaf(8.f, r & 1 ? y.z : y.x, r & 1 ? y.w : y.y);  // what a code of 8 stands for
+            for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    float &xx = x[rt][i][r];
-                    total[rt] += p[rt][i][r];
-                    if (careful && p[rt][i][r] == 0.f)
-                        xx = 0.f;
-                    else
-                        low[rt] = __builtin_fmaf(p[rt][i][r], v8, low[rt]);
-                    ph[rt][4 * i + r] = (_Float16)xx;
-                    if constexpr (PARTS == 2) pr[rt][4 * i + r] = (_Float16)(xx - (float)ph[rt][4 * i + r]);
+                for (int r = 0; r < 4; r++) {
+                    const float4 y = R::pairs(tile, true, i, r / 2, g);
+                    const float v8 = __builtin_fmaf(8.f, r & 1 ? y.z : y.x, r & 1 ? y.w : y.y);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        const bool none = p[rt][i][r] == 0.f;
+                        low[rt] = none ? low[rt] : __builtin_fmaf(p[rt][i][r], v8, low[rt]);
+                        ph[rt][4 * i + r] = none ? (_Float16)0.f : ph[rt][4 * i + r];
+                        if constexpr (PARTS == 2) pr[rt][4 * i + r] = none ? (_Float16)0.f : pr[rt][4 * i + r];
+                    }
                 }
-            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float4 y = R::pairs(tile, true, i, r / 2, g);
+                    const float v8 = __builtin_fmaf(8.f, r & 1 ? y.z : y.x, r & 1 ? y.w : y.y);  // what a code of 8 stands for
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) low[rt] = __builtin_fmaf(p[rt][i][r], v8, low[rt]);
+                }
+        }
         weigh_values<HD, PARTS, RT>(take, [&](int b, int i) {  // keys 4 g .. of each half, whose rows lie in the order 0 4 8 12 1 ..
             return *(const uint32_t *)(tile + 16 * (HD + R::HALF * (i >> 2)) + (4 * (i & 3) + g) * (HD / 2) + word_at<HD>(b, col));
         }, ph, pr, col, o);
