@@ -952,7 +952,9 @@ __global__ __launch_bounds__(256, 2) void k_decode4(const AttnArgs a) {
     const bool no_pages = c.pages == 0 && end > span.lo + u.cut0;
 
     // Pages of the next 16 tiles' quarters, a quarter a lane: -1 one outside the cache, 0 (not looked at) behind the end.
-    const int page_rows = c.hkv * c.page, head_row = u.head * c.page;
+    const int page_rows = alone(c.hkv * c.page), head_row = alone(u.head * c.page), page_mask = alone(c.page - 1), window = alone(a.window);
+    const uint8_t *const k_codes = alone(c.k_codes), *const v_codes = alone(c.v_codes);
+    const float2 *const k_scales = alone(c.k_scales), *const v_scales = alone(c.v_scales);
     int entries = 0, entries_to = 0;
     uint32_t bad = 0;  // of the tiles in the ring, four bits each
     auto bring_tile = [&](int it, int slot) {
@@ -970,14 +972,14 @@ __global__ __launch_bounds__(256, 2) void k_decode4(const AttnArgs a) {
         int64_t row[4];
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            row[i] = (int64_t)max(st::lane_value(entries, i0 + i), 0) * page_rows + (head_row + ((key + 16 * i) & (c.page - 1)));
+            row[i] = (int64_t)max(st::lane_value(entries, i0 + i), 0) * page_rows + (head_row + ((key + 16 * i) & page_mask));
         const uint32_t to = ring_at + slot * R::BYTES;
-        const bool one_page = c.page >= 64;
+        const bool one_page = page_mask >= 63;
 #pragma unroll
         for (int i = 0; i < R::LOADS - 1; i++) {
             const bool v = i >= HD / 32;
             const int n = 64 * (v ? i - HD / 32 : i);
-            const uint8_t *codes = v ? c.v_codes : c.k_codes;
+            const uint8_t *codes = v ? v_codes : k_codes;
             if constexpr (R::EVEN) {  // 16 keys of one quarter
                 bring(codes + row[n / 64] * (HD / 2), (R::key_of(n + lane, v) & 15) * (HD / 2) + R::byte_of(n + lane, v), to + 1024 * i);
             } else if (one_page) {
@@ -990,7 +992,7 @@ __global__ __launch_bounds__(256, 2) void k_decode4(const AttnArgs a) {
         }
         const int q = (lane & 31) >> 3;
         const int64_t at = (q & 2 ? q & 1 ? row[3] : row[2] : q & 1 ? row[1] : row[0]) + 2 * (lane & 7);
-        bring((lane < 32 ? c.k_scales : c.v_scales) + at, to + 1024 * (R::LOADS - 1));
+        bring((lane < 32 ? k_scales : v_scales) + at, to + 1024 * (R::LOADS - 1));
     };
     // Rows: 16 lanes share one's components, find its largest, and leave it in LDS scaled to f16 for all lanes to read.
     // Lane (block, row) of the 4 x 4 x 4 products holds row lane % 4 of each 4.
@@ -1068,7 +1070,7 @@ __global__ __launch_bounds__(256, 2) void k_decode4(const AttnArgs a) {
 
     auto process = [&](char *tile, int it, int bad_quarters) {
         const int kt = first_key + it * 256, key = kt + lane;
-        const bool masked = kt + 63 > pos_first || kt + 63 >= end || (a.window > 0 && kt <= pos_last - a.window);
+        const bool masked = kt + 63 > pos_first || kt + 63 >= end || (window > 0 && kt <= pos_last - window);
         float2 kp = *(const float2 *)(tile + R::PAIRS + 8 * lane), vp = *(const float2 *)(tile + R::PAIRS + 512 + 8 * lane);
         bool careful = false;
         if (masked || bad_quarters) {
@@ -1107,7 +1109,7 @@ __global__ __launch_bounds__(256, 2) void k_decode4(const AttnArgs a) {
             for (int r = 0; r < ROWS; r++) z[r] = __builtin_fmaf(kp.x, s[r >> 2][r & 3] * unscale[r], kp.y * qsum[r]);
             if (masked) {
 #pragma unroll
-                for (int r = 0; r < ROWS; r++) z[r] = key <= pos[r] && key > (a.window > 0 ? pos[r] - a.window : -1) ? z[r] : -INFINITY;
+                for (int r = 0; r < ROWS; r++) z[r] = key <= pos[r] && key > (window > 0 ? pos[r] - window : -1) ? z[r] : -INFINITY;
             }
         };
         // p = 2^(z - R) and p aV.  For the first tile, and where p aV would pass f16's range or p an f32's, the scores set R.
