@@ -402,8 +402,9 @@ st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int64_t k, int
  * [pages, hkv, page, 2] for the keys and for the values, 16-byte aligned; a
  * token's head vector is one group of the 4-bit format.  hd is 32, 64, 96, 128,
  * 192 or 256; page a power of two from 16 to 1024 tokens; hq a multiple of hkv.
- * Token p of sequence s is in page table[s, p / page] (table [nseq, max_pages]),
- * slot p % page; entries that no call needs are not read.
+ * Token p of sequence s is in page table[s, p / page] (table [nseq, max_pages],
+ * nseq <= 2^20, max_pages * page <= 2^30), slot p % page; entries that no call
+ * needs are not read.
  *
  * Appends n tokens: token t belongs at position pos[t] of sequence seq[t].  Its
  * queries q [n, hq, hd] (NULL: none) and keys k [n, hkv, hd] have their first

@@ -51,8 +51,8 @@ inline bool cache_ok(const char *name, Cache &c, int64_t nseq, const int32_t *ta
         fail(ST_ERR_INVALID, "%s: pages of %lld tokens are no power of two from 16 to 1024", name, (long long)page);
         return false;
     }
-    if (max_pages > INT32_MAX / page) {
-        fail(ST_ERR_INVALID, "%s: %lld pages of %lld tokens a sequence pass 2^31", name, (long long)max_pages, (long long)page);
+    if (max_pages > (1 << 30) / page) {  // (a tile's keys past the last one stay within 32 bits)
+        fail(ST_ERR_INVALID, "%s: %lld pages of %lld tokens a sequence pass 2^30", name, (long long)max_pages, (long long)page);
         return false;
     }
     if (page * hkv * 256 > INT32_MAX) {

@@ -53,7 +53,7 @@ ATTEND = dict(q=FAKE, dtype=0, n=4, hq=8, hkv=2, hd=64, q_stride=512, q_start=FA
 SHARED = [(dict(hq=7), "multiple"), (dict(hkv=0), "key heads"), (dict(hd=80), "head width"), (dict(hd=48), "head width"),
           (dict(hd=512), "head width"), (dict(page=8), "power of two"), (dict(page=48), "power of two"), (dict(page=2048), "power of two"),
           (dict(n=-1), "-1"), (dict(dtype=3), "dtype"), (dict(nseq=-1), "sequences"), (dict(pages=-1), "sequences"),
-          (dict(max_pages=1 << 30), "2^31"), (dict(table=None), "NULL"), (dict(k_codes=None), "NULL"), (dict(v_scales=None), "NULL"),
+          (dict(max_pages=1 << 30), "2^30"), (dict(max_pages=(1 << 26) + 1, page=16), "2^30"), (dict(table=None), "NULL"), (dict(k_codes=None), "NULL"), (dict(v_scales=None), "NULL"),
           (dict(k_scales=FAKE + 8), "aligned"), (dict(v_codes=FAKE + 4), "aligned"), (dict(q_stride=511), "apart")]
 
 
