@@ -123,7 +123,8 @@ def check_append(cache, before, q, k, v, seq, pos, table, inv_freq, interleaved,
 @pytest.mark.parametrize("t", sorted(TYPES))
 @pytest.mark.parametrize("heads,hq,hd,page,rot,interleaved,tokens", [
     (4, 4, 64, 16, 64, False, 1), (8, 32, 128, 64, 128, False, 70), (3, 15, 96, 32, 96, True, 33), (1, 7, 32, 16, 30, False, 50),
-    (2, 2, 256, 128, 128, True, 129), (2, 10, 192, 16, 0, False, 40), (5, 5, 64, 1024, 2, True, 17)])
+    (2, 2, 256, 256, 128, True, 129), (2, 10, 192, 16, 0, False, 40), (5, 5, 64, 1024, 2, True, 17),
+    (3, 15, 96, 64, 96, False, 1100), (1, 4, 32, 256, 30, False, 1024)])
 def test_append_is_exact(dev, heads, hq, hd, page, rot, interleaved, tokens, t):
     """Tokens of several sequences at scattered places, some of them padding or nowhere, from views of a fused projection."""
     t = TYPES[t]
@@ -334,6 +335,14 @@ def test_long_sequences(dev, t, hq, new, length):
     lens = [length, 129]
     cache, table = filled(lens, 2, 64, 64, 9, dev)
     run(cache, table, lens, [new, 1], hq, TYPES[t], dev, spread=2.0)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("lens,news,heads,hq", [([3000, 9000], [1, 90], 1, 1), ([700] * 5 + [6000], [1] * 5 + [150], 2, 8)])
+def test_one_sequence_of_many_rows_among_single_tokens(dev, lens, news, heads, hq, t):
+    """Parts of units with far more rows than the sequences have on average."""
+    cache, table = filled(lens, heads, 64, 64, 14, dev)
+    run(cache, table, lens, news, hq, TYPES[t], dev, spread=2.0)
 
 
 def test_many_sequences(dev):

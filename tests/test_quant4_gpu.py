@@ -64,6 +64,24 @@ def test_quantiser_on_borders_ties_and_extremes(dev, t):
         check_quantised(y, group, *quant4.quantize_4bit(y, group, values=True))
 
 
+def test_quantiser_over_all_sizes_of_numbers(dev):
+    """Group widths from f32's subnormals to its largest values, each far from zero and near it: the quotients in f32 and those
+    in 64 bits hold the same codes."""
+    g = torch.Generator().manual_seed(21)
+    scale = torch.tensor([2.0 ** e for e in range(-146, 126)], dtype=torch.float64)[:, None]
+    x = torch.rand(272, 1024, generator=g, dtype=torch.float64) * scale
+    x = torch.cat((x, x + 3 * scale, x - 2 * scale)).float().to(dev)
+    for group in (32, 128):
+        check_quantised(x, group, *quant4.quantize_4bit(x, group, values=True))
+
+
+def test_quantiser_of_short_and_of_strided_rows(dev):
+    """Rows shorter than a workgroup's share, apart and together."""
+    for n, k, stride in ((1000, 32, 35), (77, 96, 96), (513, 64, 64), (3, 8192, 8200), (5, 2080, 2084)):
+        x = weights(n, stride, torch.float32, n).to(dev)[:, :k]
+        check_quantised(x, 32, *quant4.quantize_4bit(x, 32, values=True))
+
+
 @pytest.mark.parametrize("t", sorted(TYPES))
 def test_quantiser_takes_views_and_fills_tensors(dev, t):
     base = weights(9, 331, TYPES[t], 5).to(dev)
@@ -110,7 +128,8 @@ def check_product(x, codes, scales, bias, relu, got):
 @pytest.mark.parametrize("t", sorted(TYPES))
 @pytest.mark.parametrize("m,k,n,group", [(1, 32, 1, 32), (1, 256, 1024, 64), (1, 8192, 77, 128), (2, 96, 17, 32), (3, 192, 130, 64),
                                          (16, 4096, 515, 32), (17, 640, 255, 128), (33, 1088, 64, 64), (70, 128, 300, 128),
-                                         (1, 20480, 16, 32), (5, 32, 40000, 32)])
+                                         (1, 20480, 16, 32), (5, 32, 40000, 32), (16, 1056, 8200, 32), (20, 640, 8200, 64),
+                                         (2, 1408, 8255, 128)])
 def test_products_against_64_bits(dev, m, k, n, group, t):
     g = torch.Generator().manual_seed(m + k + n)
     codes, scales = quant4.quantize_4bit(torch.randn(n, k, generator=g).to(dev) * 0.05, group)
