@@ -45,7 +45,8 @@ __global__ __launch_bounds__(256) void k_quantise4(const T *__restrict__ x, int6
 // operand as it lies in memory (f16 and bf16), and a code is the f16 or bf16 number 16 + c, its four bits put under the
 // exponent of 16 by a shift and a v_and_or (a VALU operation per code), so that sum x c = sum x (16 + c) - 16 sum x loses two
 // bits of the f32 sum and not seven, as 1024 + c or 128 + c would.  sum x is one more product, with ones, which comes out
-// in the lanes that want it.  f32 rows are three bf16 parts of 8 bits each, taken off one after the other without rounding.
+// in the lanes that want it.  f32 rows are three bf16 parts of 8 bits each, taken off one after the other without rounding, and
+// codes beside them are taken less 8.
 //
 // Lane (i, q) of a wave reads 16 bytes (32 codes) of weight row i: 64 bytes of each of 16 rows a load.  For groups of 32
 // and 64 a product over 32 k has to stay inside a group: the four lanes of a row exchange words (a 4 x 4 transposition by
@@ -77,7 +78,12 @@ __device__ __forceinline__ f4 product(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
-// Codes as 16 + c in f16 or bf16: the exponent of 16, c in the upper four bits of the mantissa.
+// The upper halves (bf16 parts) of two f32 words, the first below.
+__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
+
+// 8 codes as the products' operand, in the order 0 4 1 5 2 6 3 7.  Beside f16 and bf16 rows: 16 + c, the exponent of 16 with c in
+// the upper four bits of the mantissa.  Beside f32's parts: (c - 8) / 16 in bf16 (twice the operations), as an f32 sum has no bits to
+// spare for an offset (groups of 128 of 4096: 2.2e-6 off with 16 + c).
 template <class T>
 struct Numbers {
     uint32_t mask, exponent, ones;
@@ -93,10 +99,25 @@ struct Numbers {
         }
     }
     __device__ __forceinline__ u4 operator()(uint32_t c) const {
-        if constexpr (std::is_same_v<T, _Float16>)
+        if constexpr (std::is_same_v<T, float>) {
+            const uint32_t low = c ^ 0x88888888u, high = low >> 16;  // c - 8 in two's complement
+            auto pair = [](uint32_t a, uint32_t b) {
+                return upper_halves(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_off_f32_i4((int)a)),
+                                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_off_f32_i4((int)b)));
+            };
+            return u4{pair(low, high), pair(low >> 4, high >> 4), pair(low >> 8, high >> 8), pair(low >> 12, high >> 12)};
+        } else if constexpr (std::is_same_v<T, _Float16>) {
             return u4{((c << 6) & mask) | exponent, ((c << 2) & mask) | exponent, ((c >> 2) & mask) | exponent, ((c >> 6) & mask) | exponent};
-        else
+        } else {
             return u4{((c << 3) & mask) | exponent, ((c >> 1) & mask) | exponent, ((c >> 5) & mask) | exponent, ((c >> 9) & mask) | exponent};
+        }
+    }
+    // A group's scale and lowest value for sums over these numbers.
+    static __device__ __forceinline__ float2 scaled(float2 pair) {
+        if constexpr (std::is_same_v<T, float>)
+            return make_float2(16.f * pair.x, __builtin_fmaf(8.f, pair.x, pair.y));
+        else
+            return make_float2(pair.x, __builtin_fmaf(-16.f, pair.x, pair.y));
     }
 };
 
@@ -105,9 +126,6 @@ __device__ __forceinline__ u4 in_code_order(u4 x) {
     return u4{__builtin_amdgcn_perm(x[2], x[0], 0x05040100), __builtin_amdgcn_perm(x[2], x[0], 0x07060302),
               __builtin_amdgcn_perm(x[3], x[1], 0x05040100), __builtin_amdgcn_perm(x[3], x[1], 0x07060302)};
 }
-
-// The upper halves (bf16 parts) of two f32 words, the first below.
-__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
 
 // 8 elements as the products take them: in the codes' order, f32 in three parts.
 template <class T>
@@ -231,8 +249,8 @@ __global__ __launch_bounds__(256, 2) void k_matvec4(const T *__restrict__ x, int
             }
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                const float2 pair = block[wave][t][col][group + i];
-                const float scale = pair.x, lo = __builtin_fmaf(-16.f, scale, pair.y);
+                const float2 pair = numbers.scaled(block[wave][t][col][group + i]);
+                const float scale = pair.x, lo = pair.y;
 #pragma unroll
                 for (int b = 0; b < MB; b++)
 #pragma unroll
