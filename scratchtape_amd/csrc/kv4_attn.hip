@@ -10,7 +10,7 @@
 // 2^-24, half the work, and the matrix cores take them; but they line up the sums by the exponent that subnormals share,
 // and lose the 6 to 10 bits that n leaves unused: 4e-5 off in f32.)
 // Rows are scaled by a power of two to f16 (f32 rows, PARTS = 2, as two f16 parts, 22 bits), scores and sums are f32; the
-// weights are rounded to f16, in two parts for f32 rows.  A row's reference M is no running maximum of its scores but follows
+// weights are rounded to f16, in two parts for f32 rows and for few rows of f16.  A row's reference M is no running maximum of its scores but follows
 // max(z log2 e + log2 aV), so that p aV stays inside f16's normal range whatever the sizes of the values; it is raised only
 // where p aV would pass 2^15, so the common tile has no reduction over lanes at all.
 //
@@ -419,8 +419,8 @@ struct Taker {
 
 // O^T += V^T P^T for 32 keys: `word(b, i)` is this lane's word of block b of the i-th of its 8 keys, ph (and pr, the weights'
 // second parts) its 8 weights of each 16 rows.
-template <int HD, int PARTS, int RT, class Word>
-__device__ __forceinline__ void weigh_values(const Taker &take, const Word &word, const h8 (&ph)[RT], const h8 (&pr)[PARTS == 2 ? RT : 1], int col,
+template <int HD, int WEIGHTS, int RT, class Word>
+__device__ __forceinline__ void weigh_values(const Taker &take, const Word &word, const h8 (&ph)[RT], const h8 (&pr)[WEIGHTS == 2 ? RT : 1], int col,
                                              f4 (&o)[RT][HD / 16]) {
 #pragma unroll
     for (int b = 0; b < blocks_of(HD); b++) {
@@ -442,7 +442,7 @@ __device__ __forceinline__ void weigh_values(const Taker &take, const Word &word
                 f4 &e = o[rt][b * first + 2 * i], &d = o[rt][b * first + 2 * i + 1];
                 e = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph[rt], e, 0, 0, 0);
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph[rt], d, 0, 0, 0);
-                if constexpr (PARTS == 2) {
+                if constexpr (WEIGHTS == 2) {
                     e = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pr[rt], e, 0, 0, 0);
                     d = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pr[rt], d, 0, 0, 0);
                 }
@@ -536,7 +536,7 @@ __device__ __forceinline__ T alone(T x) {
     return x;
 }
 
-template <int HD, int PARTS, int RT>
+template <int HD, int PARTS, int WEIGHTS, int RT>
 __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attention4(const AttnArgs a) {
     using R = Ring<HD>;
     constexpr int NW = HD / 32, WAVE_ROWS = 16 * RT, LDO = HD + 4, STAGES = RT == 1 ? 2 : 3;
@@ -749,7 +749,7 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
             // are taken again to set R: seldom, and the common tile holds no registers for it.
             // (The tile's p are no larger than their sum.)
             float p[RT][2][4], sum[RT];
-            h8 ph[RT], pr[PARTS == 2 ? RT : 1];
+            h8 ph[RT], pr[WEIGHTS == 2 ? RT : 1];
             auto weights = [&](const char *tile) {  // p aV in f16, rounded once
 #pragma unroll
                 for (int i = 0; i < 2; i++)
@@ -760,7 +760,7 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
 #pragma unroll
                         for (int rt = 0; rt < RT; rt++) {
                             ph[rt][4 * i + r] = (_Float16)__builtin_fmaf(p[rt][i][r], v, 0.f);
-                            if constexpr (PARTS == 2) pr[rt][4 * i + r] = (_Float16)__builtin_fmaf(p[rt][i][r], v, -(float)ph[rt][4 * i + r]);
+                            if constexpr (WEIGHTS == 2) pr[rt][4 * i + r] = (_Float16)__builtin_fmaf(p[rt][i][r], v, -(float)ph[rt][4 * i + r]);
                         }
                     }
             };
@@ -839,7 +839,7 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
                             const bool none = p[rt][i][r] == 0.f;
                             low[rt] = none ? low[rt] : __builtin_fmaf(p[rt][i][r], v8, low[rt]);
                             ph[rt][4 * i + r] = none ? (_Float16)0.f : ph[rt][4 * i + r];
-                            if constexpr (PARTS == 2) pr[rt][4 * i + r] = none ? (_Float16)0.f : pr[rt][4 * i + r];
+                            if constexpr (WEIGHTS == 2) pr[rt][4 * i + r] = none ? (_Float16)0.f : pr[rt][4 * i + r];
                         }
                     }
             } else {
@@ -853,7 +853,7 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
                         for (int rt = 0; rt < RT; rt++) low[rt] = __builtin_fmaf(p[rt][i][r], v8, low[rt]);
                     }
             }
-            weigh_values<HD, PARTS, RT>(take, [&](int b, int i) {  // keys 4 g .. of each half, whose rows lie in the order 0 4 8 12 1 ..
+            weigh_values<HD, WEIGHTS, RT>(take, [&](int b, int i) {  // keys 4 g .. of each half, whose rows lie in the order 0 4 8 12 1 ..
                 return *(const uint32_t *)(tile + 16 * (HD + R::HALF * (i >> 2)) + (4 * (i & 3) + g) * (HD / 2) + word_at<HD>(b, col));
             }, ph, pr, col, o);
         };
@@ -1048,16 +1048,13 @@ extern "C" st_status st_kv_attention_4bit(const void *q, int32_t dtype, int64_t 
         constexpr int HD = decltype(hd_)::value;
         const hipStream_t s = st::stream_of(stream);
         const uint32_t grid = cut.groups;
-        auto with = [&](auto kernel_f32, auto kernel) {
-            if (dtype == ST_F32)
-                kernel_f32<<<grid, 256, 0, s>>>(a);
-            else
-                kernel<<<grid, 256, 0, s>>>(a);
-        };
+        auto with = [&](auto f32, auto f16, auto bf16) { (dtype == ST_F32 ? f32 : dtype == ST_F16 ? f16 : bf16)<<<grid, 256, 0, s>>>(a); };
+        // f16 outputs show the rounding of the weights to f16 (1.4 times the error of their own rounding).  Two parts cost few rows
+        // little (64 sequences 88.1 and 88.7 us, one long one 46.6 and 48.1), a prompt 529 and 579: there one does.
         if (cut.rt == 1)
-            with(k_attention4<HD, 2, 1>, k_attention4<HD, 1, 1>);
+            with(k_attention4<HD, 2, 2, 1>, k_attention4<HD, 1, 2, 1>, k_attention4<HD, 1, 1, 1>);
         else if constexpr (HD <= 128)
-            with(k_attention4<HD, 2, 2>, k_attention4<HD, 1, 2>);
+            with(k_attention4<HD, 2, 2, 2>, k_attention4<HD, 1, 1, 2>, k_attention4<HD, 1, 1, 2>);
         ST_LAUNCH_CHECK();
         if (cut.part_rows == 0) return ST_OK;
         // Four waves a row where it has many parts (one long sequence: 45.7 us with four, 49.7 with one),
