@@ -12,6 +12,7 @@ Python mirrors of the reference interfaces they replace:
 - knn.KnnStore2bit (search_ivf, search_masked) / quantize_2bit / Centroids
                                                                 (gpu_step/knn.rs, knn/ivf.rs)
 - store.save / load: the 2-bit store in the reference's cache file format (gpu_step/knn/cache.rs)
+- quant4.quantize_4bit / matvec_4bit, kv4.KvCache4bit (append, attention): a decoding step in 4 bits (no counterpart)
 """
 from ._lib import ScratchtapeError, lib  # noqa: F401
 from .matmul import (Epilogue, MatRef, f16_enabled, f16_route, matmul, matmul_f32, matmul_grouped,  # noqa: F401
