@@ -57,6 +57,8 @@ struct Turn {
 
 // A token's vectors (hq of q, then hkv of k, then hkv of v), `stretch` of them a workgroup, LANES lanes each, 8 components a
 // lane.  The cosines and sines are taken once a workgroup, in 64 bits; sequence, position and page are the same for all its lanes.
+// 8191 tokens of 48 vectors of 128 in f16, 210 MB: 67 us (3.1 TB/s), of which the waves wait for loads two thirds (233 us with the angles
+// taken for each component and 64-bit quotients).
 template <class T, int LANES>
 __global__ __launch_bounds__(256) void k_append4(const T *__restrict__ q, const T *__restrict__ k,
                                                  const T *__restrict__ v, T *__restrict__ q_out, T *__restrict__ k_out,

@@ -9,7 +9,8 @@
 namespace {
 
 // One thread per 8 values; a group is 4, 8 or 16 neighbouring lanes.  `width`: 8-value units of a row (of all rows, where they
-// lie behind each other).
+// lie behind each other).  Bound by HBM: 16384 x 8192 bf16 with values, 612 MB, 122 us (5.0 TB/s, a large copy's rate; 154 us with a 64-bit
+// quotient for each value).
 template <class T, int GROUP>
 __global__ __launch_bounds__(256) void k_quantise4(const T *__restrict__ x, int64_t total, int64_t width, int64_t stride,
                                                    bool vec, uint32_t *__restrict__ codes, float2 *__restrict__ scales,
@@ -53,6 +54,9 @@ __global__ __launch_bounds__(256) void k_quantise4(const T *__restrict__ x, int6
 // v_permlane swaps), so that lane q has the q-th 8 codes of each 32.  Lines of 128 bytes are read whole while they are there
 // (16 waves' rows are four times the L1 cache): two steps' codes at once, and a row's scales 16 groups at once, into LDS,
 // which the lanes of the row then read.
+//
+// 32768 x 8192 and one row of bf16: 36 us (4.2 TB/s; the weights' bytes alone would take 23), 11003 x 4096 and 16 rows of f16: 19 (5).  Both
+// wait for the issue of instructions rather than for memory: two waves to a SIMD at most, by their registers.
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
