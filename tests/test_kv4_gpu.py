@@ -337,6 +337,34 @@ def test_long_sequences(dev, t, hq, new, length):
     run(cache, table, lens, [new, 1], hq, TYPES[t], dev, spread=2.0)
 
 
+def test_caches_and_tables_without_pages(dev):
+    """Nothing is written; rows without tokens get 0, rows that should see one NaN."""
+    x = torch.randn(2, 2, 64, device=dev)
+    for pages, width in ((0, 3), (4, 0), (0, 0)):
+        cache = KvCache4bit.empty(pages, 2, 16, 64, dev)
+        table = torch.zeros(2, width, dtype=torch.int32, device=dev)
+        outs = [torch.full_like(x, 9.0) for _ in range(3)]
+        cache.append(x, x, x, ints([0, 1], dev), ints([0, 5], dev), table, inv_freq=frequencies(64, dev), values=True, out=outs)
+        assert all(bool((o == 9).all()) for o in outs) and not any(bool(b.any()) for b, _ in cache._buffers())
+        out, lse = cache.attention(x, table, ints([0, 1, 2], dev), ints([0, 1], dev), lse=True)
+        assert not bool(out[0].any()) and bool((lse[0] == -math.inf).all())
+        assert bool(out[1].isnan().all()) and bool(lse[1].isnan().all())
+
+
+def test_calls_on_two_streams_at_once(dev):
+    """Calls that overlap have workspaces of their own."""
+    lens = [9000, 4000]
+    cache, table = filled(lens, 2, 64, 64, 15, dev)
+    q = [torch.randn(2, 8, 64, device=dev) for _ in range(2)]
+    args = (table, ints([0, 1, 2], dev), ints(lens, dev))
+    want = [cache.attention(x, *args) for x in q]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [cache.attention(q[i % 2], *args, stream=streams[i % 2]) for i in range(20)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
+
+
 @pytest.mark.parametrize("t", ["f32", "f16"])
 @pytest.mark.parametrize("lens,news,heads,hq", [([3000, 9000], [1, 90], 1, 1), ([700] * 5 + [6000], [1] * 5 + [150], 2, 8)])
 def test_one_sequence_of_many_rows_among_single_tokens(dev, lens, news, heads, hq, t):
