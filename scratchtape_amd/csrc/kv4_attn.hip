@@ -911,6 +911,15 @@ __global__ __launch_bounds__(256) void k_merge4(const AttnArgs a) {
     float *weight = weights[team];
     for (int y = blockIdx.y * TEAMS + team; y < rows; y += gridDim.y * TEAMS) {  // (with four waves a row all of the workgroup's)
         auto slot = [&](int i) { return (2 * (int64_t)min((int)blockIdx.x + i, a.groups - 1) + (i == 0 ? 1 : 0)) * a.part_rows + y; };
+        // The first parts' sums are under way while their weights are found (12 sequences with 5 tokens each 23.9 to 23.0 us, a prompt 531 to 528).
+        const int gr = me / LANES, e = 4 * (me % LANES);
+        float4 x[8];
+        auto load = [&](int i0) {
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (k == 0 || k * GROUPS < parts) x[k] = *(const float4 *)(a.part_o + slot(min(i0 + k * GROUPS, parts - 1)) * HD + e);
+        };
+        load(gr);
         float m = -INFINITY, l = 0.f;
         for (int i = me; i < parts; i += 64 * WAVES) {
             const float2 t = a.part_ml[slot(i)];
@@ -938,13 +947,10 @@ __global__ __launch_bounds__(256) void k_merge4(const AttnArgs a) {
             __syncthreads();
             sum = (stat[4] + stat[5]) + (stat[6] + stat[7]);
         }
-        const int gr = me / LANES, e = 4 * (me % LANES);
         if (gr < GROUPS) {
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int i0 = gr; i0 < parts; i0 += 8 * GROUPS) {  // eight loads under way
-                float4 x[8];
-#pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = *(const float4 *)(a.part_o + slot(min(i0 + k * GROUPS, parts - 1)) * HD + e);
+            for (int i0 = gr; i0 < parts; i0 += 8 * GROUPS) {
+                if (i0 > gr) load(i0);
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     const float w = i0 + k * GROUPS < parts ? weight[i0 + k * GROUPS] : 0.f;
