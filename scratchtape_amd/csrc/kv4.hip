@@ -15,7 +15,7 @@ using st::page_of;
 struct AppendArgs {
     int64_t n, q_stride, k_stride, v_stride;
     int32_t hq, hd, half, interleaved, stretch;
-    bool vec_q, vec_k, vec_v, vec_out;
+    bool vec, vec_out;
     const int32_t *seq, *pos;
     const float *inv_freq;
     uint8_t *k_codes, *v_codes;
@@ -35,43 +35,63 @@ struct Turn {
             c[i] = t.x, s[i] = second ? t.y : -t.y;
         }
     }
-    // The components e .. e + 7 of the vector `from`, x; the first 2 half are rotated.
-    template <class T>
-    __device__ __forceinline__ void operator()(const T *from, int e, bool vec, int half, bool interleaved, float (&x)[8]) const {
-        if (e >= 2 * half) return;
-        float other[8];
-        if (interleaved) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) other[i] = x[i ^ 1];
-        } else if (half % 8 == 0) {  // the eight others lie side by side
-            st::load8(from + (e >= half ? e - half : e + half), vec, other);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) other[i] = e + i >= 2 * half ? 0.f : (float)from[e + i >= half ? e + i - half : e + i + half];
-        }
+    __device__ __forceinline__ void operator()(int e, int half, float (&x)[8], const float (&other)[8]) const {
 #pragma unroll
         for (int i = 0; i < 8; i++)
             if (e + i < 2 * half) x[i] = (float)((double)x[i] * c[i] + (double)other[i] * s[i]);
     }
 };
 
+// Eight elements as they lie in memory.  vec: they are 16-byte aligned.
+template <class T>
+struct Eight {
+    typedef T V __attribute__((ext_vector_type(8), aligned(16)));
+    V v;
+    __device__ __forceinline__ void load(const T *p, bool vec) {
+        if (vec) {
+            v = *(const V *)p;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = p[i];
+        }
+    }
+};
+
 // A token's vectors (hq of q, then hkv of k, then hkv of v), `stretch` of them a workgroup, LANES lanes each, 8 components a
 // lane.  The cosines and sines are taken once a workgroup, in 64 bits; sequence, position and page are the same for all its lanes.
-// 8191 tokens of 48 vectors of 128 in f16, 210 MB: 67 us (3.1 TB/s), of which the waves wait for loads two thirds (233 us with the angles
-// taken for each component and 64-bit quotients).
+// 8191 tokens of 48 vectors of 128 in f16, 210 MB: 58 us (3.6 TB/s; 68 with loads behind the page's and the angles' and five waves a
+// SIMD instead of six, for which some registers are put away around the sines; 233 with the angles taken for each component and 64-bit quotients).  Bound by waits for loads.
 template <class T, int LANES>
-__global__ __launch_bounds__(256) void k_append4(const T *__restrict__ q, const T *__restrict__ k,
+__global__ __launch_bounds__(256, 6) void k_append4(const T *__restrict__ q, const T *__restrict__ k,
                                                  const T *__restrict__ v, T *__restrict__ q_out, T *__restrict__ k_out,
                                                  T *__restrict__ v_out, AppendArgs a) {
     __shared__ double2 turn[128];
     const int hq = a.hq, hkv = a.cache.hkv, e = (threadIdx.x % LANES) * 8;
     const int64_t token = (int64_t)blockIdx.z * gridDim.x + blockIdx.x;
     if (token >= a.n) return;
+    const int begin = blockIdx.y * a.stretch, end = min(begin + a.stretch, hq + 2 * hkv);
+    // The lane's components of a vector and the seconds of their pairs, a pass ahead (lanes without a vector repeat another's).
+    Eight<T> mine, pairs;
+    const int es = e < a.hd ? e : 0;
+    auto fetch = [&](int first) {
+        const int head = min(first + (int)threadIdx.x / LANES, end - 1);
+        const bool is_q = head < hq, is_k = !is_q && head < hq + hkv;
+        const T *from = is_q ? q + token * a.q_stride + (int64_t)head * a.hd
+                             : is_k ? k + token * a.k_stride + (int64_t)(head - hq) * a.hd : v + token * a.v_stride + (int64_t)(head - hq - hkv) * a.hd;
+        mine.load(from + es, a.vec);
+        if (a.interleaved) return;
+        if (a.half % 8 == 0) {  // the eight others lie side by side
+            pairs.load(from + (es >= 2 * a.half ? es : es >= a.half ? es - a.half : es + a.half), a.vec);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) pairs.v[i] = from[es + i >= 2 * a.half ? es + i : es + i >= a.half ? es + i - a.half : es + i + a.half];
+        }
+    };
+    fetch(begin);
     const int64_t s = a.seq[token], pos = a.pos[token];
     if (s < 0 || s >= a.cache.nseq || pos < 0) return;
     const int64_t page = page_of(a.cache, s, pos);
     if (page < 0) return;
-    const int begin = blockIdx.y * a.stretch, end = min(begin + a.stretch, hq + 2 * hkv);
     if (a.half && begin < hq + hkv) {
         if ((int)threadIdx.x < a.half) {
             double si, co;
@@ -85,14 +105,12 @@ __global__ __launch_bounds__(256) void k_append4(const T *__restrict__ q, const 
         const int head = first + threadIdx.x / LANES;
         const bool used = head < end && e < a.hd, is_q = head < hq, is_k = !is_q && head < hq + hkv;
         const int h = is_q ? head : is_k ? head - hq : head - hq - hkv;
-        float x[8] = {};
-        if (used) {
-            const T *from = (is_q ? q + token * a.q_stride : is_k ? k + token * a.k_stride : v + token * a.v_stride) + (int64_t)h * a.hd;
-            const bool vec = is_q ? a.vec_q : is_k ? a.vec_k : a.vec_v;
-            st::load8(from + e, vec, x);
-            if (is_q || is_k) rotate(from, e, vec, a.half, a.interleaved, x);
-            if (is_q) st::store8(q_out + (token * hq + h) * a.hd + e, a.vec_out, x);
-        }
+        float x[8], other[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)mine.v[i], other[i] = (float)(a.interleaved ? mine.v[i ^ 1] : pairs.v[i]);
+        if (first + 256 / LANES < end) fetch(first + 256 / LANES);
+        if (head < hq + hkv) rotate(e, a.half, x, other);
+        if (used && is_q) st::store8(q_out + (token * hq + h) * a.hd + e, a.vec_out, x);
         if (first + 256 / LANES <= hq) continue;  // queries only
         float scale, lo;
         const uint32_t codes = st::quantise8<LANES>(x, used, scale, lo);
@@ -136,13 +154,13 @@ extern "C" st_status st_kv_append_4bit(const void *q, const void *k, const void 
     const int64_t queries = q ? hq : 0;
     a.n = n, a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
     a.hq = (int32_t)queries, a.hd = (int32_t)hd, a.half = (int32_t)rot / 2, a.interleaved = interleaved;
-    a.vec_q = st::rows_aligned(q, q_stride, size), a.vec_k = st::rows_aligned(k, k_stride, size), a.vec_v = st::rows_aligned(v, v_stride, size);
+    a.vec = (!q || st::rows_aligned(q, q_stride, size)) && st::rows_aligned(k, k_stride, size) && st::rows_aligned(v, v_stride, size);
     a.vec_out = (((uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0;
     a.seq = seq, a.pos = pos, a.inv_freq = inv_freq;
     a.k_codes = k_codes, a.v_codes = v_codes, a.k_scales = (float2 *)k_scales, a.v_scales = (float2 *)v_scales;
     const int64_t lanes = hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32;
-    // With tokens enough to fill the chip a workgroup takes a whole token (8191 tokens of 48 vectors of 128: 68 us, 98 with a pass
-    // of 16 vectors each, which take the sines three times); with few, one pass (64 tokens: 5.1 us, 6.2).
+    // With tokens enough to fill the chip a workgroup takes a whole token (8191 tokens of 48 vectors of 128: 59 us, 90 with a pass
+    // of 16 vectors each, which take the sines three times); with few, one pass (64 tokens: 5.5 us, 6.4).
     const int64_t vectors = queries + 2 * hkv, once = 256 / lanes;
     a.stretch = (int32_t)(n >= 1024 ? vectors : once);
     const int64_t along = std::min<int64_t>(n, 1 << 23);  // (a launch holds less than 2^32 threads along x)
