@@ -29,7 +29,7 @@
 // through its stretch of the line unit by unit; waves without rows of their own share the unit's keys.  What a workgroup
 // has of a unit that others work on too goes to its slots in `work`, and k_merge4 joins the parts.
 //
-// 32 heads over 8 of 128: 64 sequences of 200 to 8192 keys (311 MB) 81 to 86 us, one of 131072 (151 MB) 47 (3.2 TB/s), 2048 rows of a prompt over 8192
+// 32 heads over 8 of 128: 64 sequences of 200 to 8192 keys (311 MB) 75 to 86 us, one of 131072 (151 MB) 47 (3.2 TB/s), 2048 rows of a prompt over 8192
 // keys (240 GFLOP) 530 (450 TFLOP/s).  The first two are the arithmetic of three waves a SIMD (70 percent issue) and units' starts, the last
 // that of two (72 percent, the matrix cores busy 23).
 #include <algorithm>
