@@ -58,9 +58,10 @@ struct Eight {
 };
 
 // A token's vectors (hq of q, then hkv of k, then hkv of v), `stretch` of them a workgroup, LANES lanes each, 8 components a
-// lane.  The cosines and sines are taken once a workgroup, in 64 bits; sequence, position and page are the same for all its lanes.
-// 8191 tokens of 48 vectors of 128 in f16, 210 MB: 58 us (3.6 TB/s; 68 with loads behind the page's and the angles' and five waves a
-// SIMD instead of six, for which some registers are put away around the sines; 233 with the angles taken for each component and 64-bit quotients).  Bound by waits for loads.
+// lane.  The cosines and sines are taken once a workgroup, in 64 bits; sequence, position and page are the same for all its
+// lanes. 8191 tokens of 48 vectors of 128 in f16, 210 MB: 58 us (3.6 TB/s; 68 with loads behind the page's and the angles' and
+// five waves a SIMD instead of six, for which some registers are put away around the sines; 233 with the angles taken for each
+// component and 64-bit quotients).  Bound by waits for loads.
 template <class T, int LANES>
 __global__ __launch_bounds__(256, 6) void k_append4(const T *__restrict__ q, const T *__restrict__ k,
                                                  const T *__restrict__ v, T *__restrict__ q_out, T *__restrict__ k_out,
@@ -138,10 +139,15 @@ extern "C" st_status st_kv_append_4bit(const void *q, const void *k, const void 
     const char *name = "kv_append_4bit";
     if (!st::heads_ok(name, hq, hkv, hd)) return ST_ERR_INVALID;
     if (n < 0 || n > INT32_MAX) return st::fail(ST_ERR_INVALID, "%s: %lld tokens", name, (long long)n);
-    if (dtype < ST_F32 || dtype > ST_BF16) return st::fail(ST_ERR_INVALID, "%s: dtype %d is none of ST_F32, ST_F16, ST_BF16", name, (int)dtype);
-    if (rot < 0 || rot > hd || (rot & 1)) return st::fail(ST_ERR_INVALID, "%s: %lld rotated components of %lld (an even number of them)", name, (long long)rot, (long long)hd);
+    if (dtype < ST_F32 || dtype > ST_BF16)
+        return st::fail(ST_ERR_INVALID, "%s: dtype %d is none of ST_F32, ST_F16, ST_BF16",
+                        name, (int)dtype);
+    if (rot < 0 || rot > hd || (rot & 1))
+        return st::fail(ST_ERR_INVALID, "%s: %lld rotated components of %lld (an even number of them)",
+                        name, (long long)rot, (long long)hd);
     if ((q && q_stride < hq * hd) || k_stride < hkv * hd || v_stride < hkv * hd)
-        return st::fail(ST_ERR_INVALID, "%s: tokens lie %lld, %lld, %lld elements apart, less than their heads", name, (long long)q_stride, (long long)k_stride, (long long)v_stride);
+        return st::fail(ST_ERR_INVALID, "%s: tokens lie %lld, %lld, %lld elements apart, less than their heads",
+                        name, (long long)q_stride, (long long)k_stride, (long long)v_stride);
     AppendArgs a = {};
     if (!st::cache_ok(name, a.cache, nseq, table, max_pages, pages, page, hkv, k_codes, k_scales, v_codes, v_scales)) return ST_ERR_INVALID;
     if (n == 0) return ST_OK;

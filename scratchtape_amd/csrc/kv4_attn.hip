@@ -7,12 +7,12 @@
 //   sum_j p_j v_j = sum_j (p_j aV_j) (cV_j - 8) + sum_j p_j b8V_j
 // Both products run on the matrix cores, codes as f16 integers from -8 to 7 (exact, a VALU operation per code): around 0, so
 // that the rounding of the weights p aV to f16 is not multiplied by an offset.  (Nibbles masked in place are f16 subnormals n
-// 2^-24, half the work, and the matrix cores take them; but they line up the sums by the exponent that subnormals share,
-// and lose the 6 to 10 bits that n leaves unused: 4e-5 off in f32.)
-// Rows are scaled by a power of two to f16 (f32 rows, PARTS = 2, as two f16 parts, 22 bits), scores and sums are f32; the
-// weights are rounded to f16, in two parts for f32 rows and for few rows of f16.  A row's reference M is no running maximum of its scores but follows
-// max(z log2 e + log2 aV), so that p aV stays inside f16's normal range whatever the sizes of the values; it is raised only
-// where p aV would pass 2^15, so the common tile has no reduction over lanes at all.
+// 2^-24, half the work, and the matrix cores take them; but they line up the sums by the exponent that subnormals share, and
+// lose the 6 to 10 bits that n leaves unused: 4e-5 off in f32.) Rows are scaled by a power of two to f16 (f32 rows, PARTS = 2,
+// as two f16 parts, 22 bits), scores and sums are f32; the weights are rounded to f16, in two parts for f32 rows and for few
+// rows of f16.  A row's reference M is no running maximum of its scores but follows max(z log2 e + log2 aV), so that p aV stays
+// inside f16's normal range whatever the sizes of the values; it is raised only where p aV would pass 2^15, so the common tile
+// has no reduction over lanes at all.
 //
 // What the kernel spends is the taking apart of codes, about a VALU operation each for K and for V, and the scores'
 // arithmetic; both would leave memory waiting, so the rest is arranged around them.  A wave has 16 RT rows and takes 32 keys at
@@ -29,9 +29,9 @@
 // through its stretch of the line unit by unit; waves without rows of their own share the unit's keys.  What a workgroup
 // has of a unit that others work on too goes to its slots in `work`, and k_merge4 joins the parts.
 //
-// 32 heads over 8 of 128: 64 sequences of 200 to 8192 keys (311 MB) 75 to 86 us, one of 131072 (151 MB) 47 (3.2 TB/s), 2048 rows of a prompt over 8192
-// keys (240 GFLOP) 530 (450 TFLOP/s).  The first two are the arithmetic of three waves a SIMD (70 percent issue) and units' starts, the last
-// that of two (72 percent, the matrix cores busy 23).
+// 32 heads over 8 of 128: 64 sequences of 200 to 8192 keys (311 MB) 75 to 86 us, one of 131072 (151 MB) 47 (3.2 TB/s), 2048
+// rows of a prompt over 8192 keys (240 GFLOP) 530 (450 TFLOP/s).  The first two are the arithmetic of three waves a SIMD (70
+// percent issue) and units' starts, the last that of two (72 percent, the matrix cores busy 23).
 #include <algorithm>
 #include <cmath>
 
@@ -50,11 +50,11 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// Of the line for a workgroup at least: at 128, 256 and 512 one sequence of 128 keys takes 9.7, 10.1 and 10.2 us, 12 with 5 tokens each 25.2,
-// 24.3 and 29.4.
+// Of the line for a workgroup at least: at 128, 256 and 512 one sequence of 128 keys takes 9.7, 10.1 and 10.2 us, 12 with 5
+// tokens each 25.2, 24.3 and 29.4.
 constexpr int MIN_STRETCH = 256;
-// What a unit's start costs (finding it, its rows, its first loads, its end), in keys: at 256, 512, 768 and 1024, 64 ragged sequences take
-// 95, 89, 89 and 91 us, 12 with 5 tokens each 24.5, 24.3, 26.3 and 27.9.
+// What a unit's start costs (finding it, its rows, its first loads, its end), in keys: at 256, 512, 768 and 1024, 64 ragged
+// sequences take 95, 89, 89 and 91 us, 12 with 5 tokens each 24.5, 24.3, 26.3 and 27.9.
 constexpr int LEAD = 512;
 // Units of up to so many keys are not shared among workgroups, as a merge would cost more: at 0, 512 and 2048, one sequence of 128
 // keys takes 13.0, 11.2 and 11.2 us, 64 ragged ones 83, 83 and 87, 12 with 5 tokens each 24.7, 24.7 and 40.
@@ -695,8 +695,8 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
             const bool masked = kt + 31 > pos_first || kt + 31 >= end || (window > 0 && kt <= pos_last - window);
             bool careful = false;
             if (masked || bad_halves) {
-                // What lies behind the end counts nothing, whatever it holds; keys on a page outside the cache are NaN to the rows that
-                // see them; and a value that is not finite must not reach the rows that do not see it, as 0 times it.
+                // What lies behind the end counts nothing, whatever it holds; keys on a page outside the cache are NaN to the
+                // rows that see them; and a value that is not finite must not reach the rows that do not see it, as 0 times it.
                 const int k = lane & 31;
                 const bool gone = bad_halves & (k & 16 ? 2 : 1);
                 float2 *kp = (float2 *)(tile + R::PAIRS) + k, *vp = kp + 32;
@@ -749,9 +749,9 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
                     }
                 }
             };
-            // p = 2^(z - R) and p aV of every row.  For the first tile, and where p aV would pass f16's range or p an f32's, the scores
-            // are taken again to set R: seldom, and the common tile holds no registers for it.
-            // (The tile's p are no larger than their sum.)
+            // p = 2^(z - R) and p aV of every row.  For the first tile, and where p aV would pass f16's range or p an f32's,
+            // the scores are taken again to set R: seldom, and the common tile holds no registers for it. (The tile's p are no
+            // larger than their sum.)
             float p[RT][2][4], sum[RT];
             h8 ph[RT], pr[WEIGHTS == 2 ? RT : 1];
             auto weights = [&](const char *tile) {  // p aV in f16, rounded once
@@ -911,7 +911,8 @@ __global__ __launch_bounds__(256) void k_merge4(const AttnArgs a) {
     float *weight = weights[team];
     for (int y = blockIdx.y * TEAMS + team; y < rows; y += gridDim.y * TEAMS) {  // (with four waves a row all of the workgroup's)
         auto slot = [&](int i) { return (2 * (int64_t)min((int)blockIdx.x + i, a.groups - 1) + (i == 0 ? 1 : 0)) * a.part_rows + y; };
-        // The first parts' sums are under way while their weights are found (12 sequences with 5 tokens each 23.9 to 23.0 us, a prompt 531 to 528).
+        // The first parts' sums are under way while their weights are found (12 sequences with 5 tokens each 23.9 to 23.0 us, a
+        // prompt 531 to 528).
         const int gr = me / LANES, e = 4 * (me % LANES);
         float4 x[8];
         auto load = [&](int i0) {
@@ -992,8 +993,8 @@ struct Cut {
 Cut cut_of(int32_t dtype, int64_t n, int64_t nseq, int64_t hq, int64_t hkv, int64_t hd, int64_t max_pages, int64_t page) {
     Cut c;
     const int64_t rows = n * (hq / hkv);
-    // 32 rows a wave share the work of taking codes apart, but keep two waves to a SIMD and not three: sequences of 16 rows on average take
-    // 95 us with 16 and 112 with 32 a wave, of 64 rows 265 and 195.
+    // 32 rows a wave share the work of taking codes apart, but keep two waves to a SIMD and not three: sequences of 16 rows on
+    // average take 95 us with 16 and 112 with 32 a wave, of 64 rows 265 and 195.
     c.rt = hd <= 128 && rows >= 64 * nseq ? 2 : 1, c.rows = 64 * c.rt;
     const int per_cu = c.rt == 1 && hd <= 128 ? 3 : 2;
     c.groups = std::min(per_cu * st::device_cus(), MAX_GROUPS) & ~7;
@@ -1022,16 +1023,26 @@ extern "C" st_status st_kv_attention_4bit(const void *q, int32_t dtype, int64_t 
     st::clear_error();
     const char *name = "kv_attention_4bit";
     if (!st::heads_ok(name, hq, hkv, hd)) return ST_ERR_INVALID;
-    if (n < 0 || n > INT32_MAX / hq / 256) return st::fail(ST_ERR_INVALID, "%s: %lld rows of %lld heads (up to 2^23 in all)", name, (long long)n, (long long)hq);
-    if (dtype < ST_F32 || dtype > ST_BF16) return st::fail(ST_ERR_INVALID, "%s: dtype %d is none of ST_F32, ST_F16, ST_BF16", name, (int)dtype);
-    if (q_stride < hq * hd) return st::fail(ST_ERR_INVALID, "%s: rows of %lld elements lie %lld apart", name, (long long)(hq * hd), (long long)q_stride);
-    if (window < 0 || (window > 0 && !causal)) return st::fail(ST_ERR_INVALID, "%s: a window of %lld keys%s", name, (long long)window, causal ? "" : " without the causal mask");
+    if (n < 0 || n > INT32_MAX / hq / 256)
+        return st::fail(ST_ERR_INVALID, "%s: %lld rows of %lld heads (up to 2^23 in all)",
+                        name, (long long)n, (long long)hq);
+    if (dtype < ST_F32 || dtype > ST_BF16)
+        return st::fail(ST_ERR_INVALID, "%s: dtype %d is none of ST_F32, ST_F16, ST_BF16",
+                        name, (int)dtype);
+    if (q_stride < hq * hd)
+        return st::fail(ST_ERR_INVALID, "%s: rows of %lld elements lie %lld apart",
+                        name, (long long)(hq * hd), (long long)q_stride);
+    if (window < 0 || (window > 0 && !causal))
+        return st::fail(ST_ERR_INVALID, "%s: a window of %lld keys%s",
+                        name, (long long)window, causal ? "" : " without the causal mask");
     AttnArgs a = {};
     if (!st::cache_ok(name, a.c, nseq, table, max_pages, pages, page, hkv, k_codes, k_scales, v_codes, v_scales)) return ST_ERR_INVALID;
     if (n == 0 || nseq == 0) return ST_OK;
     if (!q || !q_start || !kv_len || !out) return st::fail(ST_ERR_INVALID, "%s: NULL buffer", name);
     const int64_t size = st::dtype_size(dtype);
-    if (((uintptr_t)q | (uintptr_t)out) & (size - 1)) return st::fail(ST_ERR_INVALID, "%s: q or out not aligned to its elements", name);
+    if (((uintptr_t)q | (uintptr_t)out) & (size - 1))
+        return st::fail(ST_ERR_INVALID, "%s: q or out not aligned to its elements",
+                        name);
     const Cut cut = cut_of(dtype, n, nseq, hq, hkv, hd, max_pages, page);
     if (cut.part_rows > 0 && (!work || ((uintptr_t)work & 15) || work_bytes < work_of(cut, hd)))
         return st::fail(ST_ERR_INVALID, "%s: work is %lld bytes of 16-byte aligned device memory, got %lld", name,

@@ -9,8 +9,8 @@
 namespace {
 
 // One thread per 8 values; a group is 4, 8 or 16 neighbouring lanes.  `width`: 8-value units of a row (of all rows, where they
-// lie behind each other).  Bound by HBM: 16384 x 8192 bf16 with values, 612 MB, 122 us (5.0 TB/s, a large copy's rate; 154 us with a 64-bit
-// quotient for each value).
+// lie behind each other).  Bound by HBM: 16384 x 8192 bf16 with values, 612 MB, 122 us (5.0 TB/s, a large copy's rate; 154 us
+// with a 64-bit quotient for each value).
 template <class T, int GROUP>
 __global__ __launch_bounds__(256) void k_quantise4(const T *__restrict__ x, int64_t total, int64_t width, int64_t stride,
                                                    bool vec, uint32_t *__restrict__ codes, float2 *__restrict__ scales,
@@ -55,8 +55,8 @@ __global__ __launch_bounds__(256) void k_quantise4(const T *__restrict__ x, int6
 // (16 waves' rows are four times the L1 cache): two steps' codes at once, and a row's scales 16 groups at once, into LDS,
 // which the lanes of the row then read.
 //
-// 32768 x 8192 and one row of bf16: 36 us (4.2 TB/s; the weights' bytes alone would take 23), 11003 x 4096 and 16 rows of f16: 19 (5).  Both
-// wait for the issue of instructions rather than for memory: two waves to a SIMD at most, by their registers.
+// 32768 x 8192 and one row of bf16: 36 us (4.2 TB/s; the weights' bytes alone would take 23), 11003 x 4096 and 16 rows of f16:
+// 19 (5).  Both wait for the issue of instructions rather than for memory: two waves to a SIMD at most, by their registers.
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -85,9 +85,9 @@ __device__ __forceinline__ f4 product(u4 a, u4 b, f4 c) {
 // The upper halves (bf16 parts) of two f32 words, the first below.
 __device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
 
-// 8 codes as the products' operand, in the order 0 4 1 5 2 6 3 7.  Beside f16 and bf16 rows: 16 + c, the exponent of 16 with c in
-// the upper four bits of the mantissa.  Beside f32's parts: (c - 8) / 16 in bf16 (twice the operations), as an f32 sum has no bits to
-// spare for an offset (groups of 128 of 4096: 2.2e-6 off with 16 + c).
+// 8 codes as the products' operand, in the order 0 4 1 5 2 6 3 7.  Beside f16 and bf16 rows: 16 + c, the exponent of 16 with c
+// in the upper four bits of the mantissa.  Beside f32's parts: (c - 8) / 16 in bf16 (twice the operations), as an f32 sum has
+// no bits to spare for an offset (groups of 128 of 4096: 2.2e-6 off with 16 + c).
 template <class T>
 struct Numbers {
     uint32_t mask, exponent, ones;
@@ -335,10 +335,18 @@ extern "C" st_status st_quantize_4bit(const void *x, int32_t dtype, int64_t n, i
     if (n < 0 || k <= 0) return st::fail(ST_ERR_INVALID, "quantize_4bit: n %lld, k %lld", (long long)n, (long long)k);
     if (group != 32 && group != 64 && group != 128)
         return st::fail(ST_ERR_INVALID, "quantize_4bit: group %lld is none of 32, 64, 128", (long long)group);
-    if (k % group) return st::fail(ST_ERR_INVALID, "quantize_4bit: k %lld is not a multiple of the group %lld", (long long)k, (long long)group);
-    if (x_stride < k) return st::fail(ST_ERR_INVALID, "quantize_4bit: rows of %lld elements lie %lld apart", (long long)k, (long long)x_stride);
-    if (n > (((int64_t)1 << 31) - 1) * 256 / (k / 8)) return st::fail(ST_ERR_INVALID, "quantize_4bit: %lld x %lld values are too many for one call", (long long)n, (long long)k);
-    if (dtype < ST_F32 || dtype > ST_BF16) return st::fail(ST_ERR_INVALID, "quantize_4bit: dtype %d is none of ST_F32, ST_F16, ST_BF16", (int)dtype);
+    if (k % group)
+        return st::fail(ST_ERR_INVALID, "quantize_4bit: k %lld is not a multiple of the group %lld",
+                        (long long)k, (long long)group);
+    if (x_stride < k)
+        return st::fail(ST_ERR_INVALID, "quantize_4bit: rows of %lld elements lie %lld apart",
+                        (long long)k, (long long)x_stride);
+    if (n > (((int64_t)1 << 31) - 1) * 256 / (k / 8))
+        return st::fail(ST_ERR_INVALID, "quantize_4bit: %lld x %lld values are too many for one call",
+                        (long long)n, (long long)k);
+    if (dtype < ST_F32 || dtype > ST_BF16)
+        return st::fail(ST_ERR_INVALID, "quantize_4bit: dtype %d is none of ST_F32, ST_F16, ST_BF16",
+                        (int)dtype);
     if (n == 0) return ST_OK;
     if (!x || !codes || !scales) return st::fail(ST_ERR_INVALID, "quantize_4bit: NULL buffer");
     const int64_t size = st::dtype_size(dtype);
@@ -370,15 +378,23 @@ extern "C" st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int
                                     const uint8_t *codes, const float *scales, int64_t group, int64_t n,
                                     const float *bias, int32_t relu, void *out, int64_t out_stride, st_stream stream) {
     st::clear_error();
-    if (m < 0 || k <= 0 || n < 0) return st::fail(ST_ERR_INVALID, "matvec_4bit: m %lld, k %lld, n %lld", (long long)m, (long long)k, (long long)n);
+    if (m < 0 || k <= 0 || n < 0)
+        return st::fail(ST_ERR_INVALID, "matvec_4bit: m %lld, k %lld, n %lld",
+                        (long long)m, (long long)k, (long long)n);
     if (group != 32 && group != 64 && group != 128)
         return st::fail(ST_ERR_INVALID, "matvec_4bit: group %lld is none of 32, 64, 128", (long long)group);
-    if (k % group) return st::fail(ST_ERR_INVALID, "matvec_4bit: k %lld is not a multiple of the group %lld", (long long)k, (long long)group);
+    if (k % group)
+        return st::fail(ST_ERR_INVALID, "matvec_4bit: k %lld is not a multiple of the group %lld",
+                        (long long)k, (long long)group);
     if (m > 1 << 19 || k > 1 << 20 || n > 1 << 28)  // (a launch holds less than 2^32 threads along x, 2^16 workgroups along y)
-        return st::fail(ST_ERR_INVALID, "matvec_4bit: m %lld (up to 2^19), k %lld (up to 2^20), n %lld (up to 2^28)", (long long)m, (long long)k, (long long)n);
+        return st::fail(ST_ERR_INVALID, "matvec_4bit: m %lld (up to 2^19), k %lld (up to 2^20), n %lld (up to 2^28)",
+                        (long long)m, (long long)k, (long long)n);
     if (x_stride < k || out_stride < n)
-        return st::fail(ST_ERR_INVALID, "matvec_4bit: rows of %lld and %lld elements lie %lld and %lld apart", (long long)k, (long long)n, (long long)x_stride, (long long)out_stride);
-    if (dtype < ST_F32 || dtype > ST_BF16) return st::fail(ST_ERR_INVALID, "matvec_4bit: dtype %d is none of ST_F32, ST_F16, ST_BF16", (int)dtype);
+        return st::fail(ST_ERR_INVALID, "matvec_4bit: rows of %lld and %lld elements lie %lld and %lld apart",
+                        (long long)k, (long long)n, (long long)x_stride, (long long)out_stride);
+    if (dtype < ST_F32 || dtype > ST_BF16)
+        return st::fail(ST_ERR_INVALID, "matvec_4bit: dtype %d is none of ST_F32, ST_F16, ST_BF16",
+                        (int)dtype);
     if (m == 0 || n == 0) return ST_OK;
     if (!x || !codes || !scales || !out) return st::fail(ST_ERR_INVALID, "matvec_4bit: NULL buffer");
     const int64_t size = st::dtype_size(dtype);
@@ -395,10 +411,10 @@ extern "C" st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int
         };
         auto pick = [&](auto group_) {
             constexpr int GROUP = decltype(group_)::value;
-            // Rows of weights a workgroup (16 NT): with more of them x is read and summed less often, with fewer there are workgroups
-            // for every CU.  us at NT 1, 2, 4: 32768 x 8192 in groups of 128, one row of bf16: 48.8, 42.3, 38.8; 11003 x 4096 in groups
-            // of 32, 16 rows of f16: 23.9, 22.2, 20.2; 1024 x 256, one row of f32: 4.05 and 10.9 at NT 1 and 4.  f32's three parts
-            // leave registers for half as many tiles, and 16 rows of x at a time.
+            // Rows of weights a workgroup (16 NT): with more of them x is read and summed less often, with fewer there are
+            // workgroups for every CU.  us at NT 1, 2, 4: 32768 x 8192 in groups of 128, one row of bf16: 48.8, 42.3, 38.8;
+            // 11003 x 4096 in groups of 32, 16 rows of f16: 23.9, 22.2, 20.2; 1024 x 256, one row of f32: 4.05 and 10.9 at NT 1
+            // and 4.  f32's three parts leave registers for half as many tiles, and 16 rows of x at a time.
             constexpr int WIDE = sizeof(T) == 2 ? 4 : 2;
             if constexpr (sizeof(T) == 2)
                 if (m > 16) return go(k_matvec4<T, GROUP, 2, 2>, 2, 2);
