@@ -107,8 +107,9 @@ class KvCache4bit:
                     raise ValueError("out[0] is given without q")
                 _plain(t, k.dtype, shape, name)
         ins = [(q, "q"), (k, "k"), (v, "v"), (seq, "seq"), (pos, "pos"), (table, "table"), (inv_freq, "inv_freq")]
-        _apart([(t, f"out[{i}]") for i, t in enumerate(outs)] + self._buffers(), ins)
-        _on_gpu(k, ins + self._buffers() + [(t, f"out[{i}]") for i, t in enumerate(outs)])
+        written = [(outs[0], "out[0]"), (outs[1], "out[1]"), (outs[2], "out[2]")] + self._buffers()
+        _apart(written, ins)
+        _on_gpu(k, ins + written)
         with _launch(k.device, stream) as handle:
             wanted = (True, values, values)
             q_out, k_out, v_out = (t if t is not None or shape is None or not want else
@@ -116,8 +117,8 @@ class KvCache4bit:
                                    for t, shape, want in zip(outs, shapes, wanted))
             _lib.call("st_kv_append_4bit", _addr(q), k.data_ptr(), v.data_ptr(), dtype, n, hq, heads, 2 * half, q_stride,
                       k_stride, v_stride, seq.data_ptr(), pos.data_ptr(), nseq, table.data_ptr(), max_pages, pages, page,
-                      _addr(inv_freq), rot, int(bool(interleaved)), *(t.data_ptr() for t, _ in self._buffers()),
-                      _addr(q_out), _addr(k_out), _addr(v_out), handle)
+                      _addr(inv_freq), rot, int(bool(interleaved)), self.k_codes.data_ptr(), self.k_scales.data_ptr(),
+                      self.v_codes.data_ptr(), self.v_scales.data_ptr(), _addr(q_out), _addr(k_out), _addr(v_out), handle)
         return [q_out, k_out, v_out] if values else q_out
 
     def attention(self, q: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
@@ -153,7 +154,7 @@ class KvCache4bit:
             work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
             _lib.call("st_kv_attention_4bit", q.data_ptr(), dtype, n, hq, heads, 2 * half, q_stride, q_start.data_ptr(),
                       kv_len.data_ptr(), nseq, table.data_ptr(), max_pages, pages, page,
-                      *(t.data_ptr() for t, _ in self._buffers()), float((2 * half) ** -0.5 if scale is None else scale),
+                      self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr(), float((2 * half) ** -0.5 if scale is None else scale),
                       int(bool(causal)), int(window), int(bool(one)), out.data_ptr(), _addr(stats), _addr(work), nbytes,
                       handle)
         return (out, stats) if lse else out

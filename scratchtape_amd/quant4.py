@@ -65,9 +65,13 @@ def _extent(t: torch.Tensor) -> Tuple[int, int]:
 
 def _apart(outs, ins) -> None:
     """No output shares memory with an input or with another output; (tensor or None, name) pairs."""
-    spans = [(*_extent(t), True, name) for t, name in outs if t is not None]
-    spans += [(*_extent(t), False, name) for t, name in ins if t is not None]
-    spans = [s for s in spans if s[0] < s[1]]
+    spans = []
+    for pairs, out in ((outs, True), (ins, False)):
+        for t, name in pairs:
+            if t is not None:
+                a, b = _extent(t)
+                if a < b:
+                    spans.append((a, b, out, name))
     spans.sort()
     # By their starts: an output may not start before the end of anything earlier, an input not before an output's.
     end = out_end = 0
@@ -75,9 +79,10 @@ def _apart(outs, ins) -> None:
         if a < (end if out else out_end):
             other = next(o for c, d, other_out, o in spans if c <= a < d and o != name and (out or other_out))
             raise ValueError(f"{name} shares memory with {other}" if out else f"{other} shares memory with {name}")
-        end = max(end, b)
-        if out:
-            out_end = max(out_end, b)
+        if b > end:
+            end = b
+        if out and b > out_end:
+            out_end = b
 
 
 def _on_gpu(first: torch.Tensor, tensors) -> None:
