@@ -11,8 +11,9 @@
 // lose the 6 to 10 bits that n leaves unused: 4e-5 off in f32.) Rows are scaled by a power of two to f16 (f32 rows, PARTS = 2,
 // as two f16 parts, 22 bits), scores and sums are f32; the weights are rounded to f16, in two parts for f32 rows and for few
 // rows of f16.  A row's reference M is no running maximum of its scores but follows max(z log2 e + log2 aV), so that p aV stays
-// inside f16's normal range whatever the sizes of the values; it is raised only where p aV would pass 2^15, so the common tile
-// has no reduction over lanes at all.
+// inside f16's normal range whatever the sizes of the values (and where |b8| is far above aV, as in a vector of equal components,
+// follows that, so that p b8 stays inside f32's); it is raised only where p aV would pass 2^15, p or p b8 a bound of theirs, so
+// the common tile has no reduction over lanes at all.
 //
 // What the kernel spends is the taking apart of codes, about a VALU operation each for K and for V, and the scores'
 // arithmetic; both would leave memory waiting, so the rest is arranged around them.  A wave has 16 RT rows and takes 32 keys at
@@ -61,8 +62,12 @@ constexpr int LEAD = 512;
 constexpr int WHOLE = 512;
 constexpr int MAX_GROUPS = 1024;  // workgroups of a launch
 constexpr float BASE = 7.f, MOST_X = 32768.f;  // p aV is set to 2^7 at most, and may grow to 2^15
-constexpr float MIN_E = -86.f, MOST_P = 101.f;  // values below 2^-86 of scale count as that for the reference: p <= 2^93, 2^101
-constexpr float MOST_SUM = 0x1p101f;  // of a tile's p (k_attention4), none of which is then larger
+// Scales below 2^-86 count as that for the reference, so that p is 2^93 at most when it is set; it may grow until a tile's sum
+// passes 2^101 (2^25 tiles stay within f32).
+constexpr float MIN_E = -86.f, MOST_SUM = 0x1p101f;
+// The part |b8| of a value counts for the reference too, 2^24 times less: p |b8| is set to 2^31 at most, and may grow until a tile's
+// sum of p b8 passes 2^60.  Only vectors of components that are nearly equal (|b8| above 2^24 aV) are set by it.
+constexpr float OFFSET = 0x1p-24f, MOST_LOW = 0x1p60f;
 
 // What k_merge4 joins: a unit's rows, the first of them head `head` of token `token`; the first part is in the odd slot of the
 // workgroup that this stands under, the others in the even slots of those behind it.
@@ -749,20 +754,23 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
                     }
                 }
             };
-            // p = 2^(z - R) and p aV of every row.  For the first tile, and where p aV would pass f16's range or p an f32's,
-            // the scores are taken again to set R: seldom, and the common tile holds no registers for it. (The tile's p are no
-            // larger than their sum.)
-            float p[RT][2][4], sum[RT];
+            // p = 2^(z - R), p aV and the sum of p b8 of every row.  For the first tile, and where p aV would pass f16's range or p
+            // or p b8 an f32's, the scores are taken again to set R: seldom, and the common tile holds no registers for it. (The
+            // tile's p are no larger than their sum.)
+            float p[RT][2][4], sum[RT], low_sum[RT];
             h8 ph[RT], pr[WEIGHTS == 2 ? RT : 1];
             auto weights = [&](const char *tile) {  // p aV in f16, rounded once
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) low_sum[rt] = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const float4 y = R::pairs(tile, true, i, r / 2, g);
-                        const float v = r & 1 ? y.z : y.x;
+                        const float v = r & 1 ? y.z : y.x, v8 = __builtin_fmaf(8.f, v, r & 1 ? y.w : y.y);  // v8: what a code of 8 stands for
 #pragma unroll
                         for (int rt = 0; rt < RT; rt++) {
+                            low_sum[rt] = __builtin_fmaf(p[rt][i][r], v8, low_sum[rt]);
                             ph[rt][4 * i + r] = (_Float16)__builtin_fmaf(p[rt][i][r], v, 0.f);
                             if constexpr (WEIGHTS == 2) pr[rt][4 * i + r] = (_Float16)__builtin_fmaf(p[rt][i][r], v, -(float)ph[rt][4 * i + r]);
                         }
@@ -791,6 +799,20 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
 #pragma unroll
                     for (int i = 0; i < 4; i++) most_x = __builtin_elementwise_max(most_x, h2{ph[rt][2 * i], ph[rt][2 * i + 1]});
                 past = most_p > MOST_SUM || (float)most_x[0] > MOST_X || (float)most_x[1] > MOST_X;
+                if (careful) {  // rows that see what is not finite are left alone: the others' references are as without it
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const float4 y = R::pairs(tile, true, i, r / 2, g);
+                            const float v8 = __builtin_fmaf(8.f, r & 1 ? y.z : y.x, r & 1 ? y.w : y.y);
+#pragma unroll
+                            for (int rt = 0; rt < RT; rt++) past = past || (__builtin_isfinite(v8) && fabsf(p[rt][i][r] * v8) > MOST_LOW);
+                        }
+                } else {  // (infinities that cancel leave NaN; a sum of p that is NaN is the scores')
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) past = past || (!(fabsf(low_sum[rt]) <= MOST_LOW) && sum[rt] == sum[rt]);
+                }
             }
             if (__any(past)) {
                 uint32_t from = uniform((uint32_t)(tile - mem));
@@ -806,7 +828,8 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const float4 y = R::pairs(again, true, i, r / 2, g);
-                            const float v = r & 1 ? y.z : y.x, e = v > 0.f ? (float)__builtin_amdgcn_frexp_expf(v) : MIN_E;
+                            const float v = r & 1 ? y.z : y.x, v8 = __builtin_fmaf(8.f, v, r & 1 ? y.w : y.y);
+                            const float size = fmaxf(v, fabsf(v8) * OFFSET), e = size > 0.f ? (float)__builtin_amdgcn_frexp_expf(size) : MIN_E;
                             m = fmaxf(m, p[rt][i][r] + fmaxf(e, MIN_E));
                         }
                     m = fmaxf(m, st::xor_lane(m, 16, lane));
@@ -833,6 +856,8 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
             for (int rt = 0; rt < RT; rt++) total[rt] += sum[rt];
             if (careful) {  // (a weight of 0 leaves even what is not a number out)
 #pragma unroll
+                for (int rt = 0; rt < RT; rt++) low_sum[rt] = 0.f;
+#pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
@@ -841,22 +866,14 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
 #pragma unroll
                         for (int rt = 0; rt < RT; rt++) {
                             const bool none = p[rt][i][r] == 0.f;
-                            low[rt] = none ? low[rt] : __builtin_fmaf(p[rt][i][r], v8, low[rt]);
+                            low_sum[rt] = none ? low_sum[rt] : __builtin_fmaf(p[rt][i][r], v8, low_sum[rt]);
                             ph[rt][4 * i + r] = none ? (_Float16)0.f : ph[rt][4 * i + r];
                             if constexpr (WEIGHTS == 2) pr[rt][4 * i + r] = none ? (_Float16)0.f : pr[rt][4 * i + r];
                         }
                     }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float4 y = R::pairs(tile, true, i, r / 2, g);
-                        const float v8 = __builtin_fmaf(8.f, r & 1 ? y.z : y.x, r & 1 ? y.w : y.y);  // what a code of 8 stands for
-#pragma unroll
-                        for (int rt = 0; rt < RT; rt++) low[rt] = __builtin_fmaf(p[rt][i][r], v8, low[rt]);
-                    }
             }
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) low[rt] += low_sum[rt];
             weigh_values<HD, WEIGHTS, RT>(take, [&](int b, int i) {  // keys 4 g .. of each half, whose rows lie in the order 0 4 8 12 1 ..
                 return *(const uint32_t *)(tile + 16 * (HD + R::HALF * (i >> 2)) + (4 * (i & 3) + g) * (HD / 2) + word_at<HD>(b, col));
             }, ph, pr, col, o);

@@ -1,0 +1,74 @@
+"""Attention over the paged 4-bit cache where the arithmetic inside has to reach far: values of all sizes beside one another,
+rows that see nothing beside rows that do, more rows than usual.  Against 64 bits (quant4_oracle)."""
+import math
+
+import pytest
+import torch
+
+import quant4_oracle as oracle
+from scratchtape_amd.kv4 import KvCache4bit
+from test_kv4_gpu import TYPES, check, filled, ints, run
+
+pytestmark = pytest.mark.gpu
+
+
+def place(table, page, s, at):
+    """Pages and slots of the tokens `at` (a tensor) of sequence s."""
+    return table[s].long()[at // page], at % page
+
+
+def set_pairs(scales, table, s, at, scale, lo):
+    """(scale, lo) of tokens `at` of sequence s, all heads; numbers or tensors of one a token."""
+    p, slot = place(table, scales.shape[2], s, at)
+    pair = torch.stack([torch.as_tensor(x, dtype=torch.float32, device=scales.device).expand(len(at)) for x in (scale, lo)], -1)
+    scales[p, :, slot] = pair[:, None, :].expand(-1, scales.shape[1], -1)
+
+
+# ---- values that are far from 0 and all alike --------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("length", [1, 40, 500, 6000])
+@pytest.mark.parametrize("value", [3e10, 1e11, -1e25, 1e35, 3e38])
+def test_constant_values_of_any_size(dev, value, length, t):
+    """A vector of equal values has scale 0 and stands for lo, however large: alone, and beside ordinary vectors."""
+    lens = [length, 33]
+    at = torch.arange(length, device=dev)
+    for which in (at, at[::3]):
+        cache, table = filled(lens, 2, 32, 64, 21, dev)
+        set_pairs(cache.v_scales, table, 0, which, 0.0, value)
+        run(cache, table, lens, [1, 1], 4, TYPES[t], dev)
+        run(cache, table, lens, [min(length, 70), 30], 4, TYPES[t], dev, one=True)
+
+
+def test_constant_values_of_opposite_sign(dev):
+    lens = [300, 7]
+    cache, table = filled(lens, 1, 16, 128, 22, dev)
+    at = torch.arange(300, device=dev)
+    set_pairs(cache.v_scales, table, 0, at, 0.0, torch.where(at % 2 == 0, 1e30, -1e30))
+    run(cache, table, lens, [1, 1], 2, torch.float32, dev)
+    run(cache, table, lens, [40, 1], 2, torch.float32, dev)
+
+
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("signs", [1, -1])
+def test_scores_that_rise_over_constant_values(dev, signs, new):
+    """Weights grow by up to 2^100 from a tile to the next, over values whose components are equal; one of the last tokens' is NaN,
+    and some rows see it."""
+    lens = [400, 400]
+    cache, table = filled(lens, 1, 16, 64, 28, dev)
+    at = torch.arange(400, device=dev)
+    for s in (0, 1):
+        set_pairs(cache.k_scales, table, s, at, 0.0, (at // 32).float() * (70 / 8 if s else 30 / 8))  # scores of 70, 30 a tile
+        set_pairs(cache.v_scales, table, s, at, 0.0, torch.where(at % 2 == 0, 1e11, signs * 1.1e11))
+    q = torch.ones(2 * new, 2, 64, device=dev)
+    start, kv_len = ints([0, new, 2 * new], dev), ints(lens, dev)
+    out, lse = cache.attention(q, table, start, kv_len, lse=True)
+    want = oracle.attention(q, cache, table, start, kv_len, 0.125, parts=2)
+    check(out, lse, want)
+    p, slot = place(table, 16, 0, at[390:391])
+    cache.v_scales[p, :, slot] = math.nan
+    out = cache.attention(q, table, start, kv_len)
+    seen = torch.zeros(2 * new, dtype=torch.bool, device=dev)
+    seen[max(0, new - 10):new] = True
+    assert bool(out[seen].isnan().all())
+    check(torch.where(seen[:, None, None], want[0].float(), out), None, want)
