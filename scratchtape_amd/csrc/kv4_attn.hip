@@ -75,6 +75,8 @@ struct Joint {
     int parts, rows, token, head;
 };
 
+constexpr float ROOM = 10.f;  // a power of two that a unit's parts are no more than (MAX_GROUPS)
+
 struct AttnArgs {
     Cache c;
     const void *q;
@@ -312,55 +314,75 @@ __device__ __forceinline__ void load_q(const AttnArgs &a, int64_t at, float (&x)
         st::load8((const __bf16 *)a.q + at, a.vec_q, x);
 }
 
+// x 2^d, d a whole number (or infinite).
+__device__ __forceinline__ float times_2_to(float x, float d) { return __builtin_amdgcn_ldexpf(x, (int)fminf(fmaxf(d, -1000.f), 1000.f)); }
+
 // The largest component's exponent in `most` (0 where it is 0 or not finite): a row is scaled by 2^(15 - it).
 __device__ __forceinline__ int lift_of(float most) {
     return most > 0.f && __builtin_isfinite(most) ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
 }
 
+// A row's sums to its output and log-sum-exp: v and l in units of 2^top, l at most 1.
+struct Ending {
+    float inv, shift, lse;
+    __device__ __forceinline__ Ending(const AttnArgs &a, float top, float l) {
+        const float units = a.one ? fmaxf(top, 0.f) : top;  // (the phantom weighs 1)
+        shift = a.one ? top - units : 0.f;
+        const float sum = times_2_to(l, shift) + (a.one ? __builtin_amdgcn_exp2f(-units) : 0.f);
+        inv = sum == 0.f ? 0.f : 1.f / sum;
+        lse = sum == 0.f ? -INFINITY : (units + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+    }
+    __device__ __forceinline__ float operator()(float v) const { return times_2_to(v * inv, shift); }
+};
+
 // The waves' sums of a tile's rows, each against the wave's own reference, joined: to out, or to the workgroup's slot of a
 // unit that others work on too.  `sums` [4 waves][wave_rows][hd + 4], `ml` [4][wave_rows]; `sharing` waves have the same rows.
+//
+// References follow the values' sizes and say little about weights: a wave whose values are all 0 is 2^86 and more below one
+// with ordinary ones.  So the joined row is in units of its largest weight, times 4, which takes the weights' sum to 1 at most
+// and the values' to no more than the largest value; references are whole, and so the factors powers of two.
 template <int HD>
 __device__ __forceinline__ void finish(const AttnArgs &a, const Task &u, const Span &span, const float *sums, const float2 *ml, int wave_rows,
                                        int sharing) {
     for (int i = threadIdx.x; i < span.rows * (HD / 8); i += 256) {
         const int y = i / (HD / 8), e = 8 * (i % (HD / 8)), w0 = y / wave_rows * sharing, z = y % wave_rows;
         float2 t[4];
-        float m = -INFINITY, l = 0.f, v[8] = {};
+        float top = -INFINITY, l = 0.f, v[8] = {};
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             t[k] = ml[min(w0 + k, 3) * wave_rows + z];
             if (k >= sharing) t[k] = make_float2(-INFINITY, 0.f);
-            m = fmaxf(m, t[k].x);
+            top = fmaxf(top, t[k].x + __builtin_amdgcn_logf(t[k].y));
         }
+        top = ceilf(top) + 2.f;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const float f = t[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t[k].x - m);
-            l += t[k].y * f;
+            const float d = t[k].x - top;  // (NaN where there is nothing)
+            l += times_2_to(t[k].y, d);
             if (k < sharing) {
                 float w[8];
                 st::load8(sums + ((w0 + k) * wave_rows + z) * (HD + 4) + e, true, w);
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(w[j], f, v[j]);
+                for (int j = 0; j < 8; j++) v[j] += times_2_to(w[j], d);
             }
         }
         if (u.cut0 > 0 || u.cut1 < u.keys) {
             const int64_t slot = (2 * (int64_t)u.me + (u.cut0 == 0 ? 1 : 0)) * a.part_rows + y;
             st::store8(a.part_o + slot * HD + e, true, v);
-            if (e == 0) a.part_ml[slot] = make_float2(m, l);
+            if (e == 0) a.part_ml[slot] = make_float2(top, l);
             continue;
         }
         const int64_t row = span.row_at(a, u, y);
-        const float top = a.one ? fmaxf(m, 0.f) : m, f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-        const float sum = l * f + (a.one ? __builtin_amdgcn_exp2f(-top) : 0.f), inv = sum == 0.f ? 0.f : f * __builtin_amdgcn_rcpf(sum);
+        const Ending ending(a, top, l);
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] *= inv;
+        for (int j = 0; j < 8; j++) v[j] = ending(v[j]);
         if (a.dtype == ST_F32)
             st::store8((float *)a.out + row * HD + e, a.vec_out, v);
         else if (a.dtype == ST_F16)
             st::store8((_Float16 *)a.out + row * HD + e, a.vec_out, v);
         else
             st::store8((__bf16 *)a.out + row * HD + e, a.vec_out, v);
-        if (a.lse && e == 0) a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+        if (a.lse && e == 0) a.lse[row] = ending.lse;
     }
 }
 
@@ -834,11 +856,13 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
                         }
                     m = fmaxf(m, st::xor_lane(m, 16, lane));
                     m = fmaxf(m, st::xor_lane(m, 32, lane));
-                    m = fmaxf(ref[rt], m - BASE);
-                    const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref[rt] - m);
-                    total[rt] *= keep, low[rt] *= keep;
+                    m = fmaxf(ref[rt], ceilf(m) - BASE);
+                    const float keep = ref[rt] - m;  // (NaN where there is nothing yet)
+                    total[rt] = times_2_to(total[rt], keep), low[rt] = times_2_to(low[rt], keep);
 #pragma unroll
-                    for (int j = 0; j < HD / 16; j++) o[rt][j] *= keep;
+                    for (int j = 0; j < HD / 16; j++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[rt][j][i] = times_2_to(o[rt][j][i], keep);
                     ref[rt] = m;
                     sum[rt] = 0.f;
 #pragma unroll
@@ -913,7 +937,9 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
     }
 }
 
-// Joins the parts of units that several workgroups worked on: out = sum 2^(M_i - M) O_i / sum 2^(M_i - M) l_i over a row's parts.
+// Joins the parts of units that several workgroups worked on: out = sum 2^(M_i - M) O_i / sum 2^(M_i - M) l_i over a row's parts,
+// M 2^ROOM above the largest, so that the sums pass neither 1 nor the largest value.  (l_i is between 1/8 and 1, so what is below
+// 2^-126 here weighs less than 2^-113.)
 // Workgroup (i, j) has the unit that begins in the launch's workgroup i, and WAVES waves to each row of its j-th 4 / WAVES, and of
 // those as many further on as the launch has in all.
 template <int HD, int WAVES>
@@ -952,9 +978,10 @@ __global__ __launch_bounds__(256) void k_merge4(const AttnArgs a) {
             __syncthreads();
             m = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
         }
+        m += ROOM;
         float sum = 0.f;
         for (int i = me; i < parts; i += 64 * WAVES) {
-            const float w = weight[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(weight[i] - m);
+            const float w = weight[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(weight[i] - m);  // a power of two
             weight[i] = w;
             sum += w * (i < 64 * WAVES ? l : a.part_ml[slot(i)].y);
         }
@@ -978,15 +1005,14 @@ __global__ __launch_bounds__(256) void k_merge4(const AttnArgs a) {
             *(float4 *)&red[team][gr][e] = v;
         }
         if constexpr (WAVES > 1) __syncthreads();
-        const float top = a.one ? fmaxf(m, 0.f) : m, f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-        const float all = sum * f + (a.one ? __builtin_amdgcn_exp2f(-top) : 0.f), inv = all == 0.f ? 0.f : f / all;
+        const Ending ending(a, m, sum);
         const int token = (int)(((float)(joint.head % a.share + y) + 0.5f) * a.inv_share);
         const int64_t row = (int64_t)(joint.token + token) * a.hq + joint.head + y - token * a.share;
         for (int d = me; d < HD; d += 64 * WAVES) {
             float v = 0.f;
 #pragma unroll
             for (int i = 0; i < GROUPS; i++) v += red[team][i][d];
-            v *= inv;
+            v = ending(v);
             const int64_t to = row * HD + d;
             if (a.dtype == ST_F32)
                 ((float *)a.out)[to] = v;
@@ -995,7 +1021,7 @@ __global__ __launch_bounds__(256) void k_merge4(const AttnArgs a) {
             else
                 ((__bf16 *)a.out)[to] = (__bf16)v;
         }
-        if (a.lse && me == 0) a.lse[row] = all == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(all)) * 0.693147180559945309f;
+        if (a.lse && me == 0) a.lse[row] = ending.lse;
         if constexpr (WAVES > 1) __syncthreads();  // a row's values are read before the next one's are written
     }
 }

@@ -72,3 +72,33 @@ def test_scores_that_rise_over_constant_values(dev, signs, new):
     seen[max(0, new - 10):new] = True
     assert bool(out[seen].isnan().all())
     check(torch.where(seen[:, None, None], want[0].float(), out), None, want)
+
+
+# ---- sums that are joined ----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("exponent", [20, 45, 80])
+@pytest.mark.parametrize("length,new,hd", [(300, 1, 64), (300, 40, 32), (5000, 1, 64), (5000, 200, 128)])
+def test_zero_values_weigh_as_much_beside_large_ones(dev, length, new, hd, exponent):
+    """Tokens whose values are all 0, in tiles and stretches of their own, beside tokens of large values."""
+    lens = [length, 17]
+    for run_of in (32, 1024):
+        cache, table = filled(lens, 1, 32, hd, 25, dev)
+        at = torch.arange(length, device=dev)
+        zero = at // run_of % 2 == 0
+        set_pairs(cache.v_scales, table, 0, at, torch.where(zero, 0.0, 2.0 ** exponent), torch.where(zero, 0.0, -7.0 * 2.0 ** exponent))
+        run(cache, table, lens, [new, 1], 2, torch.float32, dev, spread=0.1)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("length,new", [(64, 1), (300, 33), (3000, 1), (3000, 200)])
+def test_softmax1_of_low_scores_and_equal_values(dev, length, new, t):
+    """Weights of 2^-43 beside the phantom's: the output is as small, not 0."""
+    lens = [length, 17]
+    cache, table = filled(lens, 1, 32, 64, 26, dev)
+    at = torch.arange(length, device=dev)
+    set_pairs(cache.k_scales, table, 0, at, 0.0, -30.0 / 8)  # scores of -30 for a q of ones
+    set_pairs(cache.v_scales, table, 0, at, 0.0, 1.0)
+    q = torch.ones(new + 1, 2, 64, device=dev).to(TYPES[t])
+    start, kv_len = ints([0, new, new + 1], dev), ints(lens, dev)
+    out, lse = cache.attention(q, table, start, kv_len, lse=True, one=True)
+    check(out, lse, oracle.attention(q, cache, table, start, kv_len, 64 ** -0.5, parts=2 if t == "f32" else 1, one=True))
