@@ -75,6 +75,9 @@ struct Joint {
     int parts, rows, token, head;
 };
 
+// Once the values of a tile pass 2^40 in the reference, a wave counts the unit's values in 2^40: p aV at 2^7 would put p itself near
+// the end of f32's range (scales of 2^120: 2^-113, so that weights 2^12 below the largest were dropped).
+constexpr float LARGE = 40.f, MOST_VALUE = 0x1p40f;
 constexpr float ROOM = 10.f;  // a power of two that a unit's parts are no more than (MAX_GROUPS)
 
 struct AttnArgs {
@@ -717,11 +720,12 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
 #pragma unroll
             for (int j = 0; j < HD / 16; j++) o[rt][j] = f4{0.f, 0.f, 0.f, 0.f};
         }
+        bool large = false;  // values count in 2^LARGE
         auto process = [&](char *tile, int it, int bad_halves) {
             const int kt = first_key + it * step, key0 = kt + 4 * g;
             const bool masked = kt + 31 > pos_first || kt + 31 >= end || (window > 0 && kt <= pos_last - window);
             bool careful = false;
-            if (masked || bad_halves) {
+            if (masked || bad_halves || large) {
                 // What lies behind the end counts nothing, whatever it holds; keys on a page outside the cache are NaN to the
                 // rows that see them; and a value that is not finite must not reach the rows that do not see it, as 0 times it.
                 const int k = lane & 31;
@@ -729,7 +733,10 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
                 float2 *kp = (float2 *)(tile + R::PAIRS) + k, *vp = kp + 32;
                 const float2 v = *vp;
                 if (gone) *kp = make_float2(NAN, NAN);
-                if (gone || kt + k >= end) *vp = make_float2(0.f, 0.f);
+                if (gone || kt + k >= end)
+                    *vp = make_float2(0.f, 0.f);
+                else if (large)
+                    *vp = make_float2(times_2_to(v.x, -LARGE), times_2_to(v.y, -LARGE));
                 careful = __any(!gone && kt + k < end && !__builtin_isfinite(v.x + v.y));
             }
             // Scores of the tile less `shift`, in log2.
@@ -839,7 +846,27 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
             if (__any(past)) {
                 uint32_t from = uniform((uint32_t)(tile - mem));
                 asm volatile("" : "+s"(from));  // read again, not kept
-                const char *again = mem + from;
+                char *again = mem + from;
+                // The size of a value as the reference takes it, of its scale and its value for a code of 8.
+                auto size_of = [](float v, float v8) { return fmaxf(v, fabsf(v8) * OFFSET); };
+                float2 *const vp = (float2 *)(again + R::PAIRS) + 32 + (lane & 31);
+                const float2 v = *vp;
+                if (!large && __any(size_of(v.x, __builtin_fmaf(8.f, v.x, v.y)) >= MOST_VALUE)) {
+                    large = true;
+                    *vp = make_float2(times_2_to(v.x, -LARGE), times_2_to(v.y, -LARGE));
+                    // What is summed up: p is larger by what values are less, as far as its own range allows.
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        float all = fmaxf(total[rt], st::xor_lane(total[rt], 16, lane));
+                        all = fmaxf(all, st::xor_lane(all, 32, lane));
+                        const float up = fminf(fmaxf(100.f - (float)__builtin_amdgcn_frexp_expf(all), 0.f), LARGE);
+                        ref[rt] -= up, total[rt] = times_2_to(total[rt], up), low[rt] = times_2_to(low[rt], up - LARGE);
+#pragma unroll
+                        for (int j = 0; j < HD / 16; j++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[rt][j][i] = times_2_to(o[rt][j][i], up - LARGE);
+                    }
+                }
                 float zero[RT] = {};
                 scores(again, zero, p);
 #pragma unroll
@@ -850,9 +877,8 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const float4 y = R::pairs(again, true, i, r / 2, g);
-                            const float v = r & 1 ? y.z : y.x, v8 = __builtin_fmaf(8.f, v, r & 1 ? y.w : y.y);
-                            const float size = fmaxf(v, fabsf(v8) * OFFSET), e = size > 0.f ? (float)__builtin_amdgcn_frexp_expf(size) : MIN_E;
-                            m = fmaxf(m, p[rt][i][r] + fmaxf(e, MIN_E));
+                            const float scale = r & 1 ? y.z : y.x, size = size_of(scale, __builtin_fmaf(8.f, scale, r & 1 ? y.w : y.y));
+                            m = fmaxf(m, p[rt][i][r] + fmaxf(size > 0.f ? (float)__builtin_amdgcn_frexp_expf(size) : MIN_E, MIN_E));
                         }
                     m = fmaxf(m, st::xor_lane(m, 16, lane));
                     m = fmaxf(m, st::xor_lane(m, 32, lane));
@@ -914,6 +940,17 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
             __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the tile's last reads are over before it is overwritten
             if (it + STAGES < count) bring_tile(it + STAGES, slot);
             slot = slot + 1 == STAGES ? 0 : slot + 1;
+        }
+
+        if (large) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                low[rt] = times_2_to(low[rt], LARGE);
+#pragma unroll
+                for (int j = 0; j < HD / 16; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[rt][j][i] = times_2_to(o[rt][j][i], LARGE);
+            }
         }
 
         // The sums of the waves that share rows, each against the wave's own reference, meet in LDS.

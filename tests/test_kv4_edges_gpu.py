@@ -102,3 +102,42 @@ def test_softmax1_of_low_scores_and_equal_values(dev, length, new, t):
     start, kv_len = ints([0, new, new + 1], dev), ints(lens, dev)
     out, lse = cache.attention(q, table, start, kv_len, lse=True, one=True)
     check(out, lse, oracle.attention(q, cache, table, start, kv_len, 64 ** -0.5, parts=2 if t == "f32" else 1, one=True))
+
+
+# ---- large values ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("exponent", [30, 50, 90, 115, 120])
+@pytest.mark.parametrize("length,new", [(512, 1), (512, 90), (4000, 1), (4000, 300)])
+def test_small_weights_of_large_values_count(dev, length, new, exponent, t):
+    """One token weighs 2^15 times as much as any other: the others together make up what only their sum shows."""
+    lens = [length, 60]
+    cache, table = filled(lens, 1, 32, 64, 23, dev)
+    at = torch.arange(length, device=dev)
+    set_pairs(cache.k_scales, table, 0, at, 0.0, torch.where(at == 3, 15 * math.log(2) / 8, 0.0))  # scores 8 times that for a q of ones
+    set_pairs(cache.v_scales, table, 0, at, 2.0 ** exponent, -7 * 2.0 ** exponent)
+    q = torch.ones(new + 1, 2, 64, device=dev).to(TYPES[t])
+    start, kv_len = ints([0, new, new + 1], dev), ints(lens, dev)
+    for one in (False, True):
+        out, lse = cache.attention(q, table, start, kv_len, lse=True, one=one)
+        check(out, lse, oracle.attention(q, cache, table, start, kv_len, 64 ** -0.5, parts=2 if t == "f32" else 1, one=one))
+
+
+@pytest.mark.parametrize("new", [1, 150])
+def test_large_values_behind_and_before_ordinary_ones(dev, new):
+    """Values of 2^100 at one end of the keys and small ones at the other: rows that do not see the large ones, and rows whose
+    large ones weigh next to nothing, are as exact as without them."""
+    for first in (False, True):
+        for small in (1.0, 2.0 ** -30):
+            lens = [400, 400]
+            cache, table = filled(lens, 1, 16, 64, 24, dev)
+            at = torch.arange(400, device=dev)
+            for s in (0, 1):
+                big = (at < 64) == first if s == 0 else at >= 330  # sequence 1's last rows see large ones, the others none
+                set_pairs(cache.v_scales, table, s, at, torch.where(big, 2.0 ** 100, small), torch.where(big, -7.4 * 2.0 ** 100, -7.6 * small))
+                if s == 0:  # q is ones: scores of the large ones -160 nats below the others
+                    set_pairs(cache.k_scales, table, s, at, 0.0, torch.where(big, -20.0, 0.0))
+            q = torch.ones(2 * new, 2, 64, device=dev)
+            start, kv_len = ints([0, new, 2 * new], dev), ints(lens, dev)
+            out, lse = cache.attention(q, table, start, kv_len, lse=True)
+            check(out, lse, oracle.attention(q, cache, table, start, kv_len, 64 ** -0.5, parts=2))
