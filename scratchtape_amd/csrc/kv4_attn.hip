@@ -615,7 +615,6 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
         begin = uniform(begin), end = uniform(end);
         const int first_key = uniform(begin + 32 * turn), step = 32 * sharing;
         const int count = uniform(busy && c.pages > 0 && end > first_key ? (end - first_key + step - 1) / step : 0);
-        const bool no_pages = busy && c.pages == 0 && end > begin;
 
         // Pages of the next 32 tiles' halves, a half a lane: -1 one outside the cache, 0 (not looked at) behind the end.
         const int page_rows = alone(c.hkv * c.page), head_row = alone(u.head * c.page), page_mask = alone(c.page - 1), window = alone(a.window);
@@ -960,8 +959,8 @@ __global__ __launch_bounds__(256, (RT == 1 && HD <= 128 ? 3 : 2)) void k_attenti
             total[rt] += st::xor_lane(total[rt], 32, lane);
             low[rt] += st::xor_lane(low[rt], 16, lane);
             low[rt] += st::xor_lane(low[rt], 32, lane);
-            // A row whose own token lies past the table (or that sees a token of a cache without pages).
-            if (pos[rt] >= cap || no_pages) total[rt] = NAN;
+            // A row whose own token lies past the table, or that sees a token of a cache without pages (its own at least).
+            if (pos[rt] >= (c.pages == 0 ? 0 : cap)) total[rt] = NAN;
             if (g == 0) ml[wave][16 * rt + col] = make_float2(ref[rt], total[rt]);
         }
         __syncthreads();  // every ring is read

@@ -141,3 +141,19 @@ def test_large_values_behind_and_before_ordinary_ones(dev, new):
             start, kv_len = ints([0, new, 2 * new], dev), ints(lens, dev)
             out, lse = cache.attention(q, table, start, kv_len, lse=True)
             check(out, lse, oracle.attention(q, cache, table, start, kv_len, 64 ** -0.5, parts=2))
+
+
+# ---- caches without pages, many rows -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("one", [False, True])
+@pytest.mark.parametrize("width", [0, 3])
+def test_rows_that_see_nothing_of_a_cache_without_pages(dev, width, one):
+    """More rows than tokens: those at negative positions see nothing (0, and -inf or 0), the others a token that is nowhere."""
+    cache = KvCache4bit.empty(0, 2, 16, 64, dev)
+    table = torch.zeros(2, width, dtype=torch.int32, device=dev)
+    x = torch.randn(45, 4, 64, device=dev)
+    out, lse = cache.attention(x, table, ints([0, 5, 45], dev), ints([1, 20], dev), lse=True, one=one)
+    nothing = torch.zeros(45, dtype=torch.bool, device=dev)
+    nothing[:4] = nothing[5:25] = True
+    assert not bool(out[nothing].any()) and bool((lse[nothing] == (0 if one else -math.inf)).all())
+    assert bool(out[~nothing].isnan().all()) and bool(lse[~nothing].isnan().all())
