@@ -437,7 +437,7 @@ int64_t st_kv_attention_4bit_bytes(int32_t dtype, int64_t n, int64_t nseq, int64
  * h / (hq / hkv).  Sequence s has rows q_start[s] .. q_start[s + 1] (q_start [nseq
  * + 1], ascending) and kv_len[s] cached tokens, its own rows' among them: the
  * rows are its last tokens.  causal: a row sees the tokens up to its own position
- * (else all kv_len), and the last `window` of those where window > 0.  one:
+ * (else all kv_len), and the last `window` of those where window > 0.  n * hq <= 2^26.  one:
  * softmax1 (a phantom logit 0), as st_softmax.  out [n, hq, hd] in q's type; lse
  * [n, hq] f32 (NULL: not wanted) the log-sum-exp of the scaled scores, the
  * phantom's among them.  A row that sees no token gets 0 and -inf (softmax1: 0);

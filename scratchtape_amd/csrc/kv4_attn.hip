@@ -61,6 +61,7 @@ constexpr int LEAD = 512;
 // keys takes 13.0, 11.2 and 11.2 us, 64 ragged ones 83, 83 and 87, 12 with 5 tokens each 24.7, 24.7 and 40.
 constexpr int WHOLE = 512;
 constexpr int MAX_GROUPS = 1024;  // workgroups of a launch
+constexpr int64_t MAX_ROWS = 1 << 26;  // rows times heads: no more units than that lie on the line, whose prefix sums then fit (load)
 constexpr float BASE = 7.f, MOST_X = 32768.f;  // p aV is set to 2^7 at most, and may grow to 2^15
 // Scales below 2^-86 count as that for the reference, so that p is 2^93 at most when it is set; it may grow until a tile's sum
 // passes 2^101 (2^25 tiles stay within f32).
@@ -180,10 +181,10 @@ struct Line {
         } else {
             tiles = a.per ? (rows + a.per - 1) / a.per : (int)(((int64_t)rows * a.share + a.tile_rows - 1) / a.tile_rows);
             if (tiles > 0) head = part_of(tiles, tiles, rows, len);
-            // Prefix sums in two halves of 20 and more bits.
+            // Prefix sums in two parts: 64 times 25 bits, and the rest of what is 2^26 units of 2^30 keys and a lead at most.
             const int64_t here = head * a.c.hkv;
-            const int lo = st::wave_incl_scan((int)(here & 0xFFFFF)), hi = st::wave_incl_scan((int)(here >> 20));
-            upto = ((int64_t)hi << 20) + lo;
+            const int lo = st::wave_incl_scan((int)(here & 0x1FFFFFF)), hi = st::wave_incl_scan((int)(here >> 25));
+            upto = ((int64_t)(uint32_t)hi << 25) + lo;
         }
         inside = st::lane_value64(upto, 63);
         m.upto[lane] = upto, m.head[lane] = head;
@@ -1102,8 +1103,8 @@ extern "C" st_status st_kv_attention_4bit(const void *q, int32_t dtype, int64_t 
     st::clear_error();
     const char *name = "kv_attention_4bit";
     if (!st::heads_ok(name, hq, hkv, hd)) return ST_ERR_INVALID;
-    if (n < 0 || n > INT32_MAX / hq / 256)
-        return st::fail(ST_ERR_INVALID, "%s: %lld rows of %lld heads (up to 2^23 in all)",
+    if (n < 0 || n > MAX_ROWS / hq)
+        return st::fail(ST_ERR_INVALID, "%s: %lld rows of %lld heads (up to 2^26 in all)",
                         name, (long long)n, (long long)hq);
     if (dtype < ST_F32 || dtype > ST_BF16)
         return st::fail(ST_ERR_INVALID, "%s: dtype %d is none of ST_F32, ST_F16, ST_BF16",

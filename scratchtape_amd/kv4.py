@@ -125,7 +125,7 @@ class KvCache4bit:
                   scale: Optional[float] = None, causal: bool = True, window: int = 0, one: bool = False, lse: bool = False,
                   out: Optional[torch.Tensor] = None, stream=None):
         """softmax(scale q k^T) v for rows q [n, hq, hd] (rotated): sequence s has the rows q_start[s] .. q_start[s + 1]
-        (int32 [sequences + 1]) and kv_len[s] (int32) cached tokens, its own rows' the last of them.  A row sees the tokens
+        (int32 [sequences + 1]) and kv_len[s] (int32) cached tokens, its own rows' the last of them (n * hq up to 2^26).  A row sees the tokens
         up to its own position (causal; else all), the last `window` of those if window > 0.  scale: hd ** -0.5 unless
         given; one: softmax1.  Returns [n, hq, hd] in q's type (`out` if given), with lse also the log-sum-exp of the
         scores, float32 [n, hq].  A row that sees no token gets 0 and -inf (0 with softmax1); one that sees a token on a

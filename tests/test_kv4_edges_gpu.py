@@ -157,3 +157,17 @@ def test_rows_that_see_nothing_of_a_cache_without_pages(dev, width, one):
     nothing[:4] = nothing[5:25] = True
     assert not bool(out[nothing].any()) and bool((lse[nothing] == (0 if one else -math.inf)).all())
     assert bool(out[~nothing].isnan().all()) and bool(lse[~nothing].isnan().all())
+
+
+def test_more_than_2_to_the_23_rows_of_heads(dev):
+    """A batch of prompts whose rows and heads together pass 2^23, as a batch's append takes them."""
+    seqs, length, hq, hd = 70, 2000, 64, 32
+    cache, table = filled([length] * seqs, 1, 64, hd, 27, dev)
+    g = torch.Generator(device=dev).manual_seed(3)
+    q = torch.randn(seqs * length, hq, hd, generator=g, device=dev, dtype=torch.float16)
+    start, kv_len = ints([length * s for s in range(seqs + 1)], dev), ints([length] * seqs, dev)
+    out, lse = cache.attention(q, table, start, kv_len, lse=True, window=100)
+    for s in (0, 33, seqs - 1):  # those sequences alone, some of their heads
+        rows, heads = slice(length * s, length * (s + 1)), slice(0, hq, 21)
+        want = oracle.attention(q[rows, heads].contiguous(), cache, table[s:s + 1], ints([0, length], dev), ints([length], dev), hd ** -0.5, window=100)
+        check(out[rows, heads], lse[rows, heads], want)

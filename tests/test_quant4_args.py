@@ -73,6 +73,13 @@ def test_attention_refusals(kw, msg):
     refused("st_kv_attention_4bit", swap(ATTEND, **kw), msg)
 
 
+def test_attention_takes_2_to_the_26_rows_of_heads():
+    """One more row is refused by its number; as many as that only by what comes after."""
+    refused("st_kv_attention_4bit", swap(ATTEND, n=(1 << 23) + 1), "2^26")
+    refused("st_kv_attention_4bit", swap(ATTEND, n=1 << 62), "2^26")
+    refused("st_kv_attention_4bit", swap(ATTEND, n=1 << 23, out=None), "NULL")
+
+
 def test_nothing_to_do_is_no_error():
     L = _lib.lib()
     assert L.st_kv_append_4bit(*swap(APPEND, n=0, q=None, k=None, v=None)) == _lib.ST_OK
