@@ -392,7 +392,8 @@ st_status st_quantize_4bit(const void *x, int32_t dtype, int64_t n, int64_t k, i
  * st_quantize_4bit writes them (codes 16-byte aligned): the Linear layer
  * x @ w^T of a decoding step.  m <= 2^19, k <= 2^20, n <= 2^28; every 32 rows
  * (f32: 16) read the weights once, so large batches belong in st_matmul over
- * dequantised weights.  out may not overlap x. */
+ * dequantised weights.  out may not overlap x.  Infinities in x and sums past f32's
+ * range give what the sum above gives in f32; such outputs are computed one by one. */
 st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int64_t k, int64_t x_stride,
                          const uint8_t *codes, const float *scales, int64_t group, int64_t n,
                          const float *bias, int32_t relu, void *out, int64_t out_stride,
