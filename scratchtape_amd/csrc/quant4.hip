@@ -448,17 +448,25 @@ extern "C" st_status st_matvec_4bit(const void *x, int32_t dtype, int64_t m, int
         };
         auto pick = [&](auto group_) {
             constexpr int GROUP = decltype(group_)::value;
-            // Rows of weights a workgroup (16 NT): with more of them x is read and summed less often, with fewer there are
-            // workgroups for every CU.  us at NT 1, 2, 4: 32768 x 8192 in groups of 128, one row of bf16: 48.8, 42.3, 38.8;
-            // 11003 x 4096 in groups of 32, 16 rows of f16: 23.9, 22.2, 20.2; 1024 x 256, one row of f32: 4.05 and 10.9 at NT 1
-            // and 4.  f32's three parts leave registers for half as many tiles, and 16 rows of x at a time.
-            constexpr int WIDE = sizeof(T) == 2 ? 4 : 2;
-            if constexpr (sizeof(T) == 2)
-                if (m > 16) return go(k_matvec4<T, GROUP, 2, 2>, 2, 2);
-            if (n >= 8192)
-                go(k_matvec4<T, GROUP, WIDE, 1>, WIDE, 1);
-            else
-                go(k_matvec4<T, GROUP, 1, 1>, 1, 1);
+            // Rows of weights a workgroup (16 NT): with more of them x is read and summed less often, with fewer a workgroup takes
+            // less time.  So the fewest that leave the chip one workgroup a CU at most; where none does, 64 (for two blocks of
+            // x 32, with both in one workgroup; f32's three parts leave registers for 32, and 16 rows of x at a time).  us at NT 1,
+            // 2, 4, then 2 with two blocks, k = 4096 in groups of 128, bf16:
+            //   n =        2048                3000 to 4096         6000 to 8192         11003                16384
+            //   1 row      6.0 7.4 10.8        6.4 7.5 11.0         9.1 7.9 11.2         12.0 12.2 11.4       14.9 12.4 11.8
+            //   16 rows    9.2 10.8 14.2       9.6 10.9 14.3        15.8 11.1 14.5       22.0 18.7 14.7       27.7 18.9 15.2
+            //   32 rows    9.5 10.9 14.3 15.5  15.8 11.1 14.4 15.7  27.4 18.6 14.8 15.8  38.9 26.0 25.4 27.4  50.0 33.0 26.2 27.3
+            // (17 rows at 11003: 29.2 22.7 22.4 20.9.)  f32, groups of 64, 16 rows: 14.5 and 18.6 at 4096, 25.3 and 18.8 at 6000.
+            // Groups of 32 and k = 512 turn at the same n, but for one row of f16 in groups of 32 from 11003 on (14.0 16.1 17.0).
+            const int64_t cus = st::device_cus(), tall = (m + 15) / 16;
+            if ((n + 15) / 16 * tall <= cus) return go(k_matvec4<T, GROUP, 1, 1>, 1, 1);
+            if (sizeof(T) == 4 || (n + 31) / 32 * tall <= cus) return go(k_matvec4<T, GROUP, 2, 1>, 2, 1);
+            if constexpr (sizeof(T) == 2) {
+                if (m > 16)
+                    go(k_matvec4<T, GROUP, 2, 2>, 2, 2);
+                else
+                    go(k_matvec4<T, GROUP, 4, 1>, 4, 1);
+            }
         };
         if (group == 32)
             pick(std::integral_constant<int, 32>());

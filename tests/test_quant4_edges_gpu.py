@@ -72,3 +72,17 @@ def test_a_weight_of_zero_and_an_infinite_row(dev):
     for t in TYPES.values():
         y = quant4.matvec_4bit(x.to(t).to(dev), codes, scales).cpu()
         assert bool(y[0, 1].isnan()) and bool((y[0, [0, 2]] == math.inf).all())
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n", [(1, 4096), (1, 4097), (5, 8192), (16, 8193), (17, 2048), (17, 2049), (32, 4096), (33, 2731), (31, 4097), (70, 300),
+                                 (130, 517)])
+def test_products_around_the_widths_of_tiles(dev, m, n, group, t):
+    """Sizes at which a workgroup takes 16, 32 and 64 rows of weights, and one and two blocks of x: the same sums, held to 64 bits,
+    and for a row to the bits that it has alone."""
+    codes, scales = made(n, 384, group, 0.01, dev)
+    x = torch.randn(m, 384, generator=torch.Generator().manual_seed(n)).to(TYPES[t]).to(dev)
+    got = quant4.matvec_4bit(x, codes, scales)
+    check_product(x, codes, scales, None, False, got)
+    assert torch.equal(quant4.matvec_4bit(x[m // 2:m // 2 + 1], codes, scales)[0], got[m // 2])
