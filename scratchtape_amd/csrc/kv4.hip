@@ -165,10 +165,12 @@ extern "C" st_status st_kv_append_4bit(const void *q, const void *k, const void 
     a.seq = seq, a.pos = pos, a.inv_freq = inv_freq;
     a.k_codes = k_codes, a.v_codes = v_codes, a.k_scales = (float2 *)k_scales, a.v_scales = (float2 *)v_scales;
     const int64_t lanes = hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32;
-    // With tokens enough to fill the chip a workgroup takes a whole token (8191 tokens of 48 vectors of 128: 59 us, 90 with a pass
-    // of 16 vectors each, which take the sines three times); with few, one pass (64 tokens: 5.5 us, 6.4).
+    // With a token for every CU a workgroup takes a whole token, and its sines once; with fewer, one pass of its vectors.  us, whole
+    // and one pass, bf16 of 48 vectors of 128: 64 tokens 7.0 and 6.1, 256 7.8 and 8.0, 512 9.9 and 11.1, 1024 13.1 and 16.8, 8191 64
+    // and 98; f32: 64 9.3 and 7.2, 128 9.7 and 9.4, 256 11.7 and 12.7, 8191 202 and 220; f16 of 21 vectors of 96: 128 6.8 and 6.3,
+    // 256 7.2 and 7.1, 512 8.5 and 9.0; of 20 of 256: 128 7.3 and 7.0, 256 7.7 and 8.3.
     const int64_t vectors = queries + 2 * hkv, once = 256 / lanes;
-    a.stretch = (int32_t)(n >= 1024 ? vectors : once);
+    a.stretch = (int32_t)(n >= st::device_cus() ? vectors : once);
     const int64_t along = std::min<int64_t>(n, 1 << 23);  // (a launch holds less than 2^32 threads along x)
     const dim3 grid((uint32_t)along, (uint32_t)((vectors + a.stretch - 1) / a.stretch), (uint32_t)((n + along - 1) / along));
     return st::with_dtype(dtype, [&](auto *t) -> st_status {

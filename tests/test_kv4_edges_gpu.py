@@ -171,3 +171,25 @@ def test_more_than_2_to_the_23_rows_of_heads(dev):
         rows, heads = slice(length * s, length * (s + 1)), slice(0, hq, 21)
         want = oracle.attention(q[rows, heads].contiguous(), cache, table[s:s + 1], ints([0, length], dev), ints([length], dev), hd ** -0.5, window=100)
         check(out[rows, heads], lse[rows, heads], want)
+
+
+# ---- appends of more and fewer tokens ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("tokens", [255, 256, 257, 600])
+def test_an_append_in_pieces_writes_the_same(dev, tokens, t):
+    """Tokens at once and 100 at a time, whichever way the vectors are dealt out."""
+    hq, heads, hd, page = 10, 5, 128, 16
+    g = torch.Generator(device=dev).manual_seed(tokens)
+    q, k, v = (torch.randn(tokens, h, hd, generator=g, device=dev).to(TYPES[t]) for h in (hq, heads, heads))
+    pages = -(-tokens // page)
+    table = torch.randperm(pages, generator=g, device=dev).to(torch.int32)[None]
+    pos, seq = torch.arange(tokens, dtype=torch.int32, device=dev), torch.zeros(tokens, dtype=torch.int32, device=dev)
+    freq = torch.tensor([10000.0 ** (-i / 32) for i in range(32)], device=dev)
+    caches = [KvCache4bit.empty(pages, heads, page, hd, dev) for _ in range(2)]
+    whole = caches[0].append(q, k, v, seq, pos, table, inv_freq=freq, values=True)
+    parts = [caches[1].append(*(x[i:i + 100] for x in (q, k, v, seq, pos)), table, inv_freq=freq, values=True) for i in range(0, tokens, 100)]
+    for got, pieces in zip(whole, zip(*parts)):
+        assert torch.equal(got, torch.cat(pieces))
+    for (a, _), (b, _) in zip(caches[0]._buffers(), caches[1]._buffers()):
+        assert torch.equal(a, b)
