@@ -61,7 +61,8 @@ struct Eight {
 // lane.  The cosines and sines are taken once a workgroup, in 64 bits; sequence, position and page are the same for all its
 // lanes. 8191 tokens of 48 vectors of 128 in f16, 210 MB: 58 us (3.6 TB/s; 68 with loads behind the page's and the angles' and
 // five waves a SIMD instead of six, for which some registers are put away around the sines; 233 with the angles taken for each
-// component and 64-bit quotients).  Bound by waits for loads.
+// component and 64-bit quotients).  Bound by waits for loads.  In f32, 420 MB, 202 us (2.1 TB/s): 18 registers are put away there, 10 in
+// the 16-bit types.
 template <class T, int LANES>
 __global__ __launch_bounds__(256, 6) void k_append4(const T *__restrict__ q, const T *__restrict__ k,
                                                  const T *__restrict__ v, T *__restrict__ q_out, T *__restrict__ k_out,

@@ -30,9 +30,12 @@
 // through its stretch of the line unit by unit; waves without rows of their own share the unit's keys.  What a workgroup
 // has of a unit that others work on too goes to its slots in `work`, and k_merge4 joins the parts.
 //
-// 32 heads over 8 of 128: 64 sequences of 200 to 8192 keys (311 MB) 75 to 86 us, one of 131072 (151 MB) 47 (3.2 TB/s), 2048
-// rows of a prompt over 8192 keys (240 GFLOP) 530 (450 TFLOP/s).  The first two are the arithmetic of three waves a SIMD (70
-// percent issue) and units' starts, the last that of two (72 percent, the matrix cores busy 23).
+// 32 heads over 8 of 128: 64 sequences of 200 to 8192 keys (311 MB) 76 to 87 us, one of 131072 (151 MB) 46 (3.3 TB/s), 2048
+// rows of a prompt over 8192 keys (240 GFLOP) 507 (470 TFLOP/s).  The first two are the arithmetic of three waves a SIMD (70
+// percent issue) and units' starts, the last that of two (77 percent, the matrix cores busy 24).  Starts are dearer with many
+// sequences, which each workgroup's first wave goes through 64 at a time: the same bytes take 98 us in 256 of them, 121 in 512,
+// 165 in 1024.  Scalar registers do not suffice: 146 to 173 are put away in lanes of vector registers, and about 20 brought
+// back for each tile.
 #include <algorithm>
 #include <cmath>
 
@@ -1151,7 +1154,9 @@ extern "C" st_status st_kv_attention_4bit(const void *q, int32_t dtype, int64_t 
         const uint32_t grid = cut.groups;
         auto with = [&](auto f32, auto f16, auto bf16) { (dtype == ST_F32 ? f32 : dtype == ST_F16 ? f16 : bf16)<<<grid, 256, 0, s>>>(a); };
         // f16 outputs show the rounding of the weights to f16 (1.4 times the error of their own rounding).  Two parts cost few rows
-        // little (64 sequences 88.1 and 88.7 us, one long one 46.6 and 48.1), a prompt 529 and 579: there one does.
+        // little (64 sequences 88.1 and 88.7 us, one long one 46.6 and 48.1), a prompt 529 and 579: there one does.  Which it is
+        // goes by the batch (cut_of), so a single f16 token beside a long prompt may have its weights in one part too.  bf16
+        // outputs are rounded eight times coarser and hardly show it (1.74e-3 to 1.76e-3 off): one part always.
         if (cut.rt == 1)
             with(k_attention4<HD, 2, 2, 1>, k_attention4<HD, 1, 2, 1>, k_attention4<HD, 1, 1, 1>);
         else if constexpr (HD <= 128)

@@ -17,8 +17,7 @@
 
 namespace st {
 
-// Eight consecutive elements as f32.  vec: p is 16-byte aligned (8-byte pairs suffice for no type, so this is asked for
-// as a whole); otherwise element by element.
+// Eight consecutive elements as f32.  vec: p is 16-byte aligned, and they are read 16 bytes at a time; else one by one.
 __device__ __forceinline__ void load8(const float *p, bool vec, float (&x)[8]) {
     if (vec) {
         const float4 a = ((const float4 *)p)[0], b = ((const float4 *)p)[1];

@@ -56,8 +56,8 @@ __global__ __launch_bounds__(256) void k_quantise4(const T *__restrict__ x, int6
 // lanes of the row then read (16 groups at once take 16 registers more at 64 rows of weights, and 19 are put away: 23.5 us where
 // 8 take 18.3, 11003 x 4096 in groups of 32).
 //
-// 32768 x 8192 and one row of bf16: 36 us (4.2 TB/s; the weights' bytes alone would take 23), 11003 x 4096 and 16 rows of f16:
-// 19 (5).  Both wait for the issue of instructions rather than for memory: two waves to a SIMD at most, by their registers.
+// 32768 x 8192 and one row of bf16: 35 us (4.3 TB/s; the weights' bytes alone would take 23), 11003 x 4096 and 16 rows of f16:
+// 18 (5).  Both wait for the issue of instructions rather than for memory: two waves to a SIMD at most, by their registers.
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
