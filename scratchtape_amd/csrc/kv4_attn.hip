@@ -54,14 +54,18 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// Of the line for a workgroup at least: at 128, 256 and 512 one sequence of 128 keys takes 9.7, 10.1 and 10.2 us, 12 with 5
-// tokens each 25.2, 24.3 and 29.4.
+// The three that follow were timed over 20 shapes, of 1 to 512 sequences and 1 to 2048 new tokens; us where it matters.
+//
+// Of the line for a workgroup at least: at 128, 256 and 512 one sequence of 128 keys takes 10.2, 10.5 and 10.5, 12 with 5 tokens
+// each 24.4, 23.2 and 28.0, the others the same to 4 percent.
 constexpr int MIN_STRETCH = 256;
-// What a unit's start costs (finding it, its rows, its first loads, its end), in keys: at 256, 512, 768 and 1024, 64 ragged
-// sequences take 95, 89, 89 and 91 us, 12 with 5 tokens each 24.5, 24.3, 26.3 and 27.9.
+// What a unit's start costs (finding it, its rows, its first loads, its end), in keys: at 256, 512 and 1024, 64 ragged sequences
+// take 92.8, 87.0 and 88.9, 512 of them 138, 121 and 123, 12 with 5 tokens each 23.6, 23.2 and 26.9, 16 tokens of each of 64 213, 190
+// and 201; only prompts alone would have it smaller (300 tokens over 3000 keys 69.4, 76.4 and 75.5).
 constexpr int LEAD = 512;
 // Units of up to so many keys are not shared among workgroups, as a merge would cost more: at 0, 512 and 2048, one sequence of 128
-// keys takes 13.0, 11.2 and 11.2 us, 64 ragged ones 83, 83 and 87, 12 with 5 tokens each 24.7, 24.7 and 40.
+// keys takes 12.2, 10.5 and 10.4, 64 of 400 27.6, 21.2 and 21.3, 64 ragged ones 87.2, 87.0 and 87.9, 12 with 5 tokens each 23.4, 23.2 and
+// 37.1, 6 prompts of 500 tokens 183, 184 and 222.
 constexpr int WHOLE = 512;
 constexpr int MAX_GROUPS = 1024;  // workgroups of a launch
 constexpr int64_t MAX_ROWS = 1 << 26;  // rows times heads: no more units than that lie on the line, whose prefix sums then fit (load)
