@@ -143,6 +143,44 @@ def test_large_values_behind_and_before_ordinary_ones(dev, new):
             check(out, lse, oracle.attention(q, cache, table, start, kv_len, 64 ** -0.5, parts=2))
 
 
+# ---- all of it at once -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("news,kw", [([1, 1], {}), ([150, 40], {}), ([1, 7], dict(one=True, window=900)), ([300, 200], dict(one=True)),
+                                     ([3, 90], dict(window=65))], ids=str)
+@pytest.mark.parametrize("lengths", [[400, 330], [3000, 1500]])
+def test_values_of_all_sizes_at_once(dev, lengths, news, kw, t):
+    """Scales and lowest values from 2^-80 to 2^123 in neighbouring tokens, some vectors zero, some of equal components, in runs and
+    scattered, over scores as far apart as 30."""
+    for seed in range(3):
+        cache, table = filled(lengths, 2, 16, 64, 40 + seed, dev, spread=0.6)
+        g = torch.Generator(device=dev).manual_seed(seed)
+        for s, n in enumerate(lengths):
+            at = torch.arange(n, device=dev)
+            low, high = ((-80, 123), (-80, 0), (-20, 60))[(seed + s) % 3]
+            exponent = torch.randint(low, high, (n,), generator=g, device=dev).float()
+            if seed == 1:
+                exponent = exponent[at // 48 * 48]
+            scale = 2.0 ** exponent.double()
+            kind = torch.randint(0, 4, (n,), generator=g, device=dev)
+            lo = torch.where(kind == 0, scale * 100, -scale * 7.3)
+            scale = torch.where(kind == 1, 0.0, scale)
+            lo = torch.where(kind == 2, 0.0, lo).clamp(-3e38, 3e38)
+            set_pairs(cache.v_scales, table, s, at, scale.float(), lo.float())
+        run(cache, table, lengths, news, 4, TYPES[t], dev, seed=seed, spread=2.0, **kw)
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_values_over_the_whole_range_of_f32(dev, new):
+    """Vectors from -3.3e38 to 3.3e38: their scale times 15 passes f32, their values do not."""
+    lens = [300, 64]
+    cache, table = filled(lens, 1, 16, 64, 44, dev)
+    at = torch.arange(300, device=dev)
+    set_pairs(cache.v_scales, table, 0, at, 6.6e38 / 15, -3.3e38)
+    run(cache, table, lens, [new, 1], 2, torch.float32, dev)
+    run(cache, table, lens, [new, 1], 2, torch.float32, dev, one=True)
+
+
 # ---- caches without pages, many rows -----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("one", [False, True])
