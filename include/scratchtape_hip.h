@@ -457,6 +457,89 @@ st_status st_kv_attention_4bit(const void *q, int32_t dtype, int64_t n, int64_t 
                                int32_t causal, int64_t window, int32_t one, void *out, float *lse,
                                void *work, int64_t work_bytes, st_stream stream);
 
+/* ---- A transformer step in 8 bits -----------------------------------------
+ * No reference counterpart: Linear layers of 8-bit weights on 8-bit rows, from one
+ * token to long prompts, and the norm in front of them, which training uses too.
+ *
+ * The format: a row x (of weights: a scale per channel; of activations: a scale per
+ * token) has a = max |x| and scale = f32(a / 127); value i is held as code =
+ * round_half_even(127 x / a), decided in 64 bits (0 where a = 0), and stands for
+ * scale * code.  A row that holds a NaN or an infinity has scale NaN and codes 0.
+ * Rows of codes may be any number of bytes apart; what makes them also writes
+ * zeros from a row's end to the next multiple of 16 bytes, as far as the stride
+ * leaves room.  Products of rows that are 16-byte aligned (base and stride) are
+ * many times faster than of others; they read whole aligned units of 16 bytes (the
+ * bytes behind a row's end in its last unit count for nothing, whatever they are).
+ * Values that codes stand for are at most the element type's largest number.
+ *
+ * Element types, row strides and alignment are as for the 4-bit calls; none of
+ * these calls uses the scratch arena, and no output may overlap an input or another
+ * output. */
+#define ST_ACT_NONE 0
+#define ST_ACT_RELU 1
+#define ST_ACT_SILU 2
+#define ST_ACT_GELU 3
+
+/* Rows x [n, k] (x_stride elements apart) to codes [n, k] (codes_stride bytes
+ * apart) and scales [n].  values (NULL: not wanted) [n, k] in x's type gets what the
+ * codes stand for, for a straight-through gradient. */
+st_status st_quantize_8bit(const void *x, int32_t dtype, int64_t n, int64_t k, int64_t x_stride,
+                           int8_t *codes, int64_t codes_stride, float *scales, void *values,
+                           st_stream stream);
+
+/* Per row: h = x + residual (NULL: x itself), rounded to x's type; rstd = 1 /
+ * sqrt(mean h^2 + eps); y = h rstd weight.  weight [d] is of x's type or ST_F32.
+ * Outputs, each NULL where it is not wanted, [rows, d] contiguous and of x's type
+ * where no other is named: h; rstd [rows] f32; y; codes and scales [rows] (both or
+ * neither), the 8-bit form of the row h rstd weight, its codes those of h weight
+ * (rstd is a factor of a whole row); values, what the codes stand for.  The sum
+ * of squares is taken in 64 bits. */
+st_status st_rms_norm(const void *x, const void *residual, int32_t dtype, int64_t rows, int64_t d,
+                      int64_t x_stride, int64_t residual_stride, const void *weight,
+                      int32_t weight_dtype, float eps, void *h, float *rstd, void *y, int8_t *codes,
+                      int64_t codes_stride, float *scales, void *values, st_stream stream);
+
+/* Bytes of device memory that st_rms_norm_backward needs on the current device for
+ * these sizes (0: none). */
+int64_t st_rms_norm_backward_bytes(int64_t rows, int64_t d);
+
+/* Gradients of y from dy [rows, d], with h and rstd of the forward pass: dx = dh +
+ * rstd (dy weight - xh mean(dy weight xh)), xh = h rstd, the gradient of x and of
+ * the residual alike; dh (NULL: 0) is the gradient that reaches h by other ways.
+ * dweight [d] f32 = sum over rows of dy xh.  All rows are of type dtype, dx is
+ * contiguous.  Sums are taken in a fixed order.  work: st_rms_norm_backward_bytes of
+ * device memory, 16-byte aligned, the call's own until its work on `stream` is done. */
+st_status st_rms_norm_backward(const void *dy, const void *h, const void *dh, int32_t dtype,
+                               int64_t rows, int64_t d, int64_t dy_stride, int64_t h_stride,
+                               int64_t dh_stride, const float *rstd, const void *weight,
+                               int32_t weight_dtype, void *dx, float *dweight, void *work,
+                               int64_t work_bytes, st_stream stream);
+
+/* Bytes of device memory that st_matmul_8bit (gated 0) or st_gated_8bit (gated 1)
+ * needs on the current device for these sizes (0: none): integer sums of parts of k,
+ * where there are few outputs. */
+int64_t st_matmul_8bit_bytes(int64_t m, int64_t k, int64_t n, int32_t gated);
+
+/* out[i, j] = (sum over l of x[i, l] w[j, l]) x_scales[i] w_scales[j] + bias[j] (f32,
+ * NULL: none), then ReLU where relu != 0: the Linear layer x @ w^T of codes x [m, k]
+ * and w [n, k].  Sums of codes are exact, k <= 131072.  out [m, n] has element type
+ * dtype and is rounded once.  work: st_matmul_8bit_bytes of device memory, 16-byte
+ * aligned, the call's own until its work on `stream` is done. */
+st_status st_matmul_8bit(const int8_t *x, const float *x_scales, int64_t m, int64_t k,
+                         int64_t x_stride, const int8_t *w, const float *w_scales, int64_t n,
+                         int64_t w_stride, const float *bias, int32_t relu, void *out, int32_t dtype,
+                         int64_t out_stride, void *work, int64_t work_bytes, st_stream stream);
+
+/* out[i, j] = act(g[i, j]) u[i, j], where g and u are such products with the first n
+ * and the last n of the rows of w [2n, k] (w_scales and bias [2n]) and act is
+ * ST_ACT_SILU, g / (1 + exp(-g)), or ST_ACT_GELU, g Phi(g): both projections of a
+ * gated feed-forward layer.  The rest is as for st_matmul_8bit. */
+st_status st_gated_8bit(const int8_t *x, const float *x_scales, int64_t m, int64_t k,
+                        int64_t x_stride, const int8_t *w, const float *w_scales, int64_t n,
+                        int64_t w_stride, const float *bias, int32_t activation, void *out,
+                        int32_t dtype, int64_t out_stride, void *work, int64_t work_bytes,
+                        st_stream stream);
+
 /* ---- Device ceilings (benchmark support, no reference counterpart) ------- */
 
 /* The current device's CU count, shader clock and memory clock (kHz) and

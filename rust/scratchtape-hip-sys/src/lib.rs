@@ -41,6 +41,11 @@ pub const ST_NOALLOC_SCRATCH_BYTES: u32 = 64 << 20;
 pub const ST_F32: i32 = 0;
 pub const ST_F16: i32 = 1;
 pub const ST_BF16: i32 = 2;
+/// Activations of the 8-bit products.
+pub const ST_ACT_NONE: i32 = 0;
+pub const ST_ACT_RELU: i32 = 1;
+pub const ST_ACT_SILU: i32 = 2;
+pub const ST_ACT_GELU: i32 = 3;
 
 /// `hipStream_t`; null is the default stream.
 pub type st_stream = *mut c_void;
@@ -508,6 +513,105 @@ extern "C" {
         one: i32,
         out: *mut c_void,
         lse: *mut f32,
+        work: *mut c_void,
+        work_bytes: i64,
+        stream: st_stream,
+    ) -> st_status;
+    // A transformer step in 8 bits (no reference counterpart): the format is described in the header.
+    /// Rows to 8-bit codes with a scale per row.
+    pub fn st_quantize_8bit(
+        x: *const c_void,
+        dtype: i32,
+        n: i64,
+        k: i64,
+        x_stride: i64,
+        codes: *mut i8,
+        codes_stride: i64,
+        scales: *mut f32,
+        values: *mut c_void,
+        stream: st_stream,
+    ) -> st_status;
+    /// Root-mean-square norm with the residual's addition; rows in x's type, in 8 bits, or both.
+    pub fn st_rms_norm(
+        x: *const c_void,
+        residual: *const c_void,
+        dtype: i32,
+        rows: i64,
+        d: i64,
+        x_stride: i64,
+        residual_stride: i64,
+        weight: *const c_void,
+        weight_dtype: i32,
+        eps: f32,
+        h: *mut c_void,
+        rstd: *mut f32,
+        y: *mut c_void,
+        codes: *mut i8,
+        codes_stride: i64,
+        scales: *mut f32,
+        values: *mut c_void,
+        stream: st_stream,
+    ) -> st_status;
+    /// Bytes of `work` that `st_rms_norm_backward` needs.
+    pub fn st_rms_norm_backward_bytes(rows: i64, d: i64) -> i64;
+    /// Gradients of the norm's rows and weight.
+    pub fn st_rms_norm_backward(
+        dy: *const c_void,
+        h: *const c_void,
+        dh: *const c_void,
+        dtype: i32,
+        rows: i64,
+        d: i64,
+        dy_stride: i64,
+        h_stride: i64,
+        dh_stride: i64,
+        rstd: *const f32,
+        weight: *const c_void,
+        weight_dtype: i32,
+        dx: *mut c_void,
+        dweight: *mut f32,
+        work: *mut c_void,
+        work_bytes: i64,
+        stream: st_stream,
+    ) -> st_status;
+    /// Bytes of `work` that `st_matmul_8bit` or `st_gated_8bit` needs.
+    pub fn st_matmul_8bit_bytes(m: i64, k: i64, n: i64, gated: i32) -> i64;
+    /// A Linear layer of 8-bit rows and weights.
+    pub fn st_matmul_8bit(
+        x: *const i8,
+        x_scales: *const f32,
+        m: i64,
+        k: i64,
+        x_stride: i64,
+        w: *const i8,
+        w_scales: *const f32,
+        n: i64,
+        w_stride: i64,
+        bias: *const f32,
+        relu: i32,
+        out: *mut c_void,
+        dtype: i32,
+        out_stride: i64,
+        work: *mut c_void,
+        work_bytes: i64,
+        stream: st_stream,
+    ) -> st_status;
+    /// Both projections of a gated feed-forward layer in 8 bits, the activation and the product.
+    pub fn st_gated_8bit(
+        x: *const i8,
+        x_scales: *const f32,
+        m: i64,
+        k: i64,
+        x_stride: i64,
+        w: *const i8,
+        w_scales: *const f32,
+        n: i64,
+        w_stride: i64,
+        bias: *const f32,
+        activation: i32,
+        out: *mut c_void,
+        dtype: i32,
+        out_stride: i64,
         work: *mut c_void,
         work_bytes: i64,
         stream: st_stream,

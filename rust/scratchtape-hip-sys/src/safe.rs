@@ -1020,6 +1020,290 @@ impl<'a, H: DeviceBuffer + ?Sized> KvCache4bit<'a, H> {
     }
 }
 
+/// An optional buffer's device address, null where it is absent.
+fn opt<T, H: DeviceBuffer + ?Sized>(h: Option<&H>) -> *const T {
+    h.map_or(std::ptr::null(), |b| ptr(b))
+}
+
+fn opt_mut<T, H: DeviceBuffer + ?Sized>(h: Option<&H>) -> *mut T {
+    h.map_or(std::ptr::null_mut(), |b| dptr(b))
+}
+
+/// Rows x [n, k] (`x_stride` elements apart) to 8-bit codes [n, k] (`codes_stride` bytes apart; a multiple of 16
+/// for the products' sake) and scales [n]; `values`, where given, gets what the codes stand for.
+pub fn quantize_8bit<H: DeviceBuffer + ?Sized>(
+    x: &H,
+    dtype: Dtype,
+    n: usize,
+    k: usize,
+    x_stride: usize,
+    codes: &H,
+    codes_stride: usize,
+    scales: &H,
+    values: Option<&H>,
+) {
+    dtype.need(x, span(n, k, x_stride), "quantize_8bit x");
+    need::<i8, H>(codes, mul(n, codes_stride), "quantize_8bit codes");
+    need::<f32, H>(scales, n, "quantize_8bit scales");
+    if let Some(v) = values {
+        dtype.need(v, mul(n, k), "quantize_8bit values");
+    }
+    check(unsafe {
+        sys::st_quantize_8bit(
+            ptr(x),
+            dtype.code(),
+            n as i64,
+            k as i64,
+            x_stride as i64,
+            dptr(codes),
+            codes_stride as i64,
+            dptr(scales),
+            opt_mut(values),
+            stream(),
+        )
+    });
+}
+
+/// What [`rms_norm`] writes, each where it is wanted: h = x + residual, y and values [rows, d] in x's type,
+/// rstd and scales [rows] f32, codes [rows, d] `codes_stride` bytes apart (with scales).
+pub struct RmsOut<'a, H: DeviceBuffer + ?Sized> {
+    pub h: Option<&'a H>,
+    pub rstd: Option<&'a H>,
+    pub y: Option<&'a H>,
+    pub codes: Option<&'a H>,
+    pub codes_stride: usize,
+    pub scales: Option<&'a H>,
+    pub values: Option<&'a H>,
+}
+
+/// The root-mean-square norm of x [rows, d], plus the residual where there is one; the weight [d] is of x's type
+/// or f32.
+pub fn rms_norm<H: DeviceBuffer + ?Sized>(
+    x: &H,
+    residual: Option<&H>,
+    dtype: Dtype,
+    rows: usize,
+    d: usize,
+    x_stride: usize,
+    residual_stride: usize,
+    weight: &H,
+    weight_dtype: Dtype,
+    eps: f32,
+    out: &RmsOut<H>,
+) {
+    dtype.need(x, span(rows, d, x_stride), "rms_norm x");
+    if let Some(r) = residual {
+        dtype.need(r, span(rows, d, residual_stride), "rms_norm residual");
+    }
+    weight_dtype.need(weight, d, "rms_norm weight");
+    for (b, what) in [(out.h, "rms_norm h"), (out.y, "rms_norm y"), (out.values, "rms_norm values")] {
+        if let Some(b) = b {
+            dtype.need(b, mul(rows, d), what);
+        }
+    }
+    for (b, what) in [(out.rstd, "rms_norm rstd"), (out.scales, "rms_norm scales")] {
+        if let Some(b) = b {
+            need::<f32, H>(b, rows, what);
+        }
+    }
+    if let Some(c) = out.codes {
+        need::<i8, H>(c, mul(rows, out.codes_stride), "rms_norm codes");
+    }
+    check(unsafe {
+        sys::st_rms_norm(
+            ptr(x),
+            opt(residual),
+            dtype.code(),
+            rows as i64,
+            d as i64,
+            x_stride as i64,
+            residual_stride as i64,
+            ptr(weight),
+            weight_dtype.code(),
+            eps,
+            opt_mut(out.h),
+            opt_mut(out.rstd),
+            opt_mut(out.y),
+            opt_mut(out.codes),
+            out.codes_stride as i64,
+            opt_mut(out.scales),
+            opt_mut(out.values),
+            stream(),
+        )
+    });
+}
+
+/// Bytes of device memory that [`rms_norm_backward`] needs.
+pub fn rms_norm_backward_bytes(rows: usize, d: usize) -> usize {
+    unsafe { sys::st_rms_norm_backward_bytes(rows as i64, d as i64) as usize }
+}
+
+/// dx [rows, d] and dweight [d] (f32) of the norm from dy and what its forward pass gave (h, rstd); dh, where
+/// given, is added to dx.  `work`: [`rms_norm_backward_bytes`], the call's own until its work is done.
+pub fn rms_norm_backward<H: DeviceBuffer + ?Sized>(
+    dy: &H,
+    h: &H,
+    dh: Option<&H>,
+    dtype: Dtype,
+    rows: usize,
+    d: usize,
+    dy_stride: usize,
+    h_stride: usize,
+    dh_stride: usize,
+    rstd: &H,
+    weight: &H,
+    weight_dtype: Dtype,
+    dx: &H,
+    dweight: &H,
+    work: Option<&H>,
+) {
+    dtype.need(dy, span(rows, d, dy_stride), "rms_norm_backward dy");
+    dtype.need(h, span(rows, d, h_stride), "rms_norm_backward h");
+    if let Some(b) = dh {
+        dtype.need(b, span(rows, d, dh_stride), "rms_norm_backward dh");
+    }
+    need::<f32, H>(rstd, rows, "rms_norm_backward rstd");
+    weight_dtype.need(weight, d, "rms_norm_backward weight");
+    dtype.need(dx, mul(rows, d), "rms_norm_backward dx");
+    need::<f32, H>(dweight, d, "rms_norm_backward dweight");
+    check(unsafe {
+        sys::st_rms_norm_backward(
+            ptr(dy),
+            ptr(h),
+            opt(dh),
+            dtype.code(),
+            rows as i64,
+            d as i64,
+            dy_stride as i64,
+            h_stride as i64,
+            dh_stride as i64,
+            ptr(rstd),
+            ptr(weight),
+            weight_dtype.code(),
+            dptr(dx),
+            dptr(dweight),
+            opt_mut(work),
+            work.map_or(0, |w| w.byte_len() as i64),
+            stream(),
+        )
+    });
+}
+
+/// 8-bit rows: codes [rows, k], rows `stride` bytes apart, and a scale per row.
+pub struct Rows8<'a, H: DeviceBuffer + ?Sized> {
+    pub codes: &'a H,
+    pub stride: usize,
+    pub scales: &'a H,
+}
+
+/// Bytes of device memory that [`matmul_8bit`] (or, `gated`, [`gated_8bit`]) needs.
+pub fn matmul_8bit_bytes(m: usize, k: usize, n: usize, gated: bool) -> usize {
+    unsafe { sys::st_matmul_8bit_bytes(m as i64, k as i64, n as i64, gated as i32) as usize }
+}
+
+fn need_rows8<H: DeviceBuffer + ?Sized>(r: &Rows8<H>, rows: usize, k: usize, what: &str) {
+    need::<i8, H>(r.codes, span(rows, k, r.stride), what);
+    need::<f32, H>(r.scales, rows, what);
+}
+
+/// out [m, n] = x [m, k] @ w [n, k]^T (+ bias [n], then ReLU) of 8-bit rows.  `work`: [`matmul_8bit_bytes`], the
+/// call's own until its work is done.
+pub fn matmul_8bit<H: DeviceBuffer + ?Sized>(
+    x: &Rows8<H>,
+    m: usize,
+    k: usize,
+    w: &Rows8<H>,
+    n: usize,
+    bias: Option<&H>,
+    relu: bool,
+    out: &H,
+    dtype: Dtype,
+    out_stride: usize,
+    work: Option<&H>,
+) {
+    need_rows8(x, m, k, "matmul_8bit x");
+    need_rows8(w, n, k, "matmul_8bit w");
+    if let Some(b) = bias {
+        need::<f32, H>(b, n, "matmul_8bit bias");
+    }
+    dtype.need(out, span(m, n, out_stride), "matmul_8bit out");
+    check(unsafe {
+        sys::st_matmul_8bit(
+            ptr(x.codes),
+            ptr(x.scales),
+            m as i64,
+            k as i64,
+            x.stride as i64,
+            ptr(w.codes),
+            ptr(w.scales),
+            n as i64,
+            w.stride as i64,
+            opt(bias),
+            relu as i32,
+            dptr(out),
+            dtype.code(),
+            out_stride as i64,
+            opt_mut(work),
+            work.map_or(0, |b| b.byte_len() as i64),
+            stream(),
+        )
+    });
+}
+
+/// The activation of [`gated_8bit`].
+#[derive(Clone, Copy)]
+pub enum Gate {
+    Silu,
+    Gelu,
+}
+
+/// out [m, n] = act(x @ gate^T) * (x @ up^T) of 8-bit rows, w [2n, k] holding the gate's rows and then the
+/// other's (bias [2n] likewise).
+pub fn gated_8bit<H: DeviceBuffer + ?Sized>(
+    x: &Rows8<H>,
+    m: usize,
+    k: usize,
+    w: &Rows8<H>,
+    n: usize,
+    bias: Option<&H>,
+    activation: Gate,
+    out: &H,
+    dtype: Dtype,
+    out_stride: usize,
+    work: Option<&H>,
+) {
+    need_rows8(x, m, k, "gated_8bit x");
+    need_rows8(w, mul(n, 2), k, "gated_8bit w");
+    if let Some(b) = bias {
+        need::<f32, H>(b, mul(n, 2), "gated_8bit bias");
+    }
+    dtype.need(out, span(m, n, out_stride), "gated_8bit out");
+    check(unsafe {
+        sys::st_gated_8bit(
+            ptr(x.codes),
+            ptr(x.scales),
+            m as i64,
+            k as i64,
+            x.stride as i64,
+            ptr(w.codes),
+            ptr(w.scales),
+            n as i64,
+            w.stride as i64,
+            opt(bias),
+            match activation {
+                Gate::Silu => sys::ST_ACT_SILU,
+                Gate::Gelu => sys::ST_ACT_GELU,
+            },
+            dptr(out),
+            dtype.code(),
+            out_stride as i64,
+            opt_mut(work),
+            work.map_or(0, |b| b.byte_len() as i64),
+            stream(),
+        )
+    });
+}
+
 /// Waits for the calling thread's stream, then panics if a bounded wait of the grouped f16 kernel (grouped
 /// calls and large single f16 products) gave up since the last check.
 pub fn sync() {

@@ -92,6 +92,13 @@ SIGNATURES = {
     "st_kv_attention_4bit_bytes": [_i32] + 7 * [_i64],
     "st_kv_attention_4bit": [_vp, _i32] + 5 * [_i64] + [_vp, _vp, _i64, _vp, _i64, _i64, _i64] + 4 * [_vp]
     + [_f32, _i32, _i64, _i32, _vp, _vp, _vp, _i64, _vp],
+    "st_quantize_8bit": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp],
+    "st_rms_norm": [_vp, _vp, _i32] + 4 * [_i64] + [_vp, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp],
+    "st_rms_norm_backward_bytes": [_i64, _i64],
+    "st_rms_norm_backward": [_vp, _vp, _vp, _i32] + 5 * [_i64] + [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp],
+    "st_matmul_8bit_bytes": [_i64, _i64, _i64, _i32],
+    "st_matmul_8bit": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _i64, _vp, _i64, _vp],
+    "st_gated_8bit": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _i64, _vp, _i64, _vp],
     "st_device_info": [_vp, _vp, _vp, _vp],
     "st_peak_mfma": [_i32, _i64, _i32, _vp, _vp],
     "st_peak_read": [_vp, _i64, _i32, _vp, _vp],
@@ -103,7 +110,8 @@ SIGNATURES = {
     "st_version": [],
 }
 _RESTYPES = {"st_last_error": ctypes.c_char_p, "st_version": ctypes.c_char_p, "st_f16_enabled": _i32,
-             "st_knn_centroid_digit_bytes": _i64, "st_knn_split_bytes": _i64, "st_kv_attention_4bit_bytes": _i64}
+             "st_knn_centroid_digit_bytes": _i64, "st_knn_split_bytes": _i64, "st_kv_attention_4bit_bytes": _i64,
+             "st_rms_norm_backward_bytes": _i64, "st_matmul_8bit_bytes": _i64}
 
 _lib = None
 

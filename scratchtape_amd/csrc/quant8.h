@@ -1,0 +1,94 @@
+// The 8-bit format of rows of weights and of activations (rms.hip makes it, matmul8.hip multiplies it), and loads and
+// stores of eight neighbouring elements.
+//
+// A row x has a = max |x| and scale = f32(a / 127); value i is held as code = round_half_even(127 x / a), 0 where a = 0,
+// and stands for scale * code.  The quotient is decided in 64 bits, so that a value next to the border of two codes has one
+// answer whatever computes it.  A row that holds a NaN or an infinity has scale NaN and codes 0.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "common.h"
+#include "lanes.h"
+#include "quant4.h"
+
+namespace st {
+
+// Eight elements that need the alignment of one: a 16-byte load may begin at any element.
+template <class T>
+struct Eight {
+    typedef T type __attribute__((ext_vector_type(8), aligned(alignof(T))));
+};
+template <class T>
+using Eight_t = typename Eight<T>::type;
+
+// Elements at .. at + 7 of a row of `width`, 0 past its end.
+template <class T>
+__device__ __forceinline__ Eight_t<T> load_eight(const T *row, int64_t at, int64_t width) {
+    if (at + 8 <= width) return *(const Eight_t<T> *)(row + at);
+    Eight_t<T> v = {};
+    const int left = (int)max((int64_t)0, width - at);
+#pragma unroll
+    for (int i = 0; i < 7; i++)
+        if (i < left) v[i] = row[at + i];
+    return v;
+}
+
+template <class T>
+__device__ __forceinline__ void store_eight(T *row, int64_t at, int64_t width, Eight_t<T> v) {
+    if (at + 8 <= width) {
+        *(Eight_t<T> *)(row + at) = v;
+        return;
+    }
+    const int left = (int)max((int64_t)0, width - at);
+#pragma unroll
+    for (int i = 0; i < 7; i++)
+        if (i < left) row[at + i] = v[i];
+}
+
+// Codes of eight values t of a row with a = max |t| (finite), in 64 bits.
+//
+// f32 does as long as it leaves no doubt: t (127 / a) in f32 is off by no more than four roundings (t, a, 127 / a, the product)
+// of a number up to 127, 4 x 127 x 2^-24 = 3.03e-5, so a quotient more than 3.2e-5 from the middle of two codes has the code
+// that 64 bits give it.  A wave that has one nearer, or an `a` whose quotients could leave f32's normal numbers, divides in 64.
+struct RowCodes {
+    double a;
+    float f;
+    bool plain;
+    __device__ __forceinline__ explicit RowCodes(double a_) : a(a_), f(127.f / (float)a_), plain(a_ > 0x1p-100 && a_ < 0x1p100) {}
+
+    __device__ __forceinline__ uint2 operator()(const double (&t)[8]) const {
+        int c[8];
+        float nearest = 0.5f;  // the least distance from the middle of two codes
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float r = (float)t[i] * f, n = __builtin_rintf(r);
+            nearest = fminf(nearest, 0.5f - __builtin_fabsf(r - n));
+            c[i] = (int)n;
+        }
+        if (!plain || !(nearest > 3.2e-5f)) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) c[i] = a > 0.0 ? (int)__builtin_rint(t[i] * 127.0 / a) : 0;
+        }
+        uint2 out = make_uint2(0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; i++) out.x |= (uint32_t)(c[i] & 255) << (8 * i), out.y |= (uint32_t)(c[4 + i] & 255) << (8 * i);
+        return out;
+    }
+};
+
+// The largest finite number of a type.
+template <class T>
+__device__ constexpr float largest() { return sizeof(T) == 4 ? 0x1.fffffep127f : std::is_same_v<T, _Float16> ? 65504.f : 0x1.fep127f; }
+
+// What code i (0 .. 7) of eight stands for, no larger than T holds: 127 f32(a / 127) can pass an `a` at the end of the range.
+template <class T>
+__device__ __forceinline__ T code_value(uint2 codes, int i, float scale) {
+    const float v = (float)(int8_t)((i < 4 ? codes.x : codes.y) >> (8 * (i & 3))) * scale;
+    return (T)(__builtin_fabsf(v) > largest<T>() ? __builtin_copysignf(largest<T>(), v) : v);
+}
+
+}  // namespace st

@@ -1,13 +1,17 @@
 """Row kernels on MI355X: causal softmax and its backward (gpu_step/rows.rs:101-123),
-LayerNorm forward and backward (gpu_step/rows.rs:60-99)."""
+LayerNorm forward and backward (gpu_step/rows.rs:60-99); the root-mean-square norm with the residual's addition, its 8-bit
+rows and its backward (no reference counterpart)."""
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 from .matmul import _ptr, _stream
+from .quant4 import DTYPES, _addr, _dtype, _launch, _on_gpu, _plain, _rows
+from .quant8 import empty_codes
 
 
 def _check_rows_out(out: torch.Tensor | None, n: int, device, name: str) -> None:
@@ -64,3 +68,91 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, fwd: LnOut, rows: int
     """dx (+)= LayerNorm's input gradient; gamma / beta gradients accumulate into grads at off (rows.rs:90)."""
     _lib.call("st_layer_norm_backward", _ptr(dy), _ptr(x), _ptr(fwd.mean), _ptr(fwd.rstd), rows, d, _ptr(params),
               _ptr(grads), off, _ptr(dx), int(accumulate), models, model_stride, _stream(stream))
+
+
+@dataclass
+class RmsOut:
+    """What rms_norm returns: h, the rows it normed (x + residual, or x itself); rstd [rows] float32; and of y, codes, scales
+    and values what was asked for."""
+    h: torch.Tensor
+    rstd: torch.Tensor
+    y: Optional[torch.Tensor] = None
+    codes: Optional[torch.Tensor] = None
+    scales: Optional[torch.Tensor] = None
+    values: Optional[torch.Tensor] = None
+
+
+def _norm_rows(t: torch.Tensor, like: torch.Tensor, what: str) -> int:
+    """The row stride of a [rows, d] tensor of another's shape and type."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} is a torch tensor")
+    if t.dtype != like.dtype or t.shape != like.shape:
+        raise ValueError(f"{what} is {like.dtype} {list(like.shape)}; got {t.dtype} {list(t.shape)}")
+    return _rows(t, what)
+
+
+def _norm_weight(weight: torch.Tensor, x: torch.Tensor) -> int:
+    if not isinstance(weight, torch.Tensor):
+        raise TypeError("weight is a torch tensor")
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"weight is float32 or of the rows' type, {x.dtype}; got {weight.dtype}")
+    _plain(weight, weight.dtype, (x.shape[1],), "weight")
+    return DTYPES[weight.dtype]
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-5, y: bool = True,
+             eight_bit: bool = False, values: bool = False, stream=None) -> RmsOut:
+    """h = x + residual (x itself without one), rounded to x's type, and its norm h / sqrt(mean h^2 + eps) * weight per row of
+    x [rows, d] (float32, float16 or bfloat16, any row stride); weight [d] is of x's type or float32.
+
+    y: return the norm in x's type.  eight_bit: return it as 8-bit rows for quant8's products, codes and scales, and with
+    `values` also what those stand for in x's type.  The codes are those of the rows h * weight (1 / rms is a factor of a
+    row's scale)."""
+    dtype = _dtype(x, "x")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"x is [rows, d] with d > 0, got {list(x.shape)}")
+    n, d = x.shape
+    stride, w_dtype = _rows(x, "x"), _norm_weight(weight, x)
+    r_stride = 0 if residual is None else _norm_rows(residual, x, "residual")
+    if not eps >= 0:
+        raise ValueError(f"eps is {eps}")
+    if values and not eight_bit:
+        raise ValueError("values are those of 8-bit rows: eight_bit=True")
+    _on_gpu(x, [(weight, "weight"), (residual, "residual")])
+    device = x.device
+    with _launch(device, stream) as handle:
+        rstd = torch.empty((n,), dtype=torch.float32, device=device)
+        h = x if residual is None else torch.empty((n, d), dtype=x.dtype, device=device)
+        out = torch.empty((n, d), dtype=x.dtype, device=device) if y else None
+        codes = scales = stood = None
+        if eight_bit:
+            codes, scales = empty_codes(n, d, device), torch.empty((n,), dtype=torch.float32, device=device)
+            stood = torch.empty((n, d), dtype=x.dtype, device=device) if values else None
+        _lib.call("st_rms_norm", x.data_ptr(), _addr(residual), dtype, n, d, stride, r_stride, weight.data_ptr(), w_dtype, eps,
+                  0 if residual is None else h.data_ptr(), rstd.data_ptr(), _addr(out), _addr(codes), (d + 15) // 16 * 16, _addr(scales),
+                  _addr(stood), handle)
+    return RmsOut(h, rstd, out, codes, scales, stood)
+
+
+def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor, dh: Optional[torch.Tensor] = None,
+                      stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Gradients of rms_norm's y from dy, with h and rstd that it returned: dx [rows, d], the gradient of x and of the residual
+    alike, in the rows' type, and the weight's [d], float32.  dh: the gradient that reaches h by other ways (the residual
+    stream's), added to dx."""
+    dtype = _dtype(h, "h")
+    if h.dim() != 2 or h.shape[1] == 0:
+        raise ValueError(f"h is [rows, d] with d > 0, got {list(h.shape)}")
+    n, d = h.shape
+    stride, w_dtype = _rows(h, "h"), _norm_weight(weight, h)
+    dy_stride, dh_stride = _norm_rows(dy, h, "dy"), 0 if dh is None else _norm_rows(dh, h, "dh")
+    _plain(rstd, torch.float32, (n,), "rstd")
+    _on_gpu(h, [(dy, "dy"), (dh, "dh"), (rstd, "rstd"), (weight, "weight")])
+    device = h.device
+    with _launch(device, stream) as handle:
+        dx = torch.empty((n, d), dtype=h.dtype, device=device)
+        dweight = torch.empty((d,), dtype=torch.float32, device=device)
+        need = _lib.lib().st_rms_norm_backward_bytes(n, d)
+        work = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+        _lib.call("st_rms_norm_backward", dy.data_ptr(), h.data_ptr(), _addr(dh), dtype, n, d, dy_stride, stride, dh_stride, rstd.data_ptr(),
+                  weight.data_ptr(), w_dtype, dx.data_ptr(), dweight.data_ptr(), _addr(work), need, handle)
+    return dx, dweight
