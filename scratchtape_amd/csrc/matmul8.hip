@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "dma_tile.h"
 #include "lanes.h"
 #include "quant4.h"
 
@@ -21,10 +22,24 @@ struct Product {
     int32_t act;  // ST_ACT_NONE, _RELU, or a gated product's _SILU, _GELU
 };
 
-// gate act'd: silu is g / (1 + exp(-g)), gelu g Phi(g) = g / 2 erfc(-g / sqrt 2) (which keeps its digits far below zero).
+// act(g) u.  silu is g / (1 + exp(-g)).  gelu is g Phi(g) = g erfc(-g / sqrt 2) / 2, with erfc(z) = exp(-z^2) t P(t), t = 1 / (1 + z / 2),
+// for z >= 0: P of degree 8 is within 4.4e-8 of erfc for all z up to 14 (a least-squares fit of the relative error; erfc(14) is 0 in
+// f32), and keeps the digits of the tail where 1 + erf would cancel.  About 20 operations; the library's erfcf takes some 100
+// (gated_prompts: 605 us with it, of which a fifth).
 __device__ __forceinline__ float gated(float g, float u, int32_t act) {
-    const float a = act == ST_ACT_SILU ? g / (1.f + __expf(-g)) : 0.5f * g * erfcf(-0.70710678f * g);
-    return a * u;
+    if (act == ST_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * g)) * u;
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35355339f, __builtin_fabsf(g), 1.f));
+    float p = -0.059386503f;
+    p = __builtin_fmaf(p, t, 0.28612414f);
+    p = __builtin_fmaf(p, t, -0.49040672f);
+    p = __builtin_fmaf(p, t, 0.28173363f);
+    p = __builtin_fmaf(p, t, -0.029148735f);
+    p = __builtin_fmaf(p, t, 0.20375259f);
+    p = __builtin_fmaf(p, t, 0.24283510f);
+    p = __builtin_fmaf(p, t, 0.28241211f);
+    p = __builtin_fmaf(p, t, 0.28208434f);
+    const float half = 0.5f * p * (t * __builtin_amdgcn_exp2f(-0.72134752f * g * g));  // Phi(-|g|)
+    return g * (g < 0.f ? half : 1.f - half) * u;
 }
 
 __device__ __forceinline__ float scaled(int32_t sum, float xs, float ws, float bias) { return __builtin_fmaf((float)sum * xs, ws, bias); }
@@ -87,6 +102,349 @@ __global__ __launch_bounds__(256) void k_product8_any(Product a, int64_t tiles_n
     }
 }
 
+// Rows from `p` on as a buffer of `bytes` (up to 4 GB), whose loads give 0 past the end.  It begins 4 KB before p: offsets into it are
+// 4096 and more, as the loads' own offsets count both there and in LDS.
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u4 rows_at(const int8_t *p, int64_t bytes) {
+    const uint64_t base = (uint64_t)p - 4096;
+    return u4{st::lane_value((uint32_t)base, 0), st::lane_value((uint32_t)(base >> 32) & 0xFFFF, 0),
+              st::lane_value((uint32_t)min(bytes + 4096, (int64_t)0xFFFFFFFF), 0), 0x00020000};
+}
+
+// L 16-byte loads a lane (1 KB a wave each), one behind the other in LDS from `to` on: lane l's of load i lands at to + 1024 i + 16 l
+// and comes from offset off[i] + 1024 i + along.
+template <int L>
+__device__ __forceinline__ void dma_rows(u4 rows, const uint32_t *off, uint32_t along, uint32_t to) {
+    static_assert(L == 1 || L == 2, "loads at once");
+    uint32_t saved;
+    if constexpr (L == 2)
+        asm volatile(
+            "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
+            "buffer_load_dwordx4 %1, %4, %5 offen lds\n\t"
+            "buffer_load_dwordx4 %2, %4, %5 offen offset:1024 lds\n\t"
+            "s_mov_b32 m0, %0"
+            : "=&s"(saved) : "v"(off[0]), "v"(off[1]), "s"(to), "s"(rows), "s"(along) : "memory");
+    else
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+                     : "=&s"(saved) : "v"(off[0]), "s"(to), "s"(rows), "s"(along) : "memory");
+}
+
+// A word a lane: lane l's comes from p and lands at to + 4 l.
+__device__ __forceinline__ void dma_words(const void *p, uint32_t to) {
+    uint32_t saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(saved) : "v"(p), "s"(to) : "memory");
+}
+
+// The place of unit `at` among tiles: they go down GROUP rows of tiles, then one to the right, so that neighbours share panels.
+struct Tile {
+    int m, n;
+    __device__ __forceinline__ Tile(uint32_t at, uint32_t tiles_m, uint32_t tiles_n) {
+        constexpr uint32_t GROUP = 8;
+        const uint32_t first = at / (GROUP * tiles_n) * GROUP, high = min(GROUP, tiles_m - first), in = at - first * tiles_n;
+        m = (int)(first + in % high), n = (int)(in / high);
+    }
+};
+
+// Workgroups go to the 8 XCDs in turn: the place of workgroup `id` of `total` where each XCD has a run of neighbours, whose panels its
+// L2 then holds.
+__device__ __forceinline__ uint32_t by_xcd(uint32_t id, uint32_t total) { return id % 8 * (total / 8) + min(id % 8, total % 8) + id / 8; }
+
+struct Units {
+    uint32_t tiles_m, tiles_n, slices, total;  // total = tiles_m tiles_n slices
+    int32_t slice;                             // stages of a slice
+};
+
+template <int BK>
+__device__ __forceinline__ int swizzle(int r) { return BK == 64 ? (r >> 2) & 3 : (r >> 1) & 7; }
+
+constexpr int STAGED = 128 + 16;  // bytes of a staged row of out
+
+template <int BM, int BN, int BK, int NS>
+constexpr int lds_of() { return NS * (BM + BN) * BK + 4 * (32 * STAGED + (BM / 2 + BN) * 4); }
+
+// Tiles of BM rows of x by BN rows of weights, four waves of (BM / 2) x (BN / 2), k in stages of BK bytes that the LDS DMA brings,
+// NS of them in LDS.  Products are 32x32x32 with the weights as the first operand, so that a lane's sums are of one row of x and
+// runs of four columns.  T int32_t: sums of a slice of k, [slices, m, n], for k_join8.
+//
+// LDS: [row][BK / 16 chunks of 16 k]; chunk c of row r is in slot c ^ swizzle(r), so that the 16 rows a quarter of a wave reads
+// are in 16 different groups of four banks.  A wave reads the fragments of the next 32 k while it multiplies these; with a
+// stage's last 32 k in registers its slot is free, so behind the barrier that says so of all waves (and that the next stage has landed)
+// the stage NS further on is on its way into it.
+//
+// A workgroup stays and takes a unit (a tile, or a slice of its k) after another: the stages of all its units are one stream, and the next
+// unit's first are in flight while one's sums are scaled and stored.
+//
+// A gated tile's rows of weights are, 32 by 32 in turn, the gate's and the other half's of the same columns, so that a wave holds both
+// sums of an output.  Rows past the end repeat the last one and are not stored; x's bytes past k are zeros in LDS.
+template <class T, bool GATED, int BM, int BN, int BK, int NS>
+__global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
+    constexpr bool PART = std::is_same_v<T, int32_t>;
+    constexpr int C = BK / 16, PER = 64 / C, LX = BM / (4 * PER), LW = BN / (4 * PER), SX = BM * BK, SW = BN * BK, KS = BK / 32, S = LX < 2 || LW < 2 ? 1 : 2;
+    constexpr int WM = BM / 2, WN = BN / 2, FM = WM / 32, FN = WN / 32, BOTH = GATED ? 2 : 1;
+    constexpr int COLUMNS = BN / BOTH, WCOLS = WN / BOTH;  // of out: a tile's, a wave's
+    constexpr int STORES = WM * WCOLS * (int)sizeof(T) / 1024;  // of a wave and unit
+    static_assert(KS % 2 == 0 && FN % BOTH == 0 && !(PART && GATED), "fragments in pairs");
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+    const uint32_t ring = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)lds;
+    char *const staged = lds + NS * (SX + SW) + wave * 32 * STAGED;
+    float *const table = (float *)(lds + NS * (SX + SW) + 4 * 32 * STAGED) + wave * (WM + 2 * WN);  // xs [WM], ws [WN], bias [WN] of this wave
+    const int all = (int)((a.k + BK - 1) / BK), left = (int)(a.k - (int64_t)(all - 1) * BK);  // stages; bytes of a row in the last one
+    const int64_t whole_k = (a.k + 15) & ~(int64_t)15;  // (rows are read in whole units)
+    const uint32_t first = by_xcd(blockIdx.x, gridDim.x);
+
+    // What is being brought: a unit's stages, from those of the unit `coming` on.
+    uint32_t coming = first;
+    int st_in = 0, end_in = 0;
+    u4 xrows, wrows;
+    uint32_t xo[LX], wo[LW];
+    auto slice_of = [&](uint32_t unit, int &from, int &to) {
+        const int s = (int)(unit % units.slices);
+        from = s * units.slice, to = min(from + units.slice, all);
+    };
+    auto next_unit = [&] {
+        const Tile tile(coming / units.slices, units.tiles_m, units.tiles_n);
+        slice_of(coming, st_in, end_in);
+        const int64_t m0 = (int64_t)tile.m * BM, n0 = (int64_t)tile.n * COLUMNS;
+        xrows = rows_at(a.x + m0 * a.x_stride, (a.m - 1 - m0) * a.x_stride + whole_k);
+        wrows = rows_at(a.w + n0 * a.w_stride, ((GATED ? 2 * a.n : a.n) - 1 - n0) * a.w_stride + whole_k);
+#pragma unroll
+        for (int i = 0; i < LX; i++) {
+            const int p = (wave * LX + i) * 64 + lane, r = p / C, c = (p % C) ^ swizzle<BK>(r);
+            xo[i] = (uint32_t)min((int64_t)r, a.m - 1 - m0) * (uint32_t)a.x_stride + c * 16 + 4096 - 1024 * (i % S);
+        }
+#pragma unroll
+        for (int i = 0; i < LW; i++) {
+            const int p = (wave * LW + i) * 64 + lane, r = p / C, c = (p % C) ^ swizzle<BK>(r);
+            const uint32_t row = GATED ? (uint32_t)min((int64_t)(r / 64 * 32 + r % 32), a.n - 1 - n0) + (r / 32 % 2) * (uint32_t)a.n
+                                       : (uint32_t)min((int64_t)r, a.n - 1 - n0);
+            wo[i] = row * (uint32_t)a.w_stride + c * 16 + 4096 - 1024 * (i % S);
+        }
+    };
+    // Load l, S at once, of the stage that comes next.
+    auto bring = [&](int l, uint32_t to) {
+        if (l < LX / S)
+            dma_rows<S>(xrows, xo + l * S, (uint32_t)st_in * BK, to + (wave * LX + l * S) * 1024);
+        else
+            dma_rows<S>(wrows, wo + (l * S - LX), (uint32_t)st_in * BK, to + SX + (wave * LW + l * S - LX) * 1024);
+    };
+    // The stage after it.  Behind the last unit's last stage that one comes again (and is not used), so that there are always as many
+    // on their way.
+    auto brought = [&] {
+        if (st_in + 1 < end_in) {
+            st_in++;
+        } else if (coming + gridDim.x < units.total) {
+            coming += gridDim.x;
+            next_unit();
+        }
+    };
+
+    int at[KS];  // this lane's bytes of a block of 32 rows, for each 32 k
+#pragma unroll
+    for (int s = 0; s < KS; s++) at[s] = (lane & 31) * BK + (((2 * s + (lane >> 5)) ^ swizzle<BK>(lane & 31)) * 16);
+    // Fragments of a k step, in the order of their use: the weights' first block's, x's, the weights' others.
+    i4 f[2][FN + FM];
+    auto piece = [&](uint32_t slot, int s, int q, i4 *into) {
+        const char *const x = lds + slot + wm * WM * BK + at[s], *const w = lds + slot + SX + wn * WN * BK + at[s];
+        if (q == 0 || q > FM)
+            into[q ? q - FM : 0] = *(const i4 *)(w + (q ? q - FM : 0) * 32 * BK);
+        else
+            into[FN + q - 1] = *(const i4 *)(x + (q - 1) * 32 * BK);
+    };
+    // x's bytes past k, in a row's last stage, which has landed everywhere: zeros.
+    auto end_rows = [&](uint32_t g) {
+        char *const x = lds + g % NS * (SX + SW);
+        for (int u = tid; u < BM * C; u += 256) {
+            const int r = u / C, c = u % C;
+            char *const p = x + r * BK + ((c ^ swizzle<BK>(r)) * 16);
+            if (16 * c >= left)
+                *(i4 *)p = i4{0, 0, 0, 0};
+            else if (16 * c + 16 > left)
+                for (int b = left - 16 * c; b < 16; b++) p[b] = 0;
+        }
+        dma::bar_written();
+    };
+
+    if constexpr (!PART) {
+        if (!a.bias)
+            for (int i = lane; i < WN; i += 64) table[WM + WN + i] = 0.f;
+    }
+    next_unit();
+    for (int i = 0; i < NS; i++) {
+#pragma unroll
+        for (int l = 0; l < (LX + LW) / S; l++) bring(l, ring + i * (SX + SW));
+        brought();
+    }
+    dma::wait_vm<(NS - 1) * (LX + LW)>();
+    dma::bar();
+    {
+        int from, to;
+        slice_of(first, from, to);
+        if (from == all - 1 && left < BK) end_rows(0);
+    }
+#pragma unroll
+    for (int q = 0; q < FN + FM; q++) piece(0, 0, q, f[0]);
+
+    uint32_t g = 0;       // the stage that is multiplied, of this workgroup's
+    int older = 0;        // coming stages that were on their way before the last unit's STORES stores of this wave
+    for (uint32_t unit = first; unit < units.total; unit += gridDim.x) {
+        const Tile tile(unit / units.slices, units.tiles_m, units.tiles_n);
+        const int64_t row0 = (int64_t)tile.m * BM + wm * WM, col0 = (int64_t)tile.n * COLUMNS + wn * WCOLS;  // of this wave
+        int from, to;
+        slice_of(unit, from, to);
+        if constexpr (!PART) {  // the wave's scales and bias, for when the sums are there
+            const uint32_t where = ring + (uint32_t)((char *)table - lds);
+#pragma unroll
+            for (int i = 0; i < (WM + 63) / 64; i++) dma_words(a.xs + min(row0 + min(64 * i + lane, WM - 1), a.m - 1), where + 256 * i);
+#pragma unroll
+            for (int i = 0; i < (WN + 63) / 64; i++) {
+                const int r = min(64 * i + lane, WN - 1);
+                const int64_t row = GATED ? min(col0 + r / 64 * 32 + r % 32, a.n - 1) + (r / 32 % 2) * a.n : min(col0 + r, a.n - 1);
+                dma_words(a.ws + row, where + 4 * WM + 256 * i);
+                if (a.bias) dma_words(a.bias + row, where + 4 * (WM + WN) + 256 * i);
+            }
+        }
+        i16 acc[FN][FM];
+        i4 zero = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < FN; j++)
+#pragma unroll
+            for (int i = 0; i < FM; i++) {  // zeros by products of zeros, 32 cycles for 16 registers (which are as many writes otherwise)
+                asm volatile("" : "+v"(zero));  // (another one each time: the compiler would copy one result)
+                acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(zero, zero, i16{}, 0, 0, 0);
+            }
+        // Every operation of a stage stands between two products: the compiler's own order leaves the matrix cores waiting for the
+        // barrier, the loads' addresses and the fragments in turn (2,060 TOP/s at 8192 x 16384 x 8192 so, 2,270 in this order).
+        for (int st = from; st < to; st++) {
+            constexpr int N = FM * FN, PIECES = FN + FM, LOADS = (LX + LW) / S;
+            const uint32_t slot = g % NS * (SX + SW), next = (g + 1) % NS * (SX + SW);
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    acc[n / FM][n % FM] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[s & 1][n / FM], f[s & 1][FN + n % FM], acc[n / FM][n % FM], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (s < KS - 1) {
+#pragma unroll
+                        for (int q = 0; q < PIECES; q++)
+                            if (n == q * (3 * N / 4) / PIECES) piece(slot, s + 1, q, f[(s + 1) & 1]);
+                    } else {
+                        if (n == 0) {
+                            // The next stage has landed.  (The stages on their way when the last unit's outputs were stored are older
+                            // than those stores, and need not wait for them.)
+                            if (older > 0) {
+                                dma::wait_vm<std::min((NS - 2) * (LX + LW) + STORES, 63)>();
+                                older--;
+                            } else {
+                                dma::wait_vm<(NS - 2) * (LX + LW)>();
+                            }
+                            dma::bar_written();  // (and this one's fragments are read)
+                            if (left < BK) {
+                                int after = st + 1, end;
+                                if (after == to) slice_of(unit + gridDim.x, after, end);
+                                if (after == all - 1) end_rows(g + 1);
+                            }
+                        }
+#pragma unroll
+                        for (int q = 0; q < PIECES; q++)
+                            if (n == std::min(N - 1, 1 + q * (3 * N / 4) / PIECES)) piece(next, 0, q, f[0]);
+#pragma unroll
+                        for (int l = 0; l < LOADS; l++)
+                            if (n == std::min(N - 1, 2 + l * (5 * N / 8) / LOADS)) bring(l, ring + slot);
+                        if (n == std::min(N - 1, N - 4)) brought();
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            g++;
+        }
+
+        // 32 rows of x and 128 bytes of columns at a time: scaled and rounded, through this wave's part of LDS, whole 128-byte runs
+        // of rows to memory.
+        if (!PART && to - from <= NS) dma::wait_vm<0>();  // (else the table is behind stages that have been waited for)
+        asm volatile("" ::: "memory");
+        T *const out = PART ? (T *)a.out + (int64_t)(unit % units.slices) * a.m * a.n : (T *)a.out;
+        const int64_t stride = PART ? a.n : a.out_stride;
+        constexpr int V = 16 / (int)sizeof(T), ACROSS = 128 / (int)sizeof(T), BLOCKS = std::min(ACROSS, WCOLS) / 32;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        typedef float F4 __attribute__((ext_vector_type(4)));
+        typedef T TV __attribute__((ext_vector_type(V)));
+        // A sum out of the matrix cores' registers, when it is wanted (the compiler would move all of them at once, and put others away).
+        auto sum_of = [&](int j, int i, int e) {
+            int32_t v;
+            asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(acc[j][i][e]));
+            return v;
+        };
+        asm volatile("s_nop 15\n\ts_nop 15");  // the last product's results are there
+        typedef T TU __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+        const bool whole = row0 + WM <= a.m && col0 + WCOLS <= a.n;
+        older = whole ? NS - 1 : 0;
+#pragma unroll
+        for (int b = 0; b < WCOLS / 32; b += BLOCKS) {
+            F4 ws[BLOCKS * BOTH][4], bias[BLOCKS * BOTH][4];
+            if constexpr (!PART) {
+#pragma unroll
+                for (int h = 0; h < BLOCKS * BOTH; h++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const int c = (b * BOTH + h) * 32 + 8 * q + 4 * (lane >> 5);
+                        ws[h][q] = *(const F4 *)(table + WM + c), bias[h][q] = *(const F4 *)(table + WM + WN + c);
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < FM; i++) {
+                const float xs = PART ? 0.f : table[i * 32 + (lane & 31)];
+#pragma unroll
+                for (int h = 0; h < BLOCKS; h++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        T4 v;
+                        if constexpr (PART) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) v[e] = sum_of((b + h) * BOTH, i, 4 * q + e);
+                        } else {
+                            F4 y;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                y[e] = scaled(sum_of((b + h) * BOTH, i, 4 * q + e), xs, ws[h * BOTH][q][e], bias[h * BOTH][q][e]);
+                                if constexpr (GATED)
+                                    y[e] = gated(y[e], scaled(sum_of((b + h) * BOTH + 1, i, 4 * q + e), xs, ws[h * BOTH + 1][q][e], bias[h * BOTH + 1][q][e]), a.act);
+                            }
+                            if (!GATED && a.act == ST_ACT_RELU) {
+                                asm volatile("");  // (a branch, not selects)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) y[e] = y[e] < 0.f ? 0.f : y[e];
+                            }
+                            v = __builtin_convertvector(y, T4);
+                        }
+                        *(T4 *)(staged + (lane & 31) * STAGED + (h * 32 + 8 * q + 4 * (lane >> 5)) * (int)sizeof(T)) = v;
+                    }
+                constexpr int LINE = BLOCKS * 32 / V, AT_ONCE = 64 / LINE;  // lanes of a row, rows at once
+                const int c = lane % LINE * V;
+                const uint32_t mine = (uint32_t)(lane / LINE * stride + c) * (uint32_t)sizeof(T);  // (rows of out are less than 2^23 bytes apart)
+                char *o = (char *)(out + (row0 + i * 32) * stride + col0 + b * 32);
+#pragma unroll
+                for (int r0 = 0; r0 < 32; r0 += AT_ONCE, o += AT_ONCE * stride * (int64_t)sizeof(T)) {
+                    const TV v = *(const TV *)(staged + (r0 + lane / LINE) * STAGED + c * (int)sizeof(T));
+                    if (whole) {
+                        *(TU *)(o + mine) = v;
+                    } else if (row0 + i * 32 + r0 + lane / LINE < a.m) {
+                        const int64_t n = a.n - col0 - b * 32 - c;  // columns from here on
+                        if (n >= V) {
+                            *(TU *)(o + mine) = v;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < V; e++)
+                                if (e < n) ((T *)(o + mine))[e] = v[e];
+                        }
+                    }
+                }
+            }
+        }
+    }
+    dma::wait_vm<0>();  // (no stage may land after the workgroup has left its LDS to another)
+}
+
 st_status product8(const char *name, const Product &a, int32_t dtype, bool is_gated, const void *work, int64_t work_bytes, st_stream stream) {
     if (a.m < 0 || a.k <= 0 || a.n < 0 || a.k > 131072)
         return st::fail(ST_ERR_INVALID, "%s: m %lld, k %lld (1 to 131072), n %lld", name, (long long)a.m, (long long)a.k, (long long)a.n);
@@ -108,6 +466,21 @@ st_status product8(const char *name, const Product &a, int32_t dtype, bool is_ga
     const bool vec = (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 && (a.m == 1 || a.x_stride % 16 == 0) && (a.w_stride % 16 == 0 || (a.n == 1 && !is_gated));
     return st::with_dtype(dtype, [&](auto *t) -> st_status {
         using T = std::remove_pointer_t<decltype(t)>;
+        // A tile's offsets are 32 bits: rows of weights up to 256 on, and 2 n in a gated product.
+        if (vec && a.x_stride < 1 << 23 && a.out_stride < 1 << 21 && (a.n + 256) * a.w_stride < ((int64_t)1 << 32) - (1 << 16) && a.m >= 64) {
+            auto go = [&](auto kernel, int bm, int bn, int lds) {
+                Units u;
+                u.tiles_m = (uint32_t)((a.m + bm - 1) / bm), u.tiles_n = (uint32_t)((a.n + bn - 1) / bn), u.slices = 1;
+                u.total = u.tiles_m * u.tiles_n, u.slice = 1 << 30;
+                kernel<<<std::min<uint32_t>(u.total, (uint32_t)st::device_cus()), 256, lds, st::stream_of(stream)>>>(a, u);
+            };
+            if (is_gated)
+                go(k_product8<T, true, 256, 256, 64, 4>, 256, 128, lds_of<256, 256, 64, 4>());
+            else
+                go(k_product8<T, false, 256, 256, 64, 4>, 256, 256, lds_of<256, 256, 64, 4>());
+            ST_LAUNCH_CHECK();
+            return ST_OK;
+        }
         const int64_t tiles_n = (a.n + columns - 1) / columns, tiles = (a.m + 63) / 64 * tiles_n;
         if (is_gated)
             k_product8_any<T, true><<<(uint32_t)tiles, 256, 0, st::stream_of(stream)>>>(a, tiles_n, vec);
