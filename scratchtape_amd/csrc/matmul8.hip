@@ -2,6 +2,7 @@
 // ReLU; and the gated form act(gate) up of two such products.  Sums of codes are exact in 32-bit integers (k <= 131072:
 // 128 x 128 x 131072 = 2^31 is passed by no sum of codes up to 127, and reached only by -128 throughout); the scales enter once, in f32.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -112,21 +113,30 @@ __device__ __forceinline__ u4 rows_at(const int8_t *p, int64_t bytes) {
 }
 
 // L 16-byte loads a lane (1 KB a wave each), one behind the other in LDS from `to` on: lane l's of load i lands at to + 1024 i + 16 l
-// and comes from offset off[i] + 1024 i + along.
-template <int L>
+// and comes from offset off[i] + 1024 i + along.  ONCE: rows that nobody else reads pass by the L2 (nontemporal).
+template <int L, bool ONCE>
 __device__ __forceinline__ void dma_rows(u4 rows, const uint32_t *off, uint32_t along, uint32_t to) {
     static_assert(L == 1 || L == 2, "loads at once");
     uint32_t saved;
-    if constexpr (L == 2)
-        asm volatile(
-            "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
-            "buffer_load_dwordx4 %1, %4, %5 offen lds\n\t"
-            "buffer_load_dwordx4 %2, %4, %5 offen offset:1024 lds\n\t"
-            "s_mov_b32 m0, %0"
-            : "=&s"(saved) : "v"(off[0]), "v"(off[1]), "s"(to), "s"(rows), "s"(along) : "memory");
+#define ST_DMA2(NT)                                                                                                                    \
+    asm volatile(                                                                                                                      \
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"                                                                          \
+        "buffer_load_dwordx4 %1, %4, %5 offen" NT " lds\n\tbuffer_load_dwordx4 %2, %4, %5 offen offset:1024" NT " lds\n\t"            \
+        "s_mov_b32 m0, %0"                                                                                                             \
+        : "=&s"(saved) : "v"(off[0]), "v"(off[1]), "s"(to), "s"(rows), "s"(along) : "memory")
+#define ST_DMA1(NT)                                                                                                                    \
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, %4 offen" NT " lds\n\ts_mov_b32 m0, %0" \
+                 : "=&s"(saved) : "v"(off[0]), "s"(to), "s"(rows), "s"(along) : "memory")
+    if constexpr (L == 2 && ONCE)
+        ST_DMA2(" nt");
+    else if constexpr (L == 2)
+        ST_DMA2("");
+    else if constexpr (ONCE)
+        ST_DMA1(" nt");
     else
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
-                     : "=&s"(saved) : "v"(off[0]), "s"(to), "s"(rows), "s"(along) : "memory");
+        ST_DMA1("");
+#undef ST_DMA2
+#undef ST_DMA1
 }
 
 // A word a lane: lane l's comes from p and lands at to + 4 l.
@@ -146,9 +156,15 @@ struct Tile {
     }
 };
 
-// Workgroups go to the 8 XCDs in turn: the place of workgroup `id` of `total` where each XCD has a run of neighbours, whose panels its
-// L2 then holds.
-__device__ __forceinline__ uint32_t by_xcd(uint32_t id, uint32_t total) { return id % 8 * (total / 8) + min(id % 8, total % 8) + id / 8; }
+// Workgroups go to the 8 XCDs in turn.  Each XCD has a run of the units, whose panels its L2 then holds, and its workgroups take them in
+// turn: the first one's place, the step, and the run's end.
+struct Run {
+    uint32_t first, step, end;
+    __device__ __forceinline__ Run(uint32_t id, uint32_t groups, uint32_t total) {
+        const uint32_t xcd = id % 8, start = xcd * (total / 8) + min(xcd, total % 8);
+        first = start + id / 8, step = (groups - xcd + 7) / 8, end = start + total / 8 + (xcd < total % 8);
+    }
+};
 
 struct Units {
     uint32_t tiles_m, tiles_n, slices, total;  // total = tiles_m tiles_n slices
@@ -156,14 +172,22 @@ struct Units {
 };
 
 template <int BK>
-__device__ __forceinline__ int swizzle(int r) { return BK == 64 ? (r >> 2) & 3 : (r >> 1) & 7; }
+__device__ __forceinline__ int swizzle(int r) { return BK == 64 ? (r >> 2) & 3 : BK == 128 ? (r >> 1) & 7 : r & 15; }
 
 constexpr int STAGED = 128 + 16;  // bytes of a staged row of out
 
-template <int BM, int BN, int BK, int NS>
-constexpr int lds_of() { return NS * (BM + BN) * BK + 4 * (32 * STAGED + (BM / 2 + BN) * 4); }
+// A kernel's tile: rows of x and of weights (four waves, two down and two across), k of a stage, stages in LDS.  ONCE: there is one tile
+// of rows of x, so that the weights are read once.
+template <int BM_, int BN_, int BK_, int NS_, bool ONCE_ = false>
+struct Shape {
+    static constexpr bool ONCE = ONCE_;
+    static constexpr int BM = BM_, BN = BN_, DOWN = 2, ACROSS = 2, BK = BK_, NS = NS_, WM = BM / DOWN, WN = BN / ACROSS;
+    static constexpr int XS = std::max(WM, 64), WS = std::max(WN, 64);  // words of a wave's tables (the DMA brings 64 at once)
+    static constexpr int LDS = NS * (BM + BN) * BK + 4 * (32 * STAGED + (XS + 2 * WS) * 4);
+    static constexpr int AT_ONCE = 160 * 1024 / LDS;  // workgroups of a CU (as LDS goes)
+};
 
-// Tiles of BM rows of x by BN rows of weights, four waves of (BM / 2) x (BN / 2), k in stages of BK bytes that the LDS DMA brings,
+// Tiles of BM rows of x by BN rows of weights, four waves, k in stages of BK bytes that the LDS DMA brings,
 // NS of them in LDS.  Products are 32x32x32 with the weights as the first operand, so that a lane's sums are of one row of x and
 // runs of four columns.  T int32_t: sums of a slice of k, [slices, m, n], for k_join8.
 //
@@ -177,25 +201,26 @@ constexpr int lds_of() { return NS * (BM + BN) * BK + 4 * (32 * STAGED + (BM / 2
 //
 // A gated tile's rows of weights are, 32 by 32 in turn, the gate's and the other half's of the same columns, so that a wave holds both
 // sums of an output.  Rows past the end repeat the last one and are not stored; x's bytes past k are zeros in LDS.
-template <class T, bool GATED, int BM, int BN, int BK, int NS>
-__global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
+template <class T, bool GATED, class Tiles>
+__global__ __launch_bounds__(256, std::min(Tiles::AT_ONCE, 4)) void k_product8(Product a, Units units) {
+    constexpr int BM = Tiles::BM, BN = Tiles::BN, BK = Tiles::BK, NS = Tiles::NS, WM = Tiles::WM, WN = Tiles::WN, XS = Tiles::XS, WS = Tiles::WS;
     constexpr bool PART = std::is_same_v<T, int32_t>;
     constexpr int C = BK / 16, PER = 64 / C, LX = BM / (4 * PER), LW = BN / (4 * PER), SX = BM * BK, SW = BN * BK, KS = BK / 32, S = LX < 2 || LW < 2 ? 1 : 2;
-    constexpr int WM = BM / 2, WN = BN / 2, FM = WM / 32, FN = WN / 32, BOTH = GATED ? 2 : 1;
+    constexpr int FM = WM / 32, FN = WN / 32, BOTH = GATED ? 2 : 1;
     constexpr int COLUMNS = BN / BOTH, WCOLS = WN / BOTH;  // of out: a tile's, a wave's
     constexpr int STORES = WM * WCOLS * (int)sizeof(T) / 1024;  // of a wave and unit
     static_assert(KS % 2 == 0 && FN % BOTH == 0 && !(PART && GATED), "fragments in pairs");
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / Tiles::ACROSS, wn = wave % Tiles::ACROSS;
     const uint32_t ring = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)lds;
     char *const staged = lds + NS * (SX + SW) + wave * 32 * STAGED;
-    float *const table = (float *)(lds + NS * (SX + SW) + 4 * 32 * STAGED) + wave * (WM + 2 * WN);  // xs [WM], ws [WN], bias [WN] of this wave
+    float *const table = (float *)(lds + NS * (SX + SW) + 4 * 32 * STAGED) + wave * (XS + 2 * WS);  // xs, ws and bias of this wave
     const int all = (int)((a.k + BK - 1) / BK), left = (int)(a.k - (int64_t)(all - 1) * BK);  // stages; bytes of a row in the last one
     const int64_t whole_k = (a.k + 15) & ~(int64_t)15;  // (rows are read in whole units)
-    const uint32_t first = by_xcd(blockIdx.x, gridDim.x);
+    const Run run(blockIdx.x, gridDim.x, units.total);
 
     // What is being brought: a unit's stages, from those of the unit `coming` on.
-    uint32_t coming = first;
+    uint32_t coming = run.first;
     int st_in = 0, end_in = 0;
     u4 xrows, wrows;
     uint32_t xo[LX], wo[LW];
@@ -225,17 +250,17 @@ __global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
     // Load l, S at once, of the stage that comes next.
     auto bring = [&](int l, uint32_t to) {
         if (l < LX / S)
-            dma_rows<S>(xrows, xo + l * S, (uint32_t)st_in * BK, to + (wave * LX + l * S) * 1024);
+            dma_rows<S, false>(xrows, xo + l * S, (uint32_t)st_in * BK, to + (wave * LX + l * S) * 1024);
         else
-            dma_rows<S>(wrows, wo + (l * S - LX), (uint32_t)st_in * BK, to + SX + (wave * LW + l * S - LX) * 1024);
+            dma_rows<S, Tiles::ONCE>(wrows, wo + (l * S - LX), (uint32_t)st_in * BK, to + SX + (wave * LW + l * S - LX) * 1024);
     };
     // The stage after it.  Behind the last unit's last stage that one comes again (and is not used), so that there are always as many
     // on their way.
     auto brought = [&] {
         if (st_in + 1 < end_in) {
             st_in++;
-        } else if (coming + gridDim.x < units.total) {
-            coming += gridDim.x;
+        } else if (coming + run.step < run.end) {
+            coming += run.step;
             next_unit();
         }
     };
@@ -268,7 +293,7 @@ __global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
 
     if constexpr (!PART) {
         if (!a.bias)
-            for (int i = lane; i < WN; i += 64) table[WM + WN + i] = 0.f;
+            for (int i = lane; i < WS; i += 64) table[XS + WS + i] = 0.f;
     }
     next_unit();
     for (int i = 0; i < NS; i++) {
@@ -280,7 +305,7 @@ __global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
     dma::bar();
     {
         int from, to;
-        slice_of(first, from, to);
+        slice_of(run.first, from, to);
         if (from == all - 1 && left < BK) end_rows(0);
     }
 #pragma unroll
@@ -288,7 +313,7 @@ __global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
 
     uint32_t g = 0;       // the stage that is multiplied, of this workgroup's
     int older = 0;        // coming stages that were on their way before the last unit's STORES stores of this wave
-    for (uint32_t unit = first; unit < units.total; unit += gridDim.x) {
+    for (uint32_t unit = run.first; unit < run.end; unit += run.step) {
         const Tile tile(unit / units.slices, units.tiles_m, units.tiles_n);
         const int64_t row0 = (int64_t)tile.m * BM + wm * WM, col0 = (int64_t)tile.n * COLUMNS + wn * WCOLS;  // of this wave
         int from, to;
@@ -301,8 +326,8 @@ __global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
             for (int i = 0; i < (WN + 63) / 64; i++) {
                 const int r = min(64 * i + lane, WN - 1);
                 const int64_t row = GATED ? min(col0 + r / 64 * 32 + r % 32, a.n - 1) + (r / 32 % 2) * a.n : min(col0 + r, a.n - 1);
-                dma_words(a.ws + row, where + 4 * WM + 256 * i);
-                if (a.bias) dma_words(a.bias + row, where + 4 * (WM + WN) + 256 * i);
+                dma_words(a.ws + row, where + 4 * XS + 256 * i);
+                if (a.bias) dma_words(a.bias + row, where + 4 * (XS + WS) + 256 * i);
             }
         }
         i16 acc[FN][FM];
@@ -342,7 +367,7 @@ __global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
                             dma::bar_written();  // (and this one's fragments are read)
                             if (left < BK) {
                                 int after = st + 1, end;
-                                if (after == to) slice_of(unit + gridDim.x, after, end);
+                                if (after == to) slice_of(unit + run.step, after, end);
                                 if (after == all - 1) end_rows(g + 1);
                             }
                         }
@@ -352,7 +377,7 @@ __global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
 #pragma unroll
                         for (int l = 0; l < LOADS; l++)
                             if (n == std::min(N - 1, 2 + l * (5 * N / 8) / LOADS)) bring(l, ring + slot);
-                        if (n == std::min(N - 1, N - 4)) brought();
+                        if (n == (N > 4 ? N - 4 : N - 1)) brought();
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -363,9 +388,9 @@ __global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
         // of rows to memory.
         if (!PART && to - from <= NS) dma::wait_vm<0>();  // (else the table is behind stages that have been waited for)
         asm volatile("" ::: "memory");
-        T *const out = PART ? (T *)a.out + (int64_t)(unit % units.slices) * a.m * a.n : (T *)a.out;
+        T *const out = PART ? (T *)a.out + (int64_t)(unit % units.slices) * a.m * a.n : (T *)a.out;  // (slices of sums)
         const int64_t stride = PART ? a.n : a.out_stride;
-        constexpr int V = 16 / (int)sizeof(T), ACROSS = 128 / (int)sizeof(T), BLOCKS = std::min(ACROSS, WCOLS) / 32;
+        constexpr int V = 16 / (int)sizeof(T), BLOCKS = std::min(128 / (int)sizeof(T), WCOLS) / 32;
         typedef T T4 __attribute__((ext_vector_type(4)));
         typedef float F4 __attribute__((ext_vector_type(4)));
         typedef T TV __attribute__((ext_vector_type(V)));
@@ -388,7 +413,7 @@ __global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         const int c = (b * BOTH + h) * 32 + 8 * q + 4 * (lane >> 5);
-                        ws[h][q] = *(const F4 *)(table + WM + c), bias[h][q] = *(const F4 *)(table + WM + WN + c);
+                        ws[h][q] = *(const F4 *)(table + XS + c), bias[h][q] = *(const F4 *)(table + XS + WS + c);
                     }
             }
 #pragma unroll
@@ -445,7 +470,287 @@ __global__ __launch_bounds__(256) void k_product8(Product a, Units units) {
     dma::wait_vm<0>();  // (no stage may land after the workgroup has left its LDS to another)
 }
 
-st_status product8(const char *name, const Product &a, int32_t dtype, bool is_gated, const void *work, int64_t work_bytes, st_stream stream) {
+// A few rows of x, 16 MB of them, by 16 NT rows of weights a workgroup, whose waves share k.  Bound by the weights' bytes: a lane
+// reads 32 of one row (a load is 64 bytes of each of 16 rows, two loads whole lines), straight into the registers that
+// 16x16x64 products take, U steps of 128 k at once; nothing goes through LDS but the waves' sums at the end.  (These products run
+// at half the rate of 32x32x32, which does not show: 5 TB/s of weights keep a SIMD busy one cycle in 13 MB at 16 rows.)
+// A gated product's NT is 2: the gate's rows and the other half's of the same columns.
+template <class T, bool GATED, int MB, int NT, int WAVES, int U>
+__global__ __launch_bounds__(64 * WAVES) void k_few8(Product a) {
+    constexpr int BOTH = GATED ? 2 : 1, COLUMNS = 16 * NT / BOTH, PITCH = 16 * NT + 4;
+    static_assert(!GATED || NT == 2, "both halves");
+    __shared__ __attribute__((aligned(16))) int32_t sums[WAVES][16 * MB][PITCH];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, q = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * COLUMNS, m0 = (int64_t)blockIdx.y * 16 * MB;
+    const int8_t *w[NT], *x[MB];
+#pragma unroll
+    for (int t = 0; t < NT; t++) w[t] = a.w + (GATED ? min(n0 + i, a.n - 1) + t * a.n : min(n0 + 16 * t + i, a.n - 1)) * a.w_stride + 32 * q;
+#pragma unroll
+    for (int b = 0; b < MB; b++) x[b] = a.x + min(m0 + 16 * b + i, a.m - 1) * a.x_stride + 32 * q;
+    i4 acc[NT][MB];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int b = 0; b < MB; b++) acc[t][b] = i4{0, 0, 0, 0};
+    const int full = (int)(a.k / 128);
+    auto steps = [&](int from, auto count_) {  // `from` and every WAVES-th after it
+        constexpr int COUNT = decltype(count_)::value;
+        i4 wf[COUNT][NT][2], xf[COUNT][MB][2];
+#pragma unroll
+        for (int u = 0; u < COUNT; u++) {
+            const int64_t at = (int64_t)(from + u * WAVES) * 128;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) wf[u][t][h] = __builtin_nontemporal_load((const i4 *)(w[t] + at + 16 * h));
+#pragma unroll
+                for (int b = 0; b < MB; b++) xf[u][b][h] = *(const i4 *)(x[b] + at + 16 * h);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < COUNT; u++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int b = 0; b < MB; b++) acc[t][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][t][h], xf[u][b][h], acc[t][b], 0, 0, 0);
+    };
+    int s = wave;
+    for (; s + (U - 1) * WAVES < full; s += U * WAVES) steps(s, std::integral_constant<int, U>());
+    for (; s < full; s += WAVES) steps(s, std::integral_constant<int, 1>());
+    if (s == full && a.k % 128) {  // the part of a step behind the last: x's codes past k are zeros, units past k are not read
+        const int64_t at = (int64_t)full * 128;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int left = (int)(a.k - at) - 32 * q - 16 * h;
+            i4 wf[NT], xf[MB];
+#pragma unroll
+            for (int t = 0; t < NT; t++) wf[t] = left > 0 ? *(const i4 *)(w[t] + at + 16 * h) : i4{0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < MB; b++) {
+                xf[b] = left > 0 ? *(const i4 *)(x[b] + at + 16 * h) : i4{0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int bytes = left - 4 * e;
+                    if (bytes < 4) xf[b][e] = bytes > 0 ? xf[b][e] & ((1 << (8 * bytes)) - 1) : 0;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int b = 0; b < MB; b++) acc[t][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[t], xf[b], acc[t][b], 0, 0, 0);
+        }
+    }
+    // Lane (i, q) holds row i of x with rows 4 q .. 4 q + 3 of the weights.
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int b = 0; b < MB; b++) *(i4 *)&sums[wave][16 * b + i][16 * t + 4 * q] = acc[t][b];
+    __syncthreads();
+    for (int o = tid; o < 16 * MB * COLUMNS; o += 64 * WAVES) {
+        const int b = o / COLUMNS, j = o % COLUMNS;
+        const int64_t mi = m0 + b, ni = n0 + j;
+        if (mi >= a.m || ni >= a.n) continue;
+        int32_t sum = 0, other = 0;
+#pragma unroll
+        for (int v = 0; v < WAVES; v++) {
+            sum += sums[v][b][j];
+            if constexpr (GATED) other += sums[v][b][16 + j];
+        }
+        float y = scaled(sum, a.xs[mi], a.ws[ni], a.bias ? a.bias[ni] : 0.f);
+        if constexpr (GATED)
+            y = gated(y, scaled(other, a.xs[mi], a.ws[a.n + ni], a.bias ? a.bias[a.n + ni] : 0.f), a.act);
+        else if (a.act == ST_ACT_RELU)
+            y = y < 0.f ? 0.f : y;
+        ((T *)a.out)[mi * a.out_stride + ni] = (T)y;
+    }
+}
+
+// One to four rows of x: R rows of weights a wave, each read whole lines at a time (64 lanes by 16 bytes), U times 1024 k at once, and
+// multiplied by four codes an instruction with x in LDS, which the workgroup's waves share; the lanes' sums are added up at the end.
+// Streams of neighbouring lines are what a matrix operand's 64 bytes of 16 rows are not: 32768 x 8192 and one row 51 us with k_few8.
+template <class T, bool GATED, int M, int R, int U>
+__global__ __launch_bounds__(256) void k_one8(Product a) {
+    constexpr int BOTH = GATED ? 2 : 1;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int chunks = (int)((a.k + 1023) / 1024), width = chunks * 1024, k = (int)a.k;
+    for (int u = tid; u < M * (width / 16); u += 256) {
+        const int m = u / (width / 16), at = u % (width / 16) * 16, left = k - at;
+        i4 v = {0, 0, 0, 0};
+        if (left > 0 && m < a.m) v = *(const i4 *)(a.x + m * a.x_stride + at);
+        if (left < 16) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int bytes = left - 4 * e;
+                if (bytes < 4) v[e] = bytes > 0 ? v[e] & ((1 << (8 * bytes)) - 1) : 0;
+            }
+        }
+        *(i4 *)(lds + m * width + at) = v;
+    }
+    __syncthreads();
+    for (int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * R; n0 < a.n; n0 += (int64_t)gridDim.x * 4 * R) {
+        const int8_t *w[R * BOTH];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int h = 0; h < BOTH; h++) w[r * BOTH + h] = a.w + (min(n0 + r, a.n - 1) + h * a.n) * a.w_stride;
+        int32_t acc[R * BOTH][M];
+#pragma unroll
+        for (int r = 0; r < R * BOTH; r++)
+#pragma unroll
+            for (int m = 0; m < M; m++) acc[r][m] = 0;
+        auto some = [&](int chunk, auto count_) {
+            constexpr int COUNT = decltype(count_)::value;
+            i4 v[COUNT][R * BOTH];
+#pragma unroll
+            for (int u = 0; u < COUNT; u++) {
+                const int at = (chunk + u) * 1024 + lane * 16, from = at < k ? at : 0;  // (x is 0 past k)
+#pragma unroll
+                for (int r = 0; r < R * BOTH; r++) v[u][r] = __builtin_nontemporal_load((const i4 *)(w[r] + from));
+            }
+#pragma unroll
+            for (int u = 0; u < COUNT; u++)
+#pragma unroll
+                for (int m = 0; m < M; m++) {
+                    const i4 x = *(const i4 *)(lds + m * width + (chunk + u) * 1024 + lane * 16);
+#pragma unroll
+                    for (int r = 0; r < R * BOTH; r++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[r][m] = __builtin_amdgcn_sdot4(v[u][r][e], x[e], acc[r][m], false);
+                }
+        };
+        int c = 0;
+        for (; c + U <= chunks; c += U) some(c, std::integral_constant<int, U>());
+        for (; c < chunks; c++) some(c, std::integral_constant<int, 1>());
+        int32_t mine[BOTH] = {};
+#pragma unroll
+        for (int r = 0; r < R * BOTH; r++)
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+                int32_t v = acc[r][m];  // (step by step: a loop of six here stays a loop, 1 us a row of x)
+                v += st::xor_lane(v, 32, lane), v += st::xor_lane(v, 16, lane), v += st::xor_lane(v, 8, lane);
+                v += st::xor_lane(v, 4, lane), v += st::xor_lane(v, 2, lane), v += st::xor_lane(v, 1, lane);
+                if (lane == r / BOTH * M + m) mine[r % BOTH] = v;
+            }
+        const int64_t m = lane % M, n = n0 + lane / M;
+        if (lane >= R * M || m >= a.m || n >= a.n) continue;
+        float y = scaled(mine[0], a.xs[m], a.ws[n], a.bias ? a.bias[n] : 0.f);
+        if constexpr (GATED)
+            y = gated(y, scaled(mine[BOTH - 1], a.xs[m], a.ws[a.n + n], a.bias ? a.bias[a.n + n] : 0.f), a.act);
+        else if (a.act == ST_ACT_RELU)
+            y = y < 0.f ? 0.f : y;
+        ((T *)a.out)[m * a.out_stride + n] = (T)y;
+    }
+}
+
+// out from the sums of slices of k, four columns a thread.  A gated product's sums are [slices, m, 2 n].
+template <class T, bool GATED>
+__global__ __launch_bounds__(256) void k_join8(Product a, const int32_t *__restrict__ part, int32_t slices) {
+    typedef int32_t I4 __attribute__((ext_vector_type(4), aligned(4)));
+    const int64_t per = (a.n + 3) / 4, at = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+    if (at >= a.m * per) return;
+    const int64_t m = at / per, n = at % per * 4, width = GATED ? 2 * a.n : a.n;
+    int32_t sum[2][4] = {};
+    auto add = [&](const int32_t *p, int32_t (&s)[4]) {
+        if (n + 4 <= a.n) {
+            const I4 v = *(const I4 *)p;
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] += v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+                if (n + e < a.n) s[e] += p[e];
+        }
+    };
+#pragma unroll 4
+    for (int i = 0; i < slices; i++) {
+        const int32_t *const p = part + ((int64_t)i * a.m + m) * width + n;
+        add(p, sum[0]);
+        if constexpr (GATED) add(p + a.n, sum[1]);
+    }
+    const float xs = a.xs[m];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (n + e >= a.n) continue;
+        float y = scaled(sum[0][e], xs, a.ws[n + e], a.bias ? a.bias[n + e] : 0.f);
+        if constexpr (GATED)
+            y = gated(y, scaled(sum[1][e], xs, a.ws[a.n + n + e], a.bias ? a.bias[a.n + n + e] : 0.f), a.act);
+        else if (a.act == ST_ACT_RELU)
+            y = y < 0.f ? 0.f : y;
+        ((T *)a.out)[m * a.out_stride + n + e] = (T)y;
+    }
+}
+
+typedef Shape<256, 256, 64, 4> Large;
+typedef Shape<128, 128, 64, 3> Middle;
+typedef Shape<64, 128, 64, 4> Low;
+typedef Shape<64, 64, 128, 3> Small;
+typedef Shape<64, 64, 256, 4, true> Deep;
+typedef Shape<64, 128, 128, 5, true> DeepLow;
+
+enum Kernel { ONE, FEW, LARGE, MIDDLE, LOW, SMALL, DEEP, DEEP_LOW };
+
+template <class F>
+st_status with_shape(int kernel, F &&f) {
+    switch (kernel) {
+        case LARGE: return f(Large());
+        case MIDDLE: return f(Middle());
+        case LOW: return f(Low());
+        case SMALL: return f(Small());
+        case DEEP: return f(Deep());
+        default: return f(DeepLow());
+    }
+}
+
+struct Plan {
+    int kernel, slices;
+};
+
+// Which kernel: the one whose time, in us, comes out least.  A workgroup takes `start`, and `unit` for each unit beside its stages, of
+// which one takes `alone`, or `shared` where two workgroups of a CU run at once; or its bytes come at `rate` (MB a us) and take longer; slices cost
+// their join, `join` and `each` of them, and the memory of their sums.  Fitted to both sides' times at 400 shapes, 17 to 96 % of them where a kernel is
+// not the fastest; the choice costs 1.1 % over the fastest on average (most: 384 x 4096 x 11003, 45 us instead of 34, a tile and a half
+// a CU).
+struct Rates {
+    int kernel, bm, bn, bk, shared_by;
+    double start, unit, alone, shared, rate, join, each;
+};
+constexpr Rates RATES[] = {
+    {LARGE, 256, 256, 64, 1, 1.25, 13.5, 0.669, 0.669, 2.26, 0, 0}, {MIDDLE, 128, 128, 64, 2, 4.37, 2.98, 0.307, 0.664, 3.62, 0, 0},
+    {LOW, 64, 128, 64, 2, 3.13, 2.75, 0.264, 0.494, 8.4, 0, 0},    {SMALL, 64, 64, 128, 2, 3.95, 1.78, 0.307, 0.455, 3.44, 2.21, 0.446},
+    {DEEP, 64, 64, 256, 1, 5.23, 1.48, 0.51, 0.51, 5.58, 2.22, 0.263}, {DEEP_LOW, 64, 128, 128, 1, 3.13, 3.58, 0.427, 0.427, 4.41, 0, 0},
+};
+
+Plan plan_of(int64_t m, int64_t k, int64_t n, bool is_gated) {
+    const int64_t width = is_gated ? 2 * n : n, cus = st::device_cus();
+    if (m <= 4 && k >= 512 && (m == 1 ? 1 : m == 2 ? 2 : 4) * k <= 64 * 1024) return Plan{ONE, 1};
+    Plan best = {LARGE, 1};
+    double least = 1e300;
+    for (const Rates &r : RATES) {
+        const bool once = r.kernel == DEEP || r.kernel == DEEP_LOW, narrow = r.kernel == SMALL || r.kernel == DEEP, halves = r.kernel == LOW || r.kernel == DEEP_LOW;
+        if (once != (m <= 64) || (halves && !is_gated)) continue;
+        const int64_t stages = (k + r.bk - 1) / r.bk, tiles = (m + r.bm - 1) / r.bm * ((width + r.bn - 1) / r.bn);
+        for (const int slices : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            if (slices > 1 && (!narrow || slices > stages / 2 || tiles * slices > 5 * cus)) break;
+            if (slices == 1 && narrow && is_gated) continue;
+            const int64_t per = (tiles * slices + cus - 1) / cus, full = per / r.shared_by, rest = per % r.shared_by, of = (stages + slices - 1) / slices;
+            double t = r.start + (double)full * (r.unit + (double)of * r.shared) + (rest ? r.unit + (double)of * r.alone : 0);
+            t = std::max(t, r.start + ((double)m + (double)width) * (double)k / (1e6 * r.rate));
+            if (slices > 1) t += r.join + r.each * slices + (double)m * (double)width * 4 * (slices + 1) / 4e6;
+            if (t < least) least = t, best = Plan{r.kernel, slices};
+        }
+    }
+    if (m <= 32) {
+        const double blocks = (double)((width + 15) / 16), at_once = 8.0 * (double)cus / (is_gated ? 2 : 1);
+        const double t = 4.61 + 0.134e-6 * (double)width * (double)k * (1 + 0.613 * (double)m / 16) + 0.69 * std::ceil(blocks / at_once) * (double)k / 1024;
+        if (t < least) best = Plan{FEW, 1};
+    }
+    return best;
+}
+
+st_status product8(const char *name, const Product &a, int32_t dtype, bool is_gated, void *work, int64_t work_bytes, st_stream stream) {
     if (a.m < 0 || a.k <= 0 || a.n < 0 || a.k > 131072)
         return st::fail(ST_ERR_INVALID, "%s: m %lld, k %lld (1 to 131072), n %lld", name, (long long)a.m, (long long)a.k, (long long)a.n);
     const int64_t columns = is_gated ? 32 : 64;
@@ -464,22 +769,98 @@ st_status product8(const char *name, const Product &a, int32_t dtype, bool is_ga
         return st::fail(ST_ERR_INVALID, "%s: a buffer is not aligned to its elements (work: 16 bytes)", name);
     if (!st::device_ok()) return ST_ERR_NO_DEVICE;
     const bool vec = (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 && (a.m == 1 || a.x_stride % 16 == 0) && (a.w_stride % 16 == 0 || (a.n == 1 && !is_gated));
+    const Plan plan = plan_of(a.m, a.k, a.n, is_gated);
     return st::with_dtype(dtype, [&](auto *t) -> st_status {
         using T = std::remove_pointer_t<decltype(t)>;
-        // A tile's offsets are 32 bits: rows of weights up to 256 on, and 2 n in a gated product.
-        if (vec && a.x_stride < 1 << 23 && a.out_stride < 1 << 21 && (a.n + 256) * a.w_stride < ((int64_t)1 << 32) - (1 << 16) && a.m >= 64) {
-            auto go = [&](auto kernel, int bm, int bn, int lds) {
-                Units u;
-                u.tiles_m = (uint32_t)((a.m + bm - 1) / bm), u.tiles_n = (uint32_t)((a.n + bn - 1) / bn), u.slices = 1;
-                u.total = u.tiles_m * u.tiles_n, u.slice = 1 << 30;
-                kernel<<<std::min<uint32_t>(u.total, (uint32_t)st::device_cus()), 256, lds, st::stream_of(stream)>>>(a, u);
+        typedef std::integral_constant<int, 1> I1;
+        typedef std::integral_constant<int, 2> I2;
+        typedef std::integral_constant<int, 4> I4;
+        typedef std::integral_constant<int, 8> I8;
+        if (vec && plan.kernel == ONE) {
+            const int rows = a.m == 1 ? 1 : a.m == 2 ? 2 : 4, lds = rows * (int)((a.k + 1023) / 1024 * 1024);
+            auto go = [&](auto m_, auto r_, auto u_) {
+                constexpr int M = decltype(m_)::value, R = decltype(r_)::value, U = decltype(u_)::value;
+                const int64_t most = (int64_t)st::device_cus() * (M == 1 ? 64 : std::min(8, 160 * 1024 / lds));
+                const uint32_t groups = (uint32_t)std::min<int64_t>((a.n + 4 * R - 1) / (4 * R), most);
+                if (is_gated)
+                    k_one8<T, true, M, R, U><<<groups, 256, lds, st::stream_of(stream)>>>(a);
+                else
+                    k_one8<T, false, M, R, U><<<groups, 256, lds, st::stream_of(stream)>>>(a);
             };
-            if (is_gated)
-                go(k_product8<T, true, 256, 256, 64, 4>, 256, 128, lds_of<256, 256, 64, 4>());
+            // Rows of weights at once: two, for x's share of the LDS reads; one where there are few rows for all waves, and of long rows for
+            // one row of x (us with one and two: 32768 x 8192 40.2 and 42, 1024 x 16384 7.2 and 8; 11003 x 4096 10.9 and 10.6).
+            auto rows_of = [&](auto m_) {
+                if (a.n <= 2048 || (a.m == 1 && a.k >= 8192))
+                    go(m_, I1(), I8());
+                else
+                    go(m_, I2(), I4());
+            };
+            if (rows == 1)
+                rows_of(I1());
+            else if (rows == 2)
+                rows_of(I2());
             else
-                go(k_product8<T, false, 256, 256, 64, 4>, 256, 256, lds_of<256, 256, 64, 4>());
+                rows_of(I4());
             ST_LAUNCH_CHECK();
             return ST_OK;
+        }
+        if (vec && plan.kernel == FEW) {
+            auto go = [&](auto kernel, int mb, int waves) {
+                kernel<<<dim3((uint32_t)((a.n + 15) / 16), (uint32_t)((a.m + 16 * mb - 1) / (16 * mb))), 64 * waves, 0, st::stream_of(stream)>>>(a);
+            };
+            if (a.m <= 16 && is_gated)
+                go(k_few8<T, true, 1, 2, 4, 1>, 1, 4);
+            else if (a.m <= 16)
+                go(k_few8<T, false, 1, 1, 8, 4>, 1, 8);
+            else if (is_gated)
+                go(k_few8<T, true, 2, 2, 4, 1>, 2, 4);
+            else
+                go(k_few8<T, false, 2, 1, 8, 2>, 2, 8);
+            ST_LAUNCH_CHECK();
+            return ST_OK;
+        }
+        // A tile's offsets are 32 bits: rows of weights up to 256 on, and 2 n in a gated product.
+        const bool near = a.x_stride < 1 << 23 && a.out_stride < 1 << 21 && (a.n + 256) * a.w_stride < ((int64_t)1 << 32) - (1 << 16);
+        if (vec && near && plan.kernel >= LARGE) {
+            const int64_t width = is_gated ? 2 * a.n : a.n, need = plan.slices > 1 ? 4 * plan.slices * a.m * width : 0;
+            if (need && (!work || work_bytes < need))
+                return st::fail(ST_ERR_INVALID, "%s: %lld bytes of work memory are needed, got %lld", name, (long long)need, (long long)(work ? work_bytes : 0));
+            const st_status status = with_shape(plan.kernel, [&](auto shape) -> st_status {
+                using Tiles = decltype(shape);
+                constexpr bool SLICED = std::is_same_v<Tiles, Small> || std::is_same_v<Tiles, Deep>, NARROW = SLICED;  // (a wave's columns are 32)
+                constexpr bool HALVES = std::is_same_v<Tiles, Low> || std::is_same_v<Tiles, DeepLow>;
+                auto go = [&](auto kernel, const Product &p, int bn) {
+                    Units u;
+                    const int64_t stages = (p.k + Tiles::BK - 1) / Tiles::BK;
+                    u.slice = (int32_t)((stages + plan.slices - 1) / plan.slices), u.slices = (uint32_t)((stages + u.slice - 1) / u.slice);
+                    u.tiles_m = (uint32_t)((p.m + Tiles::BM - 1) / Tiles::BM), u.tiles_n = (uint32_t)((p.n + bn - 1) / bn);
+                    u.total = u.tiles_m * u.tiles_n * u.slices;
+                    const uint32_t most = (uint32_t)(st::device_cus() * std::min(Tiles::AT_ONCE, 4));
+                    kernel<<<std::min(u.total, most), 256, Tiles::LDS, st::stream_of(stream)>>>(p, u);
+                    return (int32_t)u.slices;
+                };
+                if (plan.slices > 1) {
+                    if constexpr (SLICED) {
+                        Product p = a;
+                        p.n = width, p.out = work;
+                        const int32_t slices = go(k_product8<int32_t, false, Tiles>, p, Tiles::BN);
+                        ST_LAUNCH_CHECK();
+                        const int64_t blocks = (a.m * ((a.n + 3) / 4) + 255) / 256, along = std::min<int64_t>(blocks, 1 << 23);
+                        const dim3 grid((uint32_t)along, (uint32_t)((blocks + along - 1) / along));
+                        if (is_gated)
+                            k_join8<T, true><<<grid, 256, 0, st::stream_of(stream)>>>(a, (const int32_t *)work, slices);
+                        else
+                            k_join8<T, false><<<grid, 256, 0, st::stream_of(stream)>>>(a, (const int32_t *)work, slices);
+                    }
+                } else if (is_gated) {
+                    if constexpr (!NARROW) go(k_product8<T, true, Tiles>, a, Tiles::BN / 2);
+                } else {
+                    if constexpr (!HALVES) go(k_product8<T, false, Tiles>, a, Tiles::BN);
+                }
+                ST_LAUNCH_CHECK();
+                return ST_OK;
+            });
+            return status;
         }
         const int64_t tiles_n = (a.n + columns - 1) / columns, tiles = (a.m + 63) / 64 * tiles_n;
         if (is_gated)
@@ -493,7 +874,11 @@ st_status product8(const char *name, const Product &a, int32_t dtype, bool is_ga
 
 }  // namespace
 
-extern "C" int64_t st_matmul_8bit_bytes(int64_t m, int64_t k, int64_t n, int32_t is_gated) { return 0; }
+extern "C" int64_t st_matmul_8bit_bytes(int64_t m, int64_t k, int64_t n, int32_t is_gated) {
+    if (m <= 0 || k <= 0 || n <= 0) return 0;
+    const Plan plan = plan_of(m, k, n, is_gated != 0);
+    return plan.slices > 1 ? 4 * plan.slices * m * (is_gated ? 2 * n : n) : 0;
+}
 
 extern "C" st_status st_matmul_8bit(const int8_t *x, const float *x_scales, int64_t m, int64_t k, int64_t x_stride, const int8_t *w,
                                     const float *w_scales, int64_t n, int64_t w_stride, const float *bias, int32_t relu, void *out, int32_t dtype,
