@@ -501,7 +501,7 @@ st_status st_rms_norm(const void *x, const void *residual, int32_t dtype, int64_
 
 /* Bytes of device memory that st_rms_norm_backward needs on the current device for
  * these sizes (0: none). */
-int64_t st_rms_norm_backward_bytes(int64_t rows, int64_t d);
+int64_t st_rms_norm_backward_bytes(int64_t rows, int64_t d, int32_t dtype);
 
 /* Gradients of y from dy [rows, d], with h and rstd of the forward pass: dx = dh +
  * rstd (dy weight - xh mean(dy weight xh)), xh = h rstd, the gradient of x and of

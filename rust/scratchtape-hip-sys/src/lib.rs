@@ -553,7 +553,7 @@ extern "C" {
         stream: st_stream,
     ) -> st_status;
     /// Bytes of `work` that `st_rms_norm_backward` needs.
-    pub fn st_rms_norm_backward_bytes(rows: i64, d: i64) -> i64;
+    pub fn st_rms_norm_backward_bytes(rows: i64, d: i64, dtype: i32) -> i64;
     /// Gradients of the norm's rows and weight.
     pub fn st_rms_norm_backward(
         dy: *const c_void,

@@ -1134,8 +1134,8 @@ pub fn rms_norm<H: DeviceBuffer + ?Sized>(
 }
 
 /// Bytes of device memory that [`rms_norm_backward`] needs.
-pub fn rms_norm_backward_bytes(rows: usize, d: usize) -> usize {
-    unsafe { sys::st_rms_norm_backward_bytes(rows as i64, d as i64) as usize }
+pub fn rms_norm_backward_bytes(rows: usize, d: usize, dtype: Dtype) -> usize {
+    unsafe { sys::st_rms_norm_backward_bytes(rows as i64, d as i64, dtype.code()) as usize }
 }
 
 /// dx [rows, d] and dweight [d] (f32) of the norm from dy and what its forward pass gave (h, rstd); dh, where

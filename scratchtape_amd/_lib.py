@@ -94,7 +94,7 @@ SIGNATURES = {
     + [_f32, _i32, _i64, _i32, _vp, _vp, _vp, _i64, _vp],
     "st_quantize_8bit": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp],
     "st_rms_norm": [_vp, _vp, _i32] + 4 * [_i64] + [_vp, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp],
-    "st_rms_norm_backward_bytes": [_i64, _i64],
+    "st_rms_norm_backward_bytes": [_i64, _i64, _i32],
     "st_rms_norm_backward": [_vp, _vp, _vp, _i32] + 5 * [_i64] + [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp],
     "st_matmul_8bit_bytes": [_i64, _i64, _i64, _i32],
     "st_matmul_8bit": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _i64, _vp, _i64, _vp],

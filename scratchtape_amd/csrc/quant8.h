@@ -62,16 +62,18 @@ struct RowCodes {
 
     __device__ __forceinline__ uint2 operator()(const double (&t)[8]) const {
         int c[8];
-        float nearest = 0.5f;  // the least distance from the middle of two codes
+        float off[8], nearest = 0.5f;  // the distances from the middle of two codes, the least of them
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const float r = (float)t[i] * f, n = __builtin_rintf(r);
-            nearest = fminf(nearest, 0.5f - __builtin_fabsf(r - n));
+            off[i] = 0.5f - __builtin_fabsf(r - n);
+            nearest = fminf(nearest, off[i]);
             c[i] = (int)n;
         }
         if (!plain || !(nearest > 3.2e-5f)) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) c[i] = a > 0.0 ? (int)__builtin_rint(t[i] * 127.0 / a) : 0;
+            for (int i = 0; i < 8; i++)
+                if (!plain || !(off[i] > 3.2e-5f)) c[i] = a > 0.0 ? (int)__builtin_rint(t[i] * 127.0 / a) : 0;
         }
         uint2 out = make_uint2(0, 0);
 #pragma unroll

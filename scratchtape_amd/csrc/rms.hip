@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int threads_of(int tpr) { return tpr < 256 ? 256 : tpr; }
+constexpr int threads_of(int tpr) { return tpr == 64 ? 256 : tpr; }
 
 __device__ __forceinline__ double wave_sum(double v) {
     const int lane = st::lane_id();
@@ -52,6 +52,7 @@ struct Norm {
 template <class T, class W, int TPR, int V, bool NORM>
 __global__ __launch_bounds__(threads_of(TPR)) void k_rms(Norm a) {
     constexpr int ROWS = threads_of(TPR) / TPR, WAVES = TPR / 64, HELD = V ? V : 1;
+    static_assert(ROWS == 1 || WAVES == 1, "rows of several waves meet at barriers");
     constexpr bool WIDE = V == 0;
     typedef st::Eight_t<T> T8;
     const int t = threadIdx.x % TPR, wave = t >> 6;
@@ -171,13 +172,18 @@ st_status launch_rms(const Norm &a, hipStream_t stream) {
         ST_LAUNCH_CHECK();
         return ST_OK;
     };
-    // The width of a row of codes counts too: its zeros are written with it.
+    // The width of a row of codes counts too: its zeros are written with it.  Threads of a row: as few as hold it, so that many rows are
+    // on their way on a CU; for few rows more of them (us with 256 and 1024 threads: 8191 rows of 8192 bf16 to 8 bits 129 and 167, 64
+    // of them 10.1 and 7.5; 2000 rows of 16384 f16 with 512 and 1024 67 and 77, 515 of 11003 14.6 and 14.2).
     const int64_t wide = std::max(a.d, a.c_width);
+    const bool many = a.rows >= 2 * st::device_cus();
     if (wide <= 512) return go(k_rms<T, W, 64, 1, NORM>, 64);
     if (wide <= 1024) return go(k_rms<T, W, 64, 2, NORM>, 64);
-    if (wide <= 2048) return go(k_rms<T, W, 256, 1, NORM>, 256);
+    if (wide <= 2048) return go(k_rms<T, W, 128, 2, NORM>, 128);
     if (wide <= 4096) return go(k_rms<T, W, 256, 2, NORM>, 256);
+    if (wide <= 8192 && many) return go(k_rms<T, W, 256, 4, NORM>, 256);
     if (wide <= 8192) return go(k_rms<T, W, 1024, 1, NORM>, 1024);
+    if (wide <= 16384 && many) return go(k_rms<T, W, 512, 4, NORM>, 512);
     if (wide <= 16384) return go(k_rms<T, W, 1024, 2, NORM>, 1024);
     return go(k_rms<T, W, 1024, 0, NORM>, 1024);
 }
@@ -195,6 +201,7 @@ struct Back {
 template <class T, class W, int TPR, int V>
 __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
     constexpr int ROWS = threads_of(TPR) / TPR, WAVES = TPR / 64;
+    static_assert(ROWS == 1 || WAVES == 1, "rows of several waves meet at barriers");
     typedef st::Eight_t<T> T8;
     const int t = threadIdx.x % TPR, wave = t >> 6, mine = threadIdx.x / TPR;
     float w[V][8], dw[V][8];
@@ -328,17 +335,19 @@ __global__ __launch_bounds__(1024) void k_rms_back_sum(const float *__restrict__
 
 constexpr int64_t BACK_WIDEST = 16384;  // columns that a workgroup's registers hold
 
-// Row lanes of a workgroup of k_rms_back, and the parts that its launch leaves to be summed.
-int64_t back_rows(int64_t d) { return d <= 1024 ? 4 : 1; }
-int64_t back_parts(int64_t rows, int64_t d) {
+// Row lanes of a workgroup of k_rms_back, and the parts that its launch leaves to be summed: a workgroup a CU where its rows keep that
+// busy (f32 rows, 1024 threads, 32 values a thread), two otherwise (us with one, two and four: 16384 x 4096 bf16 124, 113, 124, f32
+// 198, 220, 230; 4096 x 8192 bf16 49, 56, 69; 8000 x 1111 bf16 55, 63, 80).
+int64_t back_rows(int64_t d) { return d <= 2048 ? 4 : 1; }
+int64_t back_parts(int64_t rows, int64_t d, int64_t size) {
     if (d > BACK_WIDEST) return std::min<int64_t>((rows + 31) / 32, 64);
     const int64_t per = back_rows(d), groups = (rows + per - 1) / per;
-    return std::min<int64_t>(groups, 4 * st::device_cus());
+    return std::min<int64_t>(groups, (size == 4 || d > 4096 || (d > 1024 && d <= 2048) ? 1 : 2) * st::device_cus());
 }
 
 template <class T, class W>
 st_status launch_back(Back a, float *dw, hipStream_t stream) {
-    const int64_t parts = back_parts(a.rows, a.d);
+    const int64_t parts = back_parts(a.rows, a.d, sizeof(T));
     float *const part = a.part;
     if (parts == 1) a.part = dw;
     if (a.d > BACK_WIDEST) {
@@ -353,7 +362,7 @@ st_status launch_back(Back a, float *dw, hipStream_t stream) {
         else if (a.d <= 1024)
             go(k_rms_back<T, W, 64, 2>, 64);
         else if (a.d <= 2048)
-            go(k_rms_back<T, W, 256, 1>, 256);
+            go(k_rms_back<T, W, 64, 4>, 64);
         else if (a.d <= 4096)
             go(k_rms_back<T, W, 256, 2>, 256);
         else if (a.d <= 8192)
@@ -441,9 +450,9 @@ extern "C" st_status st_rms_norm(const void *x, const void *residual, int32_t dt
     });
 }
 
-extern "C" int64_t st_rms_norm_backward_bytes(int64_t rows, int64_t d) {
+extern "C" int64_t st_rms_norm_backward_bytes(int64_t rows, int64_t d, int32_t dtype) {
     if (rows <= 0 || d <= 0 || rows > MOST_ROWS || d > MOST_D) return 0;
-    const int64_t parts = back_parts(rows, d);
+    const int64_t parts = back_parts(rows, d, st::dtype_size(dtype));
     return parts > 1 ? parts * d * 4 : 0;
 }
 
@@ -460,7 +469,7 @@ extern "C" st_status st_rms_norm_backward(const void *dy, const void *h, const v
     if (weight_dtype != dtype && weight_dtype != ST_F32)
         return st::fail(ST_ERR_INVALID, "rms_norm_backward: weight dtype %d is neither ST_F32 nor the rows', %d", (int)weight_dtype, (int)dtype);
     if (!dweight || (rows && (!dy || !h || !rstd || !weight || !dx))) return st::fail(ST_ERR_INVALID, "rms_norm_backward: NULL buffer");
-    const int64_t size = st::dtype_size(dtype), need = st_rms_norm_backward_bytes(rows, d);
+    const int64_t size = st::dtype_size(dtype), need = st_rms_norm_backward_bytes(rows, d, dtype);
     if (unaligned(dy, size) || unaligned(h, size) || unaligned(dh, size) || unaligned(dx, size) || unaligned(weight, st::dtype_size(weight_dtype)) ||
         unaligned(rstd, 4) || unaligned(dweight, 4) || unaligned(work, 16))
         return st::fail(ST_ERR_INVALID, "rms_norm_backward: a buffer is not aligned to its elements (work: 16 bytes)");

@@ -151,7 +151,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, wei
     with _launch(device, stream) as handle:
         dx = torch.empty((n, d), dtype=h.dtype, device=device)
         dweight = torch.empty((d,), dtype=torch.float32, device=device)
-        need = _lib.lib().st_rms_norm_backward_bytes(n, d)
+        need = _lib.lib().st_rms_norm_backward_bytes(n, d, dtype)
         work = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
         _lib.call("st_rms_norm_backward", dy.data_ptr(), h.data_ptr(), _addr(dh), dtype, n, d, dy_stride, stride, dh_stride, rstd.data_ptr(),
                   weight.data_ptr(), w_dtype, dx.data_ptr(), dweight.data_ptr(), _addr(work), need, handle)

@@ -49,8 +49,8 @@ def test_norm_refusals():
 def test_backward_refusals():
     ok = dict(dy=FAKE, h=FAKE, dh=FAKE, dtype=0, rows=5000, d=64, dy_stride=64, h_stride=64, dh_stride=64, rstd=FAKE, weight=FAKE, weight_dtype=0,
               dx=FAKE, dweight=FAKE, work=FAKE, work_bytes=1 << 40, stream=None)
-    assert _lib.lib().st_rms_norm_backward_bytes(5000, 64) > 0
-    assert [_lib.lib().st_rms_norm_backward_bytes(*v) for v in ((1, 64), (0, 64), (-1, 64), (5, 0), (1 << 40, 64))] == 5 * [0]
+    assert _lib.lib().st_rms_norm_backward_bytes(5000, 64, 0) > 0
+    assert [_lib.lib().st_rms_norm_backward_bytes(*v, 1) for v in ((1, 64), (0, 64), (-1, 64), (5, 0), (1 << 40, 64))] == 5 * [0]
     for kw, msg in [(dict(d=0), "d 0"), (dict(rows=-1), "rows -1"), (dict(dy_stride=63), "apart"), (dict(h_stride=63), "apart"), (dict(dh_stride=63), "apart"),
                     (dict(dtype=3), "dtype"), (dict(dtype=1, weight_dtype=2), "weight"), (dict(dy=None), "NULL"), (dict(h=None), "NULL"),
                     (dict(rstd=None), "NULL"), (dict(weight=None), "NULL"), (dict(dx=None), "NULL"), (dict(dweight=None), "NULL"),
