@@ -576,6 +576,14 @@ extern "C" {
     ) -> st_status;
     /// Bytes of `work` that `st_matmul_8bit` or `st_gated_8bit` needs.
     pub fn st_matmul_8bit_bytes(m: i64, k: i64, n: i64, gated: i32) -> i64;
+    /// The kernel and the slices of k of such a call, without a device.
+    pub fn st_matmul_8bit_plan(
+        m: i64,
+        k: i64,
+        n: i64,
+        gated: i32,
+        plan: *mut i64,
+    ) -> st_status;
     /// A Linear layer of 8-bit rows and weights.
     pub fn st_matmul_8bit(
         x: *const i8,

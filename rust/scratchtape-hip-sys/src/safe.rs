@@ -1201,6 +1201,13 @@ pub fn matmul_8bit_bytes(m: usize, k: usize, n: usize, gated: bool) -> usize {
     unsafe { sys::st_matmul_8bit_bytes(m as i64, k as i64, n as i64, gated as i32) as usize }
 }
 
+/// The kernel (see the header) and the slices of k that [`matmul_8bit`] or [`gated_8bit`] takes.
+pub fn matmul_8bit_plan(m: usize, k: usize, n: usize, gated: bool) -> [i64; 2] {
+    let mut plan = [0i64; 2];
+    check(unsafe { sys::st_matmul_8bit_plan(m as i64, k as i64, n as i64, gated as i32, plan.as_mut_ptr()) });
+    plan
+}
+
 fn need_rows8<H: DeviceBuffer + ?Sized>(r: &Rows8<H>, rows: usize, k: usize, what: &str) {
     need::<i8, H>(r.codes, span(rows, k, r.stride), what);
     need::<f32, H>(r.scales, rows, what);

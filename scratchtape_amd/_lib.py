@@ -97,6 +97,7 @@ SIGNATURES = {
     "st_rms_norm_backward_bytes": [_i64, _i64, _i32],
     "st_rms_norm_backward": [_vp, _vp, _vp, _i32] + 5 * [_i64] + [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp],
     "st_matmul_8bit_bytes": [_i64, _i64, _i64, _i32],
+    "st_matmul_8bit_plan": [_i64, _i64, _i64, _i32, _vp],
     "st_matmul_8bit": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _i64, _vp, _i64, _vp],
     "st_gated_8bit": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _i64, _vp, _i64, _vp],
     "st_device_info": [_vp, _vp, _vp, _vp],

@@ -302,7 +302,7 @@ __global__ __launch_bounds__(256, std::min(Tiles::AT_ONCE, 4)) void k_product8(P
         brought();
     }
     dma::wait_vm<(NS - 1) * (LX + LW)>();
-    dma::bar();
+    dma::bar_written();
     {
         int from, to;
         slice_of(run.first, from, to);
@@ -342,7 +342,8 @@ __global__ __launch_bounds__(256, std::min(Tiles::AT_ONCE, 4)) void k_product8(P
         // Every operation of a stage stands between two products: the compiler's own order leaves the matrix cores waiting for the
         // barrier, the loads' addresses and the fragments in turn (2,060 TOP/s at 8192 x 16384 x 8192 so, 2,270 in this order).
         for (int st = from; st < to; st++) {
-            constexpr int N = FM * FN, PIECES = FN + FM, LOADS = (LX + LW) / S;
+            constexpr int N = FM * FN, PIECES = FN + FM, LOADS = (LX + LW) / S, MOVES = N > 8 ? N - 4 : N - 1;
+            static_assert(std::min(N - 1, 2 + (LOADS - 1) * (5 * N / 8) / LOADS) <= MOVES, "all of a stage's loads before the next stage's place");
             const uint32_t slot = g % NS * (SX + SW), next = (g + 1) % NS * (SX + SW);
 #pragma unroll
             for (int s = 0; s < KS; s++)
@@ -377,7 +378,7 @@ __global__ __launch_bounds__(256, std::min(Tiles::AT_ONCE, 4)) void k_product8(P
 #pragma unroll
                         for (int l = 0; l < LOADS; l++)
                             if (n == std::min(N - 1, 2 + l * (5 * N / 8) / LOADS)) bring(l, ring + slot);
-                        if (n == (N > 4 ? N - 4 : N - 1)) brought();
+                        if (n == MOVES) brought();
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -819,8 +820,8 @@ st_status product8(const char *name, const Product &a, int32_t dtype, bool is_ga
             ST_LAUNCH_CHECK();
             return ST_OK;
         }
-        // A tile's offsets are 32 bits: rows of weights up to 256 on, and 2 n in a gated product.
-        const bool near = a.x_stride < 1 << 23 && a.out_stride < 1 << 21 && (a.n + 256) * a.w_stride < ((int64_t)1 << 32) - (1 << 16);
+        // A tile's offsets are 32 bits: rows of weights up to 256 on, and in a gated product n further.
+        const bool near = a.x_stride < 1 << 23 && a.out_stride < 1 << 21 && ((is_gated ? a.n : 0) + 256) * a.w_stride < ((int64_t)1 << 32) - (1 << 16);
         if (vec && near && plan.kernel >= LARGE) {
             const int64_t width = is_gated ? 2 * a.n : a.n, need = plan.slices > 1 ? 4 * plan.slices * a.m * width : 0;
             if (need && (!work || work_bytes < need))
@@ -875,9 +876,18 @@ st_status product8(const char *name, const Product &a, int32_t dtype, bool is_ga
 }  // namespace
 
 extern "C" int64_t st_matmul_8bit_bytes(int64_t m, int64_t k, int64_t n, int32_t is_gated) {
-    if (m <= 0 || k <= 0 || n <= 0) return 0;
+    if (m <= 0 || k <= 0 || n <= 0 || m > (int64_t)1 << 30 || k > 131072 || n > (int64_t)1 << 30) return 0;
     const Plan plan = plan_of(m, k, n, is_gated != 0);
     return plan.slices > 1 ? 4 * plan.slices * m * (is_gated ? 2 * n : n) : 0;
+}
+
+extern "C" st_status st_matmul_8bit_plan(int64_t m, int64_t k, int64_t n, int32_t is_gated, int64_t *plan) {
+    st::clear_error();
+    if (m <= 0 || k <= 0 || n <= 0 || k > 131072 || !plan)
+        return st::fail(ST_ERR_INVALID, "matmul_8bit_plan: m %lld, k %lld (1 to 131072), n %lld", (long long)m, (long long)k, (long long)n);
+    const Plan p = plan_of(m, k, n, is_gated != 0);
+    plan[0] = p.kernel, plan[1] = p.slices;
+    return ST_OK;
 }
 
 extern "C" st_status st_matmul_8bit(const int8_t *x, const float *x_scales, int64_t m, int64_t k, int64_t x_stride, const int8_t *w,

@@ -7,6 +7,7 @@ scale NaN and codes 0, so that what is computed from it is NaN.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple, Union
 
 import torch
@@ -87,6 +88,17 @@ def _product(name, x, x_scales, w, w_scales, bias, flag, halves, dtype, out, str
         _lib.call(name, x.data_ptr(), x_scales.data_ptr(), m, k, x_stride, w.data_ptr(), w_scales.data_ptr(), n, w_stride, _addr(bias), flag,
                   out.data_ptr(), DTYPES[dtype], _rows(out, "out"), _addr(work), need, handle)
     return out
+
+
+KERNELS = ("one", "few", "large", "middle", "low", "small", "deep", "deep_low")
+
+
+def product_plan(m: int, k: int, n: int, gated: bool = False) -> Tuple[str, int]:
+    """The kernel (of KERNELS) that matmul_8bit, or gated_8bit, takes for x [m, k] and n columns of out where rows are 16-byte
+    aligned, and into how many slices it cuts k.  Needs no device."""
+    plan = (ctypes.c_int64 * 2)()
+    _lib.call("st_matmul_8bit_plan", m, k, n, int(gated), plan)
+    return KERNELS[plan[0]], plan[1]
 
 
 def matmul_8bit(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
