@@ -72,10 +72,10 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, fwd: LnOut, rows: int
 
 @dataclass
 class RmsOut:
-    """What rms_norm returns: h, the rows it normed (x + residual, or x itself); rstd [rows] float32; and of y, codes, scales
-    and values what was asked for."""
+    """What rms_norm returns: h, the rows it normed (x + residual, or x itself); of y with rstd [rows] float32, for the
+    backward pass, and of codes, scales and values what was asked for."""
     h: torch.Tensor
-    rstd: torch.Tensor
+    rstd: Optional[torch.Tensor] = None
     y: Optional[torch.Tensor] = None
     codes: Optional[torch.Tensor] = None
     scales: Optional[torch.Tensor] = None
@@ -105,7 +105,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     """h = x + residual (x itself without one), rounded to x's type, and its norm h / sqrt(mean h^2 + eps) * weight per row of
     x [rows, d] (float32, float16 or bfloat16, any row stride); weight [d] is of x's type or float32.
 
-    y: return the norm in x's type.  eight_bit: return it as 8-bit rows for quant8's products, codes and scales, and with
+    y: return the norm in x's type, and rstd with it.  eight_bit: return it as 8-bit rows for quant8's products, codes and scales, and with
     `values` also what those stand for in x's type.  The codes are those of the rows h * weight (1 / rms is a factor of a
     row's scale)."""
     dtype = _dtype(x, "x")
@@ -118,18 +118,20 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
         raise ValueError(f"eps is {eps}")
     if values and not eight_bit:
         raise ValueError("values are those of 8-bit rows: eight_bit=True")
+    if not y and not eight_bit:
+        raise ValueError("neither y nor 8-bit rows are asked for")
     _on_gpu(x, [(weight, "weight"), (residual, "residual")])
     device = x.device
     with _launch(device, stream) as handle:
-        rstd = torch.empty((n,), dtype=torch.float32, device=device)
         h = x if residual is None else torch.empty((n, d), dtype=x.dtype, device=device)
-        out = torch.empty((n, d), dtype=x.dtype, device=device) if y else None
-        codes = scales = stood = None
+        out = rstd = codes = scales = stood = None
+        if y:
+            out, rstd = torch.empty((n, d), dtype=x.dtype, device=device), torch.empty((n,), dtype=torch.float32, device=device)
         if eight_bit:
             codes, scales = empty_codes(n, d, device), torch.empty((n,), dtype=torch.float32, device=device)
             stood = torch.empty((n, d), dtype=x.dtype, device=device) if values else None
         _lib.call("st_rms_norm", x.data_ptr(), _addr(residual), dtype, n, d, stride, r_stride, weight.data_ptr(), w_dtype, eps,
-                  0 if residual is None else h.data_ptr(), rstd.data_ptr(), _addr(out), _addr(codes), (d + 15) // 16 * 16, _addr(scales),
+                  0 if residual is None else h.data_ptr(), _addr(rstd), _addr(out), _addr(codes), (d + 15) // 16 * 16, _addr(scales),
                   _addr(stood), handle)
     return RmsOut(h, rstd, out, codes, scales, stood)
 

@@ -121,7 +121,7 @@ def test_python_norm_refusals(monkeypatch):
     x, w = torch.zeros(4, 96).half(), torch.ones(96)
     for kw, msg in [(dict(x=x.double()), "float32"), (dict(x=x[0]), "rows, d"), (dict(x=x[:, :0]), "rows, d"), (dict(weight=w[:95]), "weight"),
                     (dict(weight=w.bfloat16()), "weight"), (dict(weight=w.double()), "weight"), (dict(residual=x[:3]), "residual"),
-                    (dict(residual=x.float()), "residual"), (dict(eps=-1.0), "eps"), (dict(values=True), "eight_bit"), (dict(x=x.t()), "weight|contiguous"),
+                    (dict(residual=x.float()), "residual"), (dict(eps=-1.0), "eps"), (dict(values=True), "eight_bit"), (dict(y=False), "neither"), (dict(x=x.t()), "weight|contiguous"),
                     ({}, "GPU")]:
         with pytest.raises(ValueError, match=msg):
             rows.rms_norm(**{**dict(x=x, weight=w), **kw})
