@@ -529,8 +529,8 @@ st_status st_matmul_8bit_plan(int64_t m, int64_t k, int64_t n, int32_t gated, in
 
 /* out[i, j] = (sum over l of x[i, l] w[j, l]) x_scales[i] w_scales[j] + bias[j] (f32,
  * NULL: none), then ReLU where relu != 0: the Linear layer x @ w^T of codes x [m, k]
- * and w [n, k].  Sums of codes are exact, k <= 131072.  out [m, n] has element type
- * dtype and is rounded once.  work: st_matmul_8bit_bytes of device memory, 16-byte
+ * and w [n, k].  Sums of codes, -127 to 127, are exact, k <= 131072.  out [m, n] has
+ * element type dtype and is rounded once.  work: st_matmul_8bit_bytes of device memory, 16-byte
  * aligned, the call's own until its work on `stream` is done. */
 st_status st_matmul_8bit(const int8_t *x, const float *x_scales, int64_t m, int64_t k,
                          int64_t x_stride, const int8_t *w, const float *w_scales, int64_t n,

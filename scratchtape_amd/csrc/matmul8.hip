@@ -1,6 +1,6 @@
 // Products of 8-bit rows and 8-bit weights (quant8.h): out[i, j] = (sum over l of x[i, l] w[j, l]) xs[i] ws[j] + bias[j], then
-// ReLU; and the gated form act(gate) up of two such products.  Sums of codes are exact in 32-bit integers (k <= 131072:
-// 128 x 128 x 131072 = 2^31 is passed by no sum of codes up to 127, and reached only by -128 throughout); the scales enter once, in f32.
+// ReLU; and the gated form act(gate) up of two such products.  Sums of codes are exact in 32-bit integers (k <= 131072; 2^31 is
+// reached by 131072 products of -128 and -128 alone, a code that the format does not have); the scales enter once, in f32.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -25,8 +25,7 @@ struct Product {
 
 // act(g) u.  silu is g / (1 + exp(-g)).  gelu is g Phi(g) = g erfc(-g / sqrt 2) / 2, with erfc(z) = exp(-z^2) t P(t), t = 1 / (1 + z / 2),
 // for z >= 0: P of degree 8 is within 4.4e-8 of erfc for all z up to 14 (a least-squares fit of the relative error; erfc(14) is 0 in
-// f32), and keeps the digits of the tail where 1 + erf would cancel.  About 20 operations; the library's erfcf takes some 100
-// (gated_prompts: 605 us with it, of which a fifth).
+// f32), and keeps the digits of the tail where 1 + erf would cancel.  About 20 operations; the library's erfcf takes some 100.
 __device__ __forceinline__ float gated(float g, float u, int32_t act) {
     if (act == ST_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * g)) * u;
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35355339f, __builtin_fabsf(g), 1.f));
@@ -745,7 +744,7 @@ Plan plan_of(int64_t m, int64_t k, int64_t n, bool is_gated) {
             if (t < least) least = t, best = Plan{r.kernel, slices};
         }
     }
-    if (m <= 32) {
+    if (m <= 32 && width <= 1 << 26) {  // (a launch has less than 2^32 threads along x)
         const double blocks = (double)((width + 15) / 16), at_once = 8.0 * (double)cus / (is_gated ? 2 : 1);
         const double t = 4.61 + 0.134e-6 * (double)width * (double)k * (1 + 0.613 * (double)m / 16) + 0.69 * std::ceil(blocks / at_once) * (double)k / 1024;
         if (t < least) best = Plan{FEW, 1};
@@ -885,8 +884,8 @@ extern "C" int64_t st_matmul_8bit_bytes(int64_t m, int64_t k, int64_t n, int32_t
 
 extern "C" st_status st_matmul_8bit_plan(int64_t m, int64_t k, int64_t n, int32_t is_gated, int64_t *plan) {
     st::clear_error();
-    if (m <= 0 || k <= 0 || n <= 0 || k > 131072 || !plan)
-        return st::fail(ST_ERR_INVALID, "matmul_8bit_plan: m %lld, k %lld (1 to 131072), n %lld", (long long)m, (long long)k, (long long)n);
+    if (m <= 0 || k <= 0 || n <= 0 || m > (int64_t)1 << 30 || k > 131072 || n > (int64_t)1 << 30 || !plan)
+        return st::fail(ST_ERR_INVALID, "matmul_8bit_plan: m %lld and n %lld (1 to 2^30), k %lld (1 to 131072)", (long long)m, (long long)n, (long long)k);
     const Plan p = plan_of(m, k, n, is_gated != 0);
     plan[0] = p.kernel, plan[1] = p.slices;
     return ST_OK;

@@ -105,7 +105,7 @@ def matmul_8bit(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scal
                 relu: bool = False, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """x [m, k] @ w [n, k]^T with both rows' scales, + bias (float32 [n]), then ReLU if asked: a Linear layer in 8 bits.
 
-    Returns [m, n] in `dtype` (`out` if given, of that type).  Sums of codes are exact (k up to 131072); scales, bias and the
+    Returns [m, n] in `dtype` (`out` if given, of that type).  Sums of codes (-127 to 127) are exact, k up to 131072; scales, bias and the
     one rounding to `dtype` follow.  Codes and out may have any row stride; codes whose rows are 16-byte aligned, as
     quantize_8bit lays them, are many times faster than others."""
     return _product("st_matmul_8bit", x, x_scales, w, w_scales, bias, int(bool(relu)), 1, dtype, out, stream)

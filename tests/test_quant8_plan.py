@@ -33,11 +33,19 @@ def test_every_kernel_is_taken(gated):
 
 
 def test_plan_refusals():
-    for bad in ((0, 5, 5), (5, 0, 5), (5, 5, 0), (5, 131073, 5), (-1, 5, 5)):
+    for bad in ((0, 5, 5), (5, 0, 5), (5, 5, 0), (5, 131073, 5), (-1, 5, 5), ((1 << 30) + 1, 5, 5), (5, 5, (1 << 30) + 1)):
         with pytest.raises(_lib.ScratchtapeError, match="matmul_8bit_plan"):
             quant8.product_plan(*bad)
         assert _lib.lib().st_matmul_8bit_bytes(*bad, 0) == 0
     assert _lib.lib().st_matmul_8bit_bytes(1 << 40, 64, 1 << 40, 0) == 0
+
+
+def test_launches_stay_within_2_to_the_32_threads():
+    """The kernel for few rows has a workgroup of up to 512 threads for 16 rows of weights, and is not taken where that is too many."""
+    for n in (1 << 27, (1 << 30) - 5):
+        for m in (1, 7, 32):
+            for gated in (False, True):
+                assert quant8.product_plan(m, 16, n, gated)[0] != "few"
 
 
 @pytest.mark.skipif(test_lds_waits.HIPCC is None, reason="needs hipcc")
