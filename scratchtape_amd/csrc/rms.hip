@@ -197,19 +197,23 @@ struct Back {
 };
 
 // dx = dh + rstd (g - xh mean(g xh)) with g = dy w, xh = h rstd; a workgroup's rows are blockIdx.x ROWS .. in steps of
-// gridDim.x ROWS, and a thread keeps the weight gradient's sums of its own columns over them.
+// gridDim.x ROWS, and a thread keeps the weight gradient's sums of its own columns over them: in 64 bits for f32 rows (up to 1.3e-7
+// off in f32, 4.5e-8 so, in the same time), but for the widest, whose registers hold f32's alone (131 us for 2000 x 16384, 117 so).
 template <class T, class W, int TPR, int V>
 __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
     constexpr int ROWS = threads_of(TPR) / TPR, WAVES = TPR / 64;
     static_assert(ROWS == 1 || WAVES == 1, "rows of several waves meet at barriers");
     typedef st::Eight_t<T> T8;
+    constexpr bool LONG = sizeof(T) == 4 && (TPR < 1024 || V == 1);
+    typedef std::conditional_t<LONG, double, float> Sum;
     const int t = threadIdx.x % TPR, wave = t >> 6, mine = threadIdx.x / TPR;
-    float w[V][8], dw[V][8];
+    float w[V][8];
+    Sum dw[V][8];
 #pragma unroll
     for (int v = 0; v < V; v++) {
         const st::Eight_t<W> wv = st::load_eight((const W *)a.w, (v * TPR + t) * 8, a.d);
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[v][i] = (float)wv[i], dw[v][i] = 0.f;
+        for (int i = 0; i < 8; i++) w[v][i] = (float)wv[i], dw[v][i] = 0;
     }
     __shared__ double sums[2][WAVES];
     int turn = 0;
@@ -243,7 +247,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float xh = (float)h[v][i] * rstd, g = (float)dy[v][i];
-                dw[v][i] = __builtin_fmaf(g, xh, dw[v][i]);
+                dw[v][i] = LONG ? (Sum)__builtin_fma((double)g, (double)xh, (double)dw[v][i]) : (Sum)__builtin_fmaf(g, xh, (float)dw[v][i]);
                 const float dx = rstd * __builtin_fmaf(-xh, mean, g * w[v][i]);
                 out[i] = (T)(a.dh ? (float)dh[v][i] + dx : dx);
             }
@@ -251,7 +255,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
         }
     }
     if constexpr (ROWS > 1) {
-        __shared__ float rows_of[ROWS - 1][V][8][TPR];
+        __shared__ Sum rows_of[ROWS - 1][V][8][TPR];
         if (mine > 0) {
 #pragma unroll
             for (int v = 0; v < V; v++)
@@ -271,7 +275,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
     for (int v = 0; v < V; v++) {
         st::Eight_t<float> out;
 #pragma unroll
-        for (int i = 0; i < 8; i++) out[i] = dw[v][i];
+        for (int i = 0; i < 8; i++) out[i] = (float)dw[v][i];
         st::store_eight(a.part + blockIdx.x * a.d, (v * TPR + t) * 8, a.d, out);
     }
 }
@@ -305,10 +309,10 @@ template <class T>
 __global__ __launch_bounds__(256) void k_rms_back_columns(Back a) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= a.d) return;
-    float s = 0.f;
+    double s = 0.0;
     for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y)
-        s = __builtin_fmaf((float)((const T *)a.dy)[row * a.dy_stride + i], (float)((const T *)a.h)[row * a.h_stride + i] * a.rstd[row], s);
-    a.part[blockIdx.y * a.d + i] = s;
+        s = __builtin_fma((double)(float)((const T *)a.dy)[row * a.dy_stride + i], (double)((float)((const T *)a.h)[row * a.h_stride + i] * a.rstd[row]), s);
+    a.part[blockIdx.y * a.d + i] = (float)s;
 }
 
 // dw[i] = sum over p of part[p, i]: 64 columns a workgroup, its 16 waves taking every 16th p, joined in order, in 64 bits.
