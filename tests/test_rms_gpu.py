@@ -195,3 +195,25 @@ def test_streams_and_graphs(dev):
                 assert torch.equal(getattr(a, name), getattr(b, name)), name
         for a in (back, kept_back):
             assert torch.equal(a[0], grads[0]) and torch.equal(a[1], grads[1])
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("d", [*range(1, 16), *range(505, 512), *range(1097, 1104), *range(4001, 4008), *range(9001, 9008)])
+def test_ends_of_rows(dev, d, t):
+    """Every number of elements behind a row's last eight; rows apart, with NaN between them that nothing may read."""
+    t = TYPES[t]
+    w = (1 + 0.3 * torch.randn(d, generator=gen(d))).to(t).to(dev)
+
+    def apart(seed):
+        base = torch.full((6, d + 9), math.nan, dtype=t, device=dev)
+        base[:, 5:5 + d] = torch.randn(6, d, generator=gen(seed)).to(t).to(dev)
+        return base[:, 5:5 + d]
+
+    x, r, dy, dh = (apart(s) for s in range(4))
+    check(x, r, w, 1e-5, rows.rms_norm(x, w, residual=r, eight_bit=True, values=True), eight=True, values=True)
+    rstd = rows.rms_norm(x, w).rstd
+    for more in (None, dh):
+        dx, dw = rows.rms_norm_backward(dy, x, rstd, w, dh=more)
+        (ex, tx), (ew, tw) = oracle.norm_backward(dy, x, rstd, w, more)
+        oracle.close(dx, ex, tx)
+        oracle.close(dw, ew, tw)
