@@ -20,8 +20,13 @@ ACTIVATIONS = {"silu": 2, "gelu": 3}  # ST_ACT_SILU, ST_ACT_GELU
 
 def empty_codes(rows: int, k: int, device) -> torch.Tensor:
     """Room for codes [rows, k] whose rows are 16-byte aligned, as the products read them fastest."""
+    return torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
+
+
+def _new_codes(rows: int, k: int, like: torch.Tensor) -> torch.Tensor:
+    """empty_codes where `like` is."""
     width = (k + 15) // 16 * 16
-    codes = torch.empty((rows, width), dtype=torch.int8, device=device)
+    codes = like.new_empty((rows, width), dtype=torch.int8)
     return codes if width == k else codes[:, :k]
 
 
@@ -41,10 +46,9 @@ def quantize_8bit(x: torch.Tensor, values: Union[bool, torch.Tensor] = False, st
         _apart([(out, "values")], [(x, "x")])
     _on_gpu(x, [(out, "values")])
     with _launch(x.device, stream) as handle:
-        codes = empty_codes(n, k, x.device)
-        scales = torch.empty((n,), dtype=torch.float32, device=x.device)
+        codes, scales = _new_codes(n, k, x), x.new_empty((n,), dtype=torch.float32)
         if out is None and values:
-            out = torch.empty((n, k), dtype=x.dtype, device=x.device)
+            out = x.new_empty((n, k))
         _lib.call("st_quantize_8bit", x.data_ptr(), dtype, n, k, stride, codes.data_ptr(), (k + 15) // 16 * 16, scales.data_ptr(),
                   _addr(out), handle)
     return (codes, scales) if out is None else (codes, scales, out)
@@ -77,16 +81,16 @@ def _product(name, x, x_scales, w, w_scales, bias, flag, halves, dtype, out, str
     else:
         if _dtype(out, "out") != DTYPES.get(dtype) or tuple(out.shape) != (m, n):
             raise ValueError(f"out is {dtype} [{m}, {n}]; got {out.dtype} {list(out.shape)}")
-        _rows(out, "out")
+        out_stride = _rows(out, "out")
         _apart([(out, "out")], [(x, "x"), (x_scales, "x_scales"), (w, "w"), (w_scales, "w_scales"), (bias, "bias")])
     _on_gpu(x, [(x_scales, "x_scales"), (w, "w"), (w_scales, "w_scales"), (bias, "bias"), (out, "out")])
     with _launch(x.device, stream) as handle:
         if out is None:
-            out = torch.empty((m, n), dtype=dtype, device=x.device)
+            out, out_stride = x_scales.new_empty((m, n), dtype=dtype), n
         need = _lib.lib().st_matmul_8bit_bytes(m, k, n, halves - 1)
-        work = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
+        work = x.new_empty((need,)) if need else None
         _lib.call(name, x.data_ptr(), x_scales.data_ptr(), m, k, x_stride, w.data_ptr(), w_scales.data_ptr(), n, w_stride, _addr(bias), flag,
-                  out.data_ptr(), DTYPES[dtype], _rows(out, "out"), _addr(work), need, handle)
+                  out.data_ptr(), DTYPES[dtype], out_stride, _addr(work), need, handle)
     return out
 
 

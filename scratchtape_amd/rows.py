@@ -11,7 +11,7 @@ import torch
 from . import _lib
 from .matmul import _ptr, _stream
 from .quant4 import DTYPES, _addr, _dtype, _launch, _on_gpu, _plain, _rows
-from .quant8 import empty_codes
+from .quant8 import _new_codes
 
 
 def _check_rows_out(out: torch.Tensor | None, n: int, device, name: str) -> None:
@@ -121,15 +121,14 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     if not y and not eight_bit:
         raise ValueError("neither y nor 8-bit rows are asked for")
     _on_gpu(x, [(weight, "weight"), (residual, "residual")])
-    device = x.device
-    with _launch(device, stream) as handle:
-        h = x if residual is None else torch.empty((n, d), dtype=x.dtype, device=device)
+    with _launch(x.device, stream) as handle:
+        h = x if residual is None else x.new_empty((n, d))
         out = rstd = codes = scales = stood = None
         if y:
-            out, rstd = torch.empty((n, d), dtype=x.dtype, device=device), torch.empty((n,), dtype=torch.float32, device=device)
+            out, rstd = x.new_empty((n, d)), x.new_empty((n,), dtype=torch.float32)
         if eight_bit:
-            codes, scales = empty_codes(n, d, device), torch.empty((n,), dtype=torch.float32, device=device)
-            stood = torch.empty((n, d), dtype=x.dtype, device=device) if values else None
+            codes, scales = _new_codes(n, d, x), x.new_empty((n,), dtype=torch.float32)
+            stood = x.new_empty((n, d)) if values else None
         _lib.call("st_rms_norm", x.data_ptr(), _addr(residual), dtype, n, d, stride, r_stride, weight.data_ptr(), w_dtype, eps,
                   0 if residual is None else h.data_ptr(), _addr(rstd), _addr(out), _addr(codes), (d + 15) // 16 * 16, _addr(scales),
                   _addr(stood), handle)
@@ -149,12 +148,10 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, wei
     dy_stride, dh_stride = _norm_rows(dy, h, "dy"), 0 if dh is None else _norm_rows(dh, h, "dh")
     _plain(rstd, torch.float32, (n,), "rstd")
     _on_gpu(h, [(dy, "dy"), (dh, "dh"), (rstd, "rstd"), (weight, "weight")])
-    device = h.device
-    with _launch(device, stream) as handle:
-        dx = torch.empty((n, d), dtype=h.dtype, device=device)
-        dweight = torch.empty((d,), dtype=torch.float32, device=device)
+    with _launch(h.device, stream) as handle:
+        dx, dweight = h.new_empty((n, d)), h.new_empty((d,), dtype=torch.float32)
         need = _lib.lib().st_rms_norm_backward_bytes(n, d, dtype)
-        work = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+        work = h.new_empty((need,), dtype=torch.uint8) if need else None
         _lib.call("st_rms_norm_backward", dy.data_ptr(), h.data_ptr(), _addr(dh), dtype, n, d, dy_stride, stride, dh_stride, rstd.data_ptr(),
                   weight.data_ptr(), w_dtype, dx.data_ptr(), dweight.data_ptr(), _addr(work), need, handle)
     return dx, dweight
