@@ -202,7 +202,7 @@ struct Back {
 // dx = dh + rstd (g - xh mean(g xh)) with g = dy w, xh = h rstd; a workgroup's rows are blockIdx.x ROWS .. in steps of
 // gridDim.x ROWS, and a thread keeps the weight gradient's sums of its own columns over them: in 64 bits for f32 rows (up to 1.3e-7
 // off in f32, 4.5e-8 so, in the same time), but for the widest, whose registers hold f32's alone (131 us for 2000 x 16384, 117 so).  Bound by HBM:
-// 16384 x 4096 bf16 with dh 95 us and 10 of the sum's launch, 5 TB/s; 4096 x 256 f32 10 and 6, latencies of rows one after the other.
+// 16384 x 4096 bf16 with dh 110 us with the sum's launch, 4.9 TB/s; 4096 x 256 f32 12, latencies of rows one after the other.
 template <class T, class W, int TPR, int V>
 __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
     constexpr int ROWS = threads_of(TPR) / TPR, WAVES = TPR / 64;
@@ -334,26 +334,35 @@ __global__ __launch_bounds__(256) void k_rms_back_columns(Back a) {
     a.part[blockIdx.y * a.d + i] = (float)s;
 }
 
-// dw[i] = sum over p of part[p, i]: 64 columns a workgroup, its 16 waves taking every 16th p, joined in order, in 64 bits.
+// dw[i] = sum over p of part[p, i]: 16 columns a workgroup, whose 64 rows of lanes take every 64th p, joined in order, in 64 bits.
+// A launch's latency and one of the loads' (4096 x 256 f32's whole backward 12.4 us, 15.5 with 64 columns a workgroup).
 __global__ __launch_bounds__(1024) void k_rms_back_sum(const float *__restrict__ part, int64_t parts, int64_t d, float *__restrict__ dw) {
-    __shared__ double sums[16][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+    __shared__ double sums[16][16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, column = lane & 15;
+    const int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16 + column;
     double s = 0.0;
     if (i < d)
-        for (int64_t p = wave; p < parts; p += 16 * 8) {
+        for (int64_t p = threadIdx.x >> 4; p < parts; p += 64 * 8) {
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = p + 16 * j < parts ? part[(p + 16 * j) * d + i] : 0.f;
+            for (int j = 0; j < 8; j++) v[j] = p + 64 * j < parts ? part[(p + 64 * j) * d + i] : 0.f;
 #pragma unroll
             for (int j = 0; j < 8; j++) s += (double)v[j];
         }
-    sums[wave][lane] = s;
+    s += st::xor_lane(s, 16, lane);
+    s += st::xor_lane(s, 32, lane);
+    if (lane < 16) sums[wave][column] = s;
     __syncthreads();
-    if (wave || i >= d) return;
+    if (threadIdx.x >= 16 || i >= d) return;
 #pragma unroll
-    for (int j = 1; j < 16; j++) s += sums[j][lane];
+    for (int j = 1; j < 16; j++) s += sums[j][column];
     dw[i] = (float)s;
+}
+
+// Its grid: a launch has less than 2^32 threads along x.
+dim3 sum_grid(int64_t d) {
+    const int64_t blocks = (d + 15) / 16, along = std::min<int64_t>(blocks, 1 << 21);
+    return dim3((uint32_t)along, (uint32_t)((blocks + along - 1) / along));
 }
 
 constexpr int64_t BACK_WIDEST = 16384;  // columns that a workgroup's registers hold
@@ -395,7 +404,7 @@ st_status launch_back(Back a, float *dw, hipStream_t stream) {
     }
     ST_LAUNCH_CHECK();
     if (parts > 1) {
-        k_rms_back_sum<<<(uint32_t)((a.d + 63) / 64), 1024, 0, stream>>>(part, parts, a.d, dw);
+        k_rms_back_sum<<<sum_grid(a.d), 1024, 0, stream>>>(part, parts, a.d, dw);
         ST_LAUNCH_CHECK();
     }
     return ST_OK;
@@ -500,7 +509,7 @@ extern "C" st_status st_rms_norm_backward(const void *dy, const void *h, const v
         return st::fail(ST_ERR_INVALID, "rms_norm_backward: %lld bytes of work memory are needed, got %lld", (long long)need, (long long)(work ? work_bytes : 0));
     if (!st::device_ok()) return ST_ERR_NO_DEVICE;
     if (rows == 0) {  // no row: the sum over none
-        k_rms_back_sum<<<(uint32_t)((d + 63) / 64), 1024, 0, st::stream_of(stream)>>>(nullptr, 0, d, dweight);
+        k_rms_back_sum<<<sum_grid(d), 1024, 0, st::stream_of(stream)>>>(nullptr, 0, d, dweight);
         ST_LAUNCH_CHECK();
         return ST_OK;
     }

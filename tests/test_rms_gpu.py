@@ -217,3 +217,14 @@ def test_ends_of_rows(dev, d, t):
         (ex, tx), (ew, tw) = oracle.norm_backward(dy, x, rstd, w, more)
         oracle.close(dx, ex, tx)
         oracle.close(dw, ew, tw)
+
+
+def test_backward_of_one_long_row(dev):
+    """A row so wide that the launch that joins the parts has more workgroups than fit one line of a grid."""
+    d = (1 << 25) + 17
+    x, dy = (torch.randn(33, d, generator=torch.Generator(dev).manual_seed(s), device=dev, dtype=torch.bfloat16) for s in (1, 2))
+    w, rstd = torch.ones(d, device=dev), torch.ones(33, device=dev)
+    dx, dw = rows.rms_norm_backward(dy, x, rstd, w)
+    for part in (slice(0, 40), slice(d // 2, d // 2 + 40), slice(d - 40, d)):
+        products = dy[:, part].cpu().double() * x[:, part].cpu().double()
+        oracle.close(dw[part], products.sum(0), 40 * oracle.U * products.abs().sum(0))
