@@ -367,14 +367,14 @@ dim3 sum_grid(int64_t d) {
 
 constexpr int64_t BACK_WIDEST = 16384;  // columns that a workgroup's registers hold
 
-// Row lanes of a workgroup of k_rms_back, and the parts that its launch leaves to be summed: a workgroup a CU where its rows keep that
-// busy (f32 rows, 1024 threads, 32 values a thread), two otherwise (us with one, two and four: 16384 x 4096 bf16 124, 113, 124, f32
-// 198, 220, 230; 4096 x 8192 bf16 49, 56, 69; 8000 x 1111 bf16 55, 63, 80).
+// Row lanes of a workgroup of k_rms_back, and the parts that its launch leaves to be summed: two workgroups a CU, one where its rows keep
+// that busy (wide f32 rows, 1024 threads).  us with one and two: 4096 x 256 f32 12.7, 11.6, 8000 x 1900 62, 66, 16384 x 4096 204, 216;
+// bf16 32768 x 512 45, 32, 8000 x 1111 34, 37, 16384 x 2048 62, 54, 16384 x 4096 131, 114, 4096 x 8192 49, 53.
 int64_t back_rows(int64_t d) { return d <= 2048 ? 4 : 1; }
 int64_t back_parts(int64_t rows, int64_t d, int64_t size) {
     if (d > BACK_WIDEST) return std::min<int64_t>((rows + 31) / 32, 64);
     const int64_t per = back_rows(d), groups = (rows + per - 1) / per;
-    return std::min<int64_t>(groups, (size == 4 || d > 4096 || (d > 1024 && d <= 2048) ? 1 : 2) * st::device_cus());
+    return std::min<int64_t>(groups, (d <= (size == 4 ? 1024 : 4096) ? 2 : 1) * st::device_cus());
 }
 
 template <class T, class W>
