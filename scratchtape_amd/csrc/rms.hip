@@ -202,7 +202,7 @@ struct Back {
 // dx = dh + rstd (g - xh mean(g xh)) with g = dy w, xh = h rstd; a workgroup's rows are blockIdx.x ROWS .. in steps of
 // gridDim.x ROWS, and a thread keeps the weight gradient's sums of its own columns over them: in 64 bits for f32 rows (up to 1.3e-7
 // off in f32, 4.5e-8 so, in the same time), but for the widest, whose registers hold f32's alone (131 us for 2000 x 16384, 117 so).  Bound by HBM:
-// 16384 x 4096 bf16 with dh 110 us with the sum's launch, 4.9 TB/s; 4096 x 256 f32 12, latencies of rows one after the other.
+// 16384 x 4096 bf16 with dh 110 us with the sum's launch, 4.9 TB/s; 4096 x 256 f32 11.6, latencies of rows one after the other.
 template <class T, class W, int TPR, int V>
 __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
     constexpr int ROWS = threads_of(TPR) / TPR, WAVES = TPR / 64;
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(256) void k_rms_back_columns(Back a) {
 }
 
 // dw[i] = sum over p of part[p, i]: 16 columns a workgroup, whose 64 rows of lanes take every 64th p, joined in order, in 64 bits.
-// A launch's latency and one of the loads' (4096 x 256 f32's whole backward 12.4 us, 15.5 with 64 columns a workgroup).
+// A launch's latency and one of the loads' (4096 x 256 f32's whole backward 3 us less than with 64 columns a workgroup).
 __global__ __launch_bounds__(1024) void k_rms_back_sum(const float *__restrict__ part, int64_t parts, int64_t d, float *__restrict__ dw) {
     __shared__ double sums[16][16];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, column = lane & 15;
