@@ -200,25 +200,43 @@ struct Back {
 };
 
 // dx = dh + rstd (g - xh mean(g xh)) with g = dy w, xh = h rstd; a workgroup's rows are blockIdx.x ROWS .. in steps of
-// gridDim.x ROWS, and a thread keeps the weight gradient's sums of its own columns over them: in 64 bits for f32 rows (up to 1.3e-7
-// off in f32, 4.5e-8 so, in the same time), but for the widest, whose registers hold f32's alone (131 us for 2000 x 16384, 117 so).  Bound by HBM:
-// 16384 x 4096 bf16 with dh 110 us with the sum's launch, 4.9 TB/s; 4096 x 256 f32 11.6, latencies of rows one after the other.
+// gridDim.x ROWS, and a thread keeps the weight gradient's sums of its own columns over them in 64 bits, so that their error does not
+// grow with the number of rows (chains of 64 rows in f32 are off by 1.5e-7, 4.4e-8 so; 32768 x 256 bf16 25 us, 24 with f32 sums); each
+// part is rounded to f32 once.  Where those sums leave too few registers, or room for one workgroup of a CU's two, the weights lie in LDS (us
+// so and in registers: 2000 x 16384 f32 114 and 131, 8000 x 1900 bf16 32 and 40; f32, which has one workgroup a CU, 64 and 61).
+// Bound by HBM: 16384 x 4096 bf16 with dh 110 us with the sum's launch, 4.9 TB/s; 4096 x 256 f32 11.6, latencies of rows one after the other.
 template <class T, class W, int TPR, int V>
 __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
     constexpr int ROWS = threads_of(TPR) / TPR, WAVES = TPR / 64;
     static_assert(ROWS == 1 || WAVES == 1, "rows of several waves meet at barriers");
     typedef st::Eight_t<T> T8;
-    constexpr bool LONG = sizeof(T) == 4 && (TPR < 1024 || V == 1);
-    typedef std::conditional_t<LONG, double, float> Sum;
+    constexpr bool W_LDS = (V == 4 && sizeof(T) == 2) || (TPR == 1024 && V == 2);
+    typedef float F4 __attribute__((ext_vector_type(4)));
+    __shared__ F4 w_lds[W_LDS ? 2 * V : 1][TPR];
     const int t = threadIdx.x % TPR, wave = t >> 6, mine = threadIdx.x / TPR;
-    float w[V][8];
-    Sum dw[V][8];
+    float w_held[W_LDS ? 1 : V][8];
+    double dw[V][8];
 #pragma unroll
     for (int v = 0; v < V; v++) {
         const st::Eight_t<W> wv = st::load_eight((const W *)a.w, (v * TPR + t) * 8, a.d);
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[v][i] = (float)wv[i], dw[v][i] = 0;
+        for (int i = 0; i < 8; i++) dw[v][i] = 0;
+        if constexpr (W_LDS) {
+            if (mine == 0) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) w_lds[2 * v + i][t] = F4{(float)wv[4 * i], (float)wv[4 * i + 1], (float)wv[4 * i + 2], (float)wv[4 * i + 3]};
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) w_held[v][i] = (float)wv[i];
+        }
     }
+    if constexpr (W_LDS && ROWS > 1) __syncthreads();  // (else a thread reads what it wrote)
+    auto weights = [&](int v, float (&w)[8]) {
+        if constexpr (W_LDS) asm volatile("" ::: "memory");  // (from LDS each time, not into registers ahead of the loop)
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = W_LDS ? w_lds[2 * v + i / 4][t][i % 4] : w_held[W_LDS ? 0 : v][i];
+    };
     // A row's last vector, of 16-bit elements, as its last eight, moved to their places when all loads are on their way (us so and with
     // load_eight: 8000 x 4003 bf16 70 and 107, 8000 x 1111 37 and 45, 16384 x 4096 114 and 114; f32 16384 x 4096 305 and 203).
     constexpr bool LATE = sizeof(T) == 2;
@@ -247,9 +265,12 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
         }
         double s = 0.0;
 #pragma unroll
-        for (int v = 0; v < V; v++)
+        for (int v = 0; v < V; v++) {
+            float w[8];
+            weights(v, w);
 #pragma unroll
-            for (int i = 0; i < 8; i++) s = __builtin_fma((double)((float)dy[v][i] * w[v][i]), (double)(float)h[v][i], s);
+            for (int i = 0; i < 8; i++) s = __builtin_fma((double)((float)dy[v][i] * w[i]), (double)(float)h[v][i], s);
+        }
         s = wave_sum(s);
         if constexpr (WAVES > 1) {
             if ((t & 63) == 0) sums[turn][wave] = s;
@@ -263,18 +284,20 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
 #pragma unroll
         for (int v = 0; v < V; v++) {
             T8 out;
+            float w[8];
+            weights(v, w);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float xh = (float)h[v][i] * rstd, g = (float)dy[v][i];
-                dw[v][i] = LONG ? (Sum)__builtin_fma((double)g, (double)xh, (double)dw[v][i]) : (Sum)__builtin_fmaf(g, xh, (float)dw[v][i]);
-                const float dx = rstd * __builtin_fmaf(-xh, mean, g * w[v][i]);
+                dw[v][i] = __builtin_fma((double)g, (double)xh, dw[v][i]);
+                const float dx = rstd * __builtin_fmaf(-xh, mean, g * w[i]);
                 out[i] = (T)(a.dh ? (float)dh[v][i] + dx : dx);
             }
             st::store_eight((T *)a.dx + row * a.d, (v * TPR + t) * 8, a.d, out);
         }
     }
     if constexpr (ROWS > 1) {
-        __shared__ Sum rows_of[ROWS - 1][V][8][TPR];
+        __shared__ double rows_of[ROWS - 1][V][8][TPR];
         if (mine > 0) {
 #pragma unroll
             for (int v = 0; v < V; v++)
