@@ -42,7 +42,12 @@ __device__ __forceinline__ float gated(float g, float u, int32_t act) {
     return g * (g < 0.f ? half : 1.f - half) * u;
 }
 
-__device__ __forceinline__ float scaled(int32_t sum, float xs, float ws, float bias) { return __builtin_fmaf((float)sum * xs, ws, bias); }
+// sum xs ws + bias.  A sum is below 2^31, so it can be multiplied by the row's scale first up to 2^96; a larger one comes last, and the sum
+// times the channel's passes f32's range only where the result does too.  (A sum times a subnormal scale loses nothing.)
+__device__ __forceinline__ float scaled(int32_t sum, float xs, float ws, float bias) {
+    const bool last = __builtin_fabsf(xs) >= 0x1p96f;
+    return __builtin_fmaf((float)sum * (last ? ws : xs), last ? xs : ws, bias);
+}
 
 // 16 codes from p on, of which `left` are inside the row; unaligned rows are read a byte at a time.
 __device__ __forceinline__ i4 load16(const int8_t *p, int64_t left, bool vec) {
