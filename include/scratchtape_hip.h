@@ -520,11 +520,16 @@ st_status st_rms_norm_backward(const void *dy, const void *h, const void *dh, in
  * where there are few outputs. */
 int64_t st_matmul_8bit_bytes(int64_t m, int64_t k, int64_t n, int32_t gated);
 
-/* The kernel that such a call of 16-byte aligned rows launches on the current device
- * (or, without one, on one of 256 CUs), and the slices of k (more than one: a second
- * launch joins them): plan[0] is 0 for one to four rows of x, 1 for few rows, 2 to 7 for
- * tiles of x by w of 256 x 256, 128 x 128, 64 x 128 (gated), 64 x 64, and, for up to 64
- * rows of x, 64 x 64 and 64 x 128 (gated). */
+/* The kernel that such a call launches on the current device (or, without one, on one
+ * of 256 CUs) where rows of codes are 16-byte aligned and as close as that leaves them
+ * and out is contiguous, and the slices of k (more than one: a second launch joins
+ * them): plan[0] is 0 for one to four rows of x, 1 for few rows, 2 to 7 for tiles of x by
+ * w of 256 x 256, 128 x 128, 64 x 128 (gated), 64 x 64, and, for up to 64 rows of x,
+ * 64 x 64 and 64 x 128 (gated), and 8 for the kernel for any strides.  That one, or for
+ * up to 32 rows of x the one for few, takes the place of tiles where their offsets would
+ * not fit 32 bits: out's rows 2^21 elements or more apart, x's 2^23 bytes, or
+ * 256 rows of w (gated: n + 256) over 2^32 - 2^16 bytes; and of all where codes
+ * are not aligned. */
 st_status st_matmul_8bit_plan(int64_t m, int64_t k, int64_t n, int32_t gated, int64_t *plan);
 
 /* out[i, j] = (sum over l of x[i, l] w[j, l]) x_scales[i] w_scales[j] + bias[j] (f32,

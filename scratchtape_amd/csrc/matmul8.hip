@@ -59,8 +59,8 @@ __device__ __forceinline__ i4 load16(const int8_t *p, int64_t left, bool vec) {
     return i4{(int)v[0], (int)v[1], (int)v[2], (int)v[3]};
 }
 
-// Any strides and alignment: 64 rows of x by 64 rows of weights a workgroup, 32 x 32 a wave; a gated product's 64 are 32 of the
-// gate's and the same 32 of the other half's.
+// Any strides and alignment, and offsets past a tile's 32 bits: 64 rows of x by 64 rows of weights a workgroup, 32 x 32 a wave; a gated
+// product's 64 are 32 of the gate's and the same 32 of the other half's.
 template <class T, bool GATED>
 __global__ __launch_bounds__(256) void k_product8_any(Product a, int64_t tiles_n, bool vec) {
     constexpr int BK = 64, PITCH = BK + 16;
@@ -703,7 +703,7 @@ typedef Shape<64, 64, 128, 3> Small;
 typedef Shape<64, 64, 256, 4, true> Deep;
 typedef Shape<64, 128, 128, 5, true> DeepLow;
 
-enum Kernel { ONE, FEW, LARGE, MIDDLE, LOW, SMALL, DEEP, DEEP_LOW };
+enum Kernel { ONE, FEW, LARGE, MIDDLE, LOW, SMALL, DEEP, DEEP_LOW, ANY };
 
 template <class F>
 st_status with_shape(int kernel, F &&f) {
@@ -736,12 +736,19 @@ constexpr Rates RATES[] = {
     {DEEP, 64, 64, 256, 1, 5.23, 1.48, 0.51, 0.51, 5.58, 2.22, 0.263}, {DEEP_LOW, 64, 128, 128, 1, 3.13, 3.58, 0.427, 0.427, 4.41, 0, 0},
 };
 
-Plan plan_of(int64_t m, int64_t k, int64_t n, bool is_gated) {
+// A tile's offsets are 32 bits: rows of weights up to 256 on, and in a gated product n further.
+bool is_near(int64_t n, bool is_gated, int64_t x_stride, int64_t w_stride, int64_t out_stride) {
+    return x_stride < 1 << 23 && out_stride < 1 << 21 && w_stride < 1 << 24 && ((is_gated ? n : 0) + 256) * w_stride < ((int64_t)1 << 32) - (1 << 16);
+}
+
+// tiles_too: offsets are near enough for the kernels with tiles.
+Plan plan_of(int64_t m, int64_t k, int64_t n, bool is_gated, bool tiles_too) {
     const int64_t width = is_gated ? 2 * n : n, cus = st::device_cus();
     if (m <= 4 && k >= 512 && (m == 1 ? 1 : m == 2 ? 2 : 4) * k <= 64 * 1024) return Plan{ONE, 1};
-    Plan best = {LARGE, 1};
+    Plan best = {ANY, 1};
     double least = 1e300;
     for (const Rates &r : RATES) {
+        if (!tiles_too) break;
         const bool once = r.kernel == DEEP || r.kernel == DEEP_LOW, narrow = r.kernel == SMALL || r.kernel == DEEP, halves = r.kernel == LOW || r.kernel == DEEP_LOW;
         if (once != (m <= 64) || (halves && !is_gated)) continue;
         const int64_t stages = (k + r.bk - 1) / r.bk, tiles = (m + r.bm - 1) / r.bm * ((width + r.bn - 1) / r.bn);
@@ -763,6 +770,12 @@ Plan plan_of(int64_t m, int64_t k, int64_t n, bool is_gated) {
     return best;
 }
 
+// The plan of rows of codes as short as 16-byte alignment leaves them and of a contiguous out: no others are nearer.
+Plan plan_of(int64_t m, int64_t k, int64_t n, bool is_gated) {
+    const int64_t stride = (k + 15) & ~(int64_t)15;
+    return plan_of(m, k, n, is_gated, is_near(n, is_gated, stride, stride, n));
+}
+
 st_status product8(const char *name, const Product &a, int32_t dtype, bool is_gated, void *work, int64_t work_bytes, st_stream stream) {
     if (a.m < 0 || a.k <= 0 || a.n < 0 || a.k > 131072)
         return st::fail(ST_ERR_INVALID, "%s: m %lld, k %lld (1 to 131072), n %lld", name, (long long)a.m, (long long)a.k, (long long)a.n);
@@ -782,14 +795,14 @@ st_status product8(const char *name, const Product &a, int32_t dtype, bool is_ga
         return st::fail(ST_ERR_INVALID, "%s: a buffer is not aligned to its elements (work: 16 bytes)", name);
     if (!st::device_ok()) return ST_ERR_NO_DEVICE;
     const bool vec = (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 && (a.m == 1 || a.x_stride % 16 == 0) && (a.w_stride % 16 == 0 || (a.n == 1 && !is_gated));
-    const Plan plan = plan_of(a.m, a.k, a.n, is_gated);
+    const Plan plan = vec ? plan_of(a.m, a.k, a.n, is_gated, is_near(a.n, is_gated, a.x_stride, a.w_stride, a.out_stride)) : Plan{ANY, 1};
     return st::with_dtype(dtype, [&](auto *t) -> st_status {
         using T = std::remove_pointer_t<decltype(t)>;
         typedef std::integral_constant<int, 1> I1;
         typedef std::integral_constant<int, 2> I2;
         typedef std::integral_constant<int, 4> I4;
         typedef std::integral_constant<int, 8> I8;
-        if (vec && plan.kernel == ONE) {
+        if (plan.kernel == ONE) {
             const int rows = a.m == 1 ? 1 : a.m == 2 ? 2 : 4, lds = rows * (int)((a.k + 1023) / 1024 * 1024);
             auto go = [&](auto m_, auto r_, auto u_) {
                 constexpr int M = decltype(m_)::value, R = decltype(r_)::value, U = decltype(u_)::value;
@@ -817,7 +830,7 @@ st_status product8(const char *name, const Product &a, int32_t dtype, bool is_ga
             ST_LAUNCH_CHECK();
             return ST_OK;
         }
-        if (vec && plan.kernel == FEW) {
+        if (plan.kernel == FEW) {
             auto go = [&](auto kernel, int mb, int waves) {
                 kernel<<<dim3((uint32_t)((a.n + 15) / 16), (uint32_t)((a.m + 16 * mb - 1) / (16 * mb))), 64 * waves, 0, st::stream_of(stream)>>>(a);
             };
@@ -832,9 +845,7 @@ st_status product8(const char *name, const Product &a, int32_t dtype, bool is_ga
             ST_LAUNCH_CHECK();
             return ST_OK;
         }
-        // A tile's offsets are 32 bits: rows of weights up to 256 on, and in a gated product n further.
-        const bool near = a.x_stride < 1 << 23 && a.out_stride < 1 << 21 && ((is_gated ? a.n : 0) + 256) * a.w_stride < ((int64_t)1 << 32) - (1 << 16);
-        if (vec && near && plan.kernel >= LARGE) {
+        if (plan.kernel != ANY) {
             const int64_t width = is_gated ? 2 * a.n : a.n, need = plan.slices > 1 ? 4 * plan.slices * a.m * width : 0;
             if (need && (!work || work_bytes < need))
                 return st::fail(ST_ERR_INVALID, "%s: %lld bytes of work memory are needed, got %lld", name, (long long)need, (long long)(work ? work_bytes : 0));

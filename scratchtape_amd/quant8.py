@@ -94,12 +94,16 @@ def _product(name, x, x_scales, w, w_scales, bias, flag, halves, dtype, out, str
     return out
 
 
-KERNELS = ("one", "few", "large", "middle", "low", "small", "deep", "deep_low")
+KERNELS = ("one", "few", "large", "middle", "low", "small", "deep", "deep_low", "any")
 
 
 def product_plan(m: int, k: int, n: int, gated: bool = False) -> Tuple[str, int]:
-    """The kernel (of KERNELS) that matmul_8bit, or gated_8bit, takes for x [m, k] and n columns of out where rows are 16-byte
-    aligned, and into how many slices it cuts k.  Needs no device."""
+    """The kernel (of KERNELS) that matmul_8bit, or gated_8bit, takes for x [m, k] and n columns of out where codes lie as
+    quantize_8bit lays them and out is contiguous, and into how many slices it cuts k.  Needs no device.
+
+    Where a tile's offsets would not fit 32 bits (rows of out 2^21 elements or more apart, of x 2^23 bytes, 256 rows of w, gated
+    n + 256, over 2^32 - 2^16 bytes) no kernel with tiles is taken: "few" for up to 32 rows of x, else "any", which also takes all
+    codes that are not 16-byte aligned."""
     plan = (ctypes.c_int64 * 2)()
     _lib.call("st_matmul_8bit_plan", m, k, n, int(gated), plan)
     return KERNELS[plan[0]], plan[1]
