@@ -72,8 +72,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, fwd: LnOut, rows: int
 
 @dataclass
 class RmsOut:
-    """What rms_norm returns: h, the rows it normed (x + residual, or x itself); of y with rstd [rows] float32, for the
-    backward pass, and of codes, scales and values what was asked for."""
+    """What rms_norm returns: h, the rows it normed (x + residual, or x itself); of y, rstd [rows] float32 (with y, and for the
+    backward pass), codes, scales and values what was asked for."""
     h: torch.Tensor
     rstd: Optional[torch.Tensor] = None
     y: Optional[torch.Tensor] = None
@@ -101,13 +101,13 @@ def _norm_weight(weight: torch.Tensor, x: torch.Tensor) -> int:
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-5, y: bool = True,
-             eight_bit: bool = False, values: bool = False, stream=None) -> RmsOut:
+             eight_bit: bool = False, values: bool = False, stream=None, *, rstd: bool = False) -> RmsOut:
     """h = x + residual (x itself without one), rounded to x's type, and its norm h / sqrt(mean h^2 + eps) * weight per row of
     x [rows, d] (float32, float16 or bfloat16, any row stride); weight [d] is of x's type or float32.
 
     y: return the norm in x's type, and rstd with it.  eight_bit: return it as 8-bit rows for quant8's products, codes and scales, and with
     `values` also what those stand for in x's type.  The codes are those of the rows h * weight (1 / rms is a factor of a
-    row's scale)."""
+    row's scale).  rstd: return it without y too, for the backward pass of who trains through `values`."""
     dtype = _dtype(x, "x")
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"x is [rows, d] with d > 0, got {list(x.shape)}")
@@ -123,16 +123,17 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     _on_gpu(x, [(weight, "weight"), (residual, "residual")])
     with _launch(x.device, stream) as handle:
         h = x if residual is None else x.new_empty((n, d))
-        out = rstd = codes = scales = stood = None
+        out = codes = scales = stood = None
         if y:
-            out, rstd = x.new_empty((n, d)), x.new_empty((n,), dtype=torch.float32)
+            out = x.new_empty((n, d))
+        inverse = x.new_empty((n,), dtype=torch.float32) if y or rstd else None
         if eight_bit:
             codes, scales = _new_codes(n, d, x), x.new_empty((n,), dtype=torch.float32)
             stood = x.new_empty((n, d)) if values else None
         _lib.call("st_rms_norm", x.data_ptr(), _addr(residual), dtype, n, d, stride, r_stride, weight.data_ptr(), w_dtype, eps,
-                  0 if residual is None else h.data_ptr(), _addr(rstd), _addr(out), _addr(codes), (d + 15) // 16 * 16, _addr(scales),
+                  0 if residual is None else h.data_ptr(), _addr(inverse), _addr(out), _addr(codes), (d + 15) // 16 * 16, _addr(scales),
                   _addr(stood), handle)
-    return RmsOut(h, rstd, out, codes, scales, stood)
+    return RmsOut(h, inverse, out, codes, scales, stood)
 
 
 def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor, dh: Optional[torch.Tensor] = None,
