@@ -726,15 +726,15 @@ struct Plan {
 
 // Which kernel: the one whose time, in us, comes out least.  A workgroup takes `start`, and `unit` for each unit beside its stages, of
 // which one takes `alone`, or `shared` where two workgroups of a CU run at once; or its bytes come at `rate` (MB a us) and take longer; slices cost
-// their join, `join` and `each` of them, and the memory of their sums.  Fitted to both sides' times at 400 shapes, 17 to 96 % of them where a kernel is
-// not the fastest; the choice costs 1.1 % over the fastest on average (most: 384 x 4096 x 11003, 45 us instead of 34, a tile and a half
-// a CU).
+// their join, `join` and `each` of them, and the memory of their sums.  Fitted to the times of all kernels at 400 shapes, at 17 to 96 % of which a
+// given one is not the fastest (256 x 256 tiles at the 244 of more than 64 rows, in stages of 128 k as they are); the choice costs
+// 1.0 % over the fastest on average (0.6 % above 64 rows; most: 384 x 4096 x 11003, 45 us instead of 35, a tile and a half a CU).
 struct Rates {
     int kernel, bm, bn, bk, shared_by;
     double start, unit, alone, shared, rate, join, each;
 };
 constexpr Rates RATES[] = {
-    {LARGE, 256, 256, 128, 1, 1.25, 13.5, 1.338, 1.338, 2.26, 0, 0}, {MIDDLE, 128, 128, 64, 2, 4.37, 2.98, 0.307, 0.664, 3.62, 0, 0},
+    {LARGE, 256, 256, 128, 1, 3.49, 13.8, 1.351, 1.351, 2.28, 0, 0}, {MIDDLE, 128, 128, 64, 2, 4.37, 2.98, 0.307, 0.664, 3.62, 0, 0},
     {LOW, 64, 128, 64, 2, 3.13, 2.75, 0.264, 0.494, 8.4, 0, 0},    {SMALL, 64, 64, 128, 2, 3.95, 1.78, 0.307, 0.455, 3.44, 2.21, 0.446},
     {DEEP, 64, 64, 256, 1, 5.23, 1.48, 0.51, 0.51, 5.58, 2.22, 0.263}, {DEEP_LOW, 64, 128, 128, 1, 3.13, 3.58, 0.427, 0.427, 4.41, 0, 0},
 };
