@@ -7,9 +7,9 @@
 // squares are summed, and one pass over the row in registers finds both the sum and the maximum.  The quantiser is the same
 // kernel with t = x and rstd = 1.
 //
-// Squares and products t are taken in 64 bits (exact for f32 values: squares of 1e30 do not overflow, and t decides codes);
-// every output is rounded once.  A row lies in the registers of TPR threads, V vectors of eight elements each; wider rows
-// (V = 0) are read twice.
+// Squares and products t are taken in 64 bits (exact for f32 values: squares of 1e30 do not overflow, and t decides codes); outputs
+// are rounded to f32 and from there to their type (16-bit ones are off by half a step and 2^-24).  A row lies in the registers of TPR
+// threads, V vectors of eight elements each; wider rows (V = 0) are read twice.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -204,7 +204,7 @@ struct Back {
 // grow with the number of rows (chains of 64 rows in f32 are off by 1.5e-7, 4.4e-8 so; 32768 x 256 bf16 25 us, 24 with f32 sums); each
 // part is rounded to f32 once.  Where those sums leave too few registers, or room for one workgroup of a CU's two, the weights lie in LDS (us
 // so and in registers: 2000 x 16384 f32 114 and 131, 8000 x 1900 bf16 32 and 40; f32, which has one workgroup a CU, 64 and 61).
-// Bound by HBM: 16384 x 4096 bf16 with dh 110 us with the sum's launch, 4.9 TB/s; 4096 x 256 f32 11.6, latencies of rows one after the other.
+// Bound by HBM: 16384 x 4096 bf16 with dh 110 us with the sum's launch, 4.9 TB/s; 4096 x 256 f32 11.2, latencies of rows one after the other.
 template <class T, class W, int TPR, int V>
 __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
     constexpr int ROWS = threads_of(TPR) / TPR, WAVES = TPR / 64;
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_back(Back a) {
         for (int i = 0; i < 8; i++) w[i] = W_LDS ? w_lds[2 * v + i / 4][t][i % 4] : w_held[W_LDS ? 0 : v][i];
     };
     // A row's last vector, of 16-bit elements, as its last eight, moved to their places when all loads are on their way (us so and with
-    // load_eight: 8000 x 4003 bf16 70 and 107, 8000 x 1111 37 and 45, 16384 x 4096 114 and 114; f32 16384 x 4096 305 and 203).
+    // load_eight: 8000 x 4003 bf16 64 and 99, 8000 x 1111 26 and 30, 16384 x 4096 109 and 109; f32 16384 x 4096, another day, 305 and 203).
     constexpr bool LATE = sizeof(T) == 2;
     auto load = [&](const T *row, int v) {
         const int64_t at = (v * TPR + t) * 8;
@@ -391,8 +391,8 @@ dim3 sum_grid(int64_t d) {
 constexpr int64_t BACK_WIDEST = 16384;  // columns that a workgroup's registers hold
 
 // Row lanes of a workgroup of k_rms_back, and the parts that its launch leaves to be summed: two workgroups a CU, one where its rows keep
-// that busy (wide f32 rows, 1024 threads).  us with one and two: 4096 x 256 f32 12.7, 11.6, 8000 x 1900 62, 66, 16384 x 4096 204, 216;
-// bf16 32768 x 512 45, 32, 8000 x 1111 34, 37, 16384 x 2048 62, 54, 16384 x 4096 131, 114, 4096 x 8192 49, 53.
+// that busy (wide f32 rows, 1024 threads).  us with one and two: 4096 x 256 f32 12.2, 11.2, 8000 x 1900 61, 65, 16384 x 4096 188, 201;
+// bf16 32768 x 512 44, 31, 8000 x 1111 33, 25, 16384 x 2048 66, 56, 16384 x 4096 131, 108, 4096 x 8192 60, 64.
 int64_t back_rows(int64_t d) { return d <= 2048 ? 4 : 1; }
 int64_t back_parts(int64_t rows, int64_t d, int64_t size) {
     if (d > BACK_WIDEST) return std::min<int64_t>((rows + 31) / 32, 64);
