@@ -47,7 +47,7 @@ def test_the_bound_tells_chains_apart(t):
     assert off(chain.double().sum(0).float(), want) > 1.5 * BOUND
 
 
-# Every kernel of the backward, 64 rows and more a row lane (400 parts' rows for the widest)
+# Every kernel of the backward, 64 rows and more a row lane (for the widest 400 a part)
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", sorted(TYPES))
 @pytest.mark.parametrize("n,d", [(131072, 256), (131072, 511), (131072, 1000), (131072, 2000), (65536, 3000), (32768, 4096), (16384, 8000), (16384, 16000),
