@@ -210,7 +210,7 @@ struct Shape {
 // sums of an output.  Rows past the end repeat the last one and are not stored; x's bytes past k are zeros in LDS.
 //
 // 8192 x 8192 x 8192 to bf16: 445 to 480 us on several cards, 2,290 to 2,470 TOP/s, bound by the card's power (operands of zeros:
-// 3,140); 4095 x 4096 x 2 x 12288 with gelu 404 to 410 us; a tile's outputs take 8 us in which its products wait.  48 x 4096 x 11003 in tiles
+// 3,140); 4095 x 4096 x 2 x 12288 with gelu 402 to 410 us; a tile's outputs take 8 us in which its products wait.  48 x 4096 x 11003 in tiles
 // of 64 x 64: 14 us, 172 workgroups.
 template <class T, bool GATED, class Tiles>
 __global__ __launch_bounds__(256, std::min(Tiles::AT_ONCE, 4)) void k_product8(Product a, Units units) {
